@@ -154,6 +154,7 @@ def prepare(case, seed):
     gain = 0.4 + 1.2 * torch.rand(heads, hd, generator=g, device=dev)
     tokens = sum(n)
     state = {"case": case, "table": table, "tokens": tokens, "longest": max(n),
+             "longest_kv": max(kv),
              "kv_len": torch.tensor(kv, dtype=torch.int32, device=dev),
              "query_start": torch.tensor([sum(n[:b]) for b in range(len(n) + 1)],
                                          dtype=torch.int32, device=dev)}
@@ -271,7 +272,7 @@ def _attention(state):
     start, kv = state["query_start"].long(), state["kv_len"].long()
     n = start[1:] - start[:-1]
     # keys and values [B, heads, S, hd]
-    j = torch.arange(case["kv_max"], device=q.device)
+    j = torch.arange(state["longest_kv"], device=q.device)
     at = table[:, j // page].long().clamp(min=0)
     held = j < kv[:, None]
     k, v = (_values(state[c + "_cache"], state[c + "_scale"], at, (j % page).expand_as(at))
