@@ -38,6 +38,10 @@ TFX_DEV_TIMEOUT_OTHER = 5
 TFX_PATH_AUTO = 0
 TFX_PATH_CHAIN = 1
 
+TFX_CACHE_F16 = 0
+TFX_CACHE_INT8 = 1
+TFX_CACHE_E4M3 = 2
+
 TFX_EPI_BIAS = 0
 TFX_EPI_BIAS_GELU = 1
 TFX_EPI_BIAS_RESIDUAL = 2
@@ -65,6 +69,10 @@ SIGNATURES = {
     "tfx_forward_static": (_I, [_P, _P, _P, _I, _I, _P, _P]),
     "tfx_forward_kv_workspace_bytes": (_I64, [_P, _I, _I]),
     "tfx_forward_kv": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, ctypes.c_size_t, _P]),
+    "tfx_paged_append": (_I, [_P, _I64, _P, _I64, _P, _P, _P]),
+    "tfx_paged_read": (_I, [_P, _P, _P, _I64, _P, _I64, _P]),
+    "tfx_paged_attention_workspace_bytes": (_I64, [_P, _P, _I]),
+    "tfx_paged_attention": (_I, [_P, _I64, _P, _P, _P, _I64, _I, _F, _I, _P, ctypes.c_size_t, _P]),
     "tfx_read_device_error": (_I, [ctypes.POINTER(_I)]),
     "tfx_selftest_bounded_wait": (_I, [_I64, _P]),
 }
@@ -97,6 +105,41 @@ class TfxModel(ctypes.Structure):
         ("final_norm_weight", ctypes.c_void_p),
         ("final_norm_bias", ctypes.c_void_p),
         ("path", ctypes.c_int),
+    ]
+
+
+class TfxPagedCache(ctypes.Structure):
+    """Mirror of ``tfx_paged_cache`` (include/tfx.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("page_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class TfxPagedBatch(ctypes.Structure):
+    """Mirror of ``tfx_paged_batch`` (include/tfx.h)."""
+
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int),
+        ("query_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("batch", ctypes.c_int),
+        ("num_tokens", ctypes.c_int),
+        ("max_query_len", ctypes.c_int),
+        ("max_kv_len", ctypes.c_int),
     ]
 
 

@@ -1,0 +1,223 @@
+// tfx_paged_attention: host-side checks, the choice of kernel and of the split
+// over keys, and the kernel that joins the splits.
+#include "paged.cuh"
+
+namespace tfx {
+namespace {
+
+// Keys of a split: a multiple of every kernel's round of tiles over its warps.
+constexpr int kSplitKeys = 256;
+
+// out[row] = sum over splits of partial O scaled to the common maximum, over
+// the sum of their sums. `wpr` warps of the CTA per (token, head) row: one when
+// there are few splits (more rows per CTA), four when there are many.
+template <int HD>
+__global__ void __launch_bounds__(128)
+    paged_join_kernel(const __grid_constant__ Paged p, const __grid_constant__ PagedAttn a,
+                      int64_t rows, int wpr) {
+  grid_dep_wait();
+  grid_dep_launch();
+  constexpr int DL = HD >= 32 ? HD / 32 : 1;  // dims of a lane
+  __shared__ float sm[4][HD];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / wpr) + warp / wpr;
+  const int part = warp % wpr, heads = p.kv_heads * a.group;
+  int n = 0, tok = 0, head = 0;
+  if (row < rows) {
+    tok = static_cast<int>(row / heads);
+    head = static_cast<int>(row % heads);
+    const int b = paged_seq_of_row(p, tok);
+    if (b >= 0) {
+      const PagedSeq s = paged_seq(p, b);
+      if (paged_is_split(a, s) && tok >= s.row0 && tok < s.row0 + s.n) {
+        const int lim = a.causal ? min(s.len, max(0, s.pos0 + (tok - s.row0) + 1)) : s.len;
+        n = (lim + a.kps - 1) / a.kps;
+        if (n == 0) n = -1;  // a split sequence's row that sees no key
+      }
+    }
+  }
+  const int64_t base = row * a.splits;
+  float m = -INFINITY, acc[DL], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < DL; ++e) acc[e] = 0.f;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, a.part_ml[base + s].x);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  for (int s = 0; s < n; ++s) {
+    const float2 ml = a.part_ml[base + s];
+    const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - m);
+    if (f == 0.f && ml.y == 0.f) continue;
+    l += f * ml.y;
+    if (s % wpr != part) continue;
+    const float* src = a.part_o + (base + s) * HD + lane * DL;
+    if (HD >= 32 || lane < HD) {
+#pragma unroll
+      for (int e = 0; e < DL; ++e) acc[e] += f * src[e];
+    }
+  }
+  if (wpr > 1) {
+    if (HD >= 32 || lane < HD) {
+#pragma unroll
+      for (int e = 0; e < DL; ++e) sm[warp][lane * DL + e] = acc[e];
+    }
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+#pragma unroll
+      for (int e = 0; e < DL; ++e)
+        if (HD >= 32 || lane < HD) acc[e] += sm[w][lane * DL + e];
+  }
+  if (n == 0 || (HD < 32 && lane >= HD)) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __half* dst = a.out + static_cast<int64_t>(tok) * a.ld_out + head * HD + lane * DL;
+#pragma unroll
+  for (int e = 0; e < DL; ++e) dst[e] = __float2half_rn(acc[e] * inv);
+}
+
+template <int HD>
+int launch_join(const Paged& p, const PagedAttn& a, cudaStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_heads * a.group;
+  const int wpr = a.splits > 8 ? 4 : 1, per_cta = 4 / wpr;
+  launch_pdl(paged_join_kernel<HD>, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)),
+             dim3(128), 0, stream, p, a, rows, wpr);
+  return check_launch("paged_join_kernel");
+}
+
+int join_hd(const Paged& p, const PagedAttn& a, int head_dim, cudaStream_t stream) {
+  switch (head_dim) {
+    case 8: return launch_join<8>(p, a, stream);
+    case 16: return launch_join<16>(p, a, stream);
+    case 32: return launch_join<32>(p, a, stream);
+    case 64: return launch_join<64>(p, a, stream);
+    case 128: return launch_join<128>(p, a, stream);
+    default: return launch_join<256>(p, a, stream);
+  }
+}
+
+struct Plan {
+  int block_rows;
+  int64_t rows;  // of the longest sequence
+  int splits, kps;
+  int64_t ml_offset, bytes;  // workspace
+};
+
+// How the work is cut: row blocks, and ranges of keys where the blocks alone
+// leave SMs idle.
+Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) {
+  Plan pl{};
+  const int group = q_heads / c->kv_heads;
+  const int q = b->max_query_len < b->num_tokens ? b->max_query_len : b->num_tokens;
+  pl.rows = static_cast<int64_t>(q) * group;
+  pl.block_rows = paged_rows_block(c->head_dim, pl.rows);
+  const int64_t blocks = static_cast<int64_t>(b->batch) * c->kv_heads *
+                         ((pl.rows + pl.block_rows - 1) / pl.block_rows);
+  // About four waves of CTAs, three to an SM: long and short sequences even out.
+  const int64_t want = blocks > 0 ? (12LL * num_sms() + blocks - 1) / blocks : 1;
+  int64_t kv = static_cast<int64_t>(b->max_pages) * c->page_size;
+  if (b->max_kv_len < kv) kv = b->max_kv_len;
+  int64_t kps = want > 1 ? (kv + want - 1) / want : kv;
+  kps = (kps + kSplitKeys - 1) / kSplitKeys * kSplitKeys;
+  if (kps < kSplitKeys) kps = kSplitKeys;
+  pl.kps = static_cast<int>(kps);
+  pl.splits = static_cast<int>((kv + kps - 1) / kps);
+  if (pl.splits < 1) pl.splits = 1;
+  if (pl.splits > 1) {
+    const int64_t parts = static_cast<int64_t>(b->num_tokens) * q_heads * pl.splits;
+    pl.ml_offset = parts * c->head_dim;  // floats; head_dim is even: float2 stays aligned
+    pl.bytes = (parts * (c->head_dim + 2) * 4 + 255) / 256 * 256;
+  }
+  return pl;
+}
+
+int check_heads(const char* fn, const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) {
+  if (q_heads <= 0 || q_heads % c->kv_heads != 0)
+    return fail(TFX_ERR_INVALID_ARGUMENT, "%s: q_heads %d is not a multiple of kv_heads %d", fn,
+                q_heads, c->kv_heads);
+  if (static_cast<int64_t>(b->num_tokens) * q_heads > 0x7fffffffLL - 1024)
+    return fail(TFX_ERR_UNSUPPORTED, "%s: num_tokens * q_heads exceeds 2^31", fn);
+  return TFX_OK;
+}
+
+}  // namespace
+
+int paged_rows_block(int head_dim, int64_t rows) {
+  // Registers hold 64 rows up to head_dim 64, 32 at 128, 16 at 256.
+  const int most = head_dim <= 64 ? 64 : (head_dim == 128 ? 32 : 16);
+  const int need = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  return need < most ? need : most;
+}
+
+}  // namespace tfx
+
+using namespace tfx;
+
+extern "C" {
+
+int64_t tfx_paged_attention_workspace_bytes(const tfx_paged_cache* cache,
+                                            const tfx_paged_batch* batch, int q_heads) {
+  fail(TFX_OK, "%s", "");
+  const char* fn = "tfx_paged_attention_workspace_bytes";
+  Paged p;
+  if (check_paged(fn, cache, batch, &p) != TFX_OK ||
+      check_heads(fn, cache, batch, q_heads) != TFX_OK)
+    return -1;
+  return make_plan(cache, batch, q_heads).bytes;
+}
+
+int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* cache,
+                        const tfx_paged_batch* batch, tfx_half* out, int64_t ld_out, int q_heads,
+                        float scale, int causal, void* workspace, size_t workspace_bytes,
+                        tfx_stream_t stream_) {
+  fail(TFX_OK, "%s", "");
+  const char* fn = "tfx_paged_attention";
+  Paged p;
+  int st = check_paged(fn, cache, batch, &p);
+  if (st == TFX_OK) st = check_heads(fn, cache, batch, q_heads);
+  if (st != TFX_OK) return st;
+  if (q == nullptr || out == nullptr) return fail(TFX_ERR_INVALID_ARGUMENT, "%s: null tensor", fn);
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.f) || !(scale_log2 < INFINITY))
+    return fail(TFX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", fn);
+  const int64_t width = static_cast<int64_t>(q_heads) * cache->head_dim;
+  if (ld_q < width || ld_out < width)
+    return fail(TFX_ERR_INVALID_ARGUMENT, "%s: leading dimension smaller than q_heads*head_dim",
+                fn);
+  if (reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(out) % 16 ||
+      ld_q % 8 != 0 || ld_out % 8 != 0)
+    return fail(TFX_ERR_MISALIGNED,
+                "%s: pointers 16-byte aligned and leading dims multiples of 8 needed", fn);
+  const Plan pl = make_plan(cache, batch, q_heads);
+  if (pl.bytes > 0) {
+    if (workspace == nullptr) return fail(TFX_ERR_INVALID_ARGUMENT, "%s: null workspace", fn);
+    if (reinterpret_cast<uintptr_t>(workspace) % 256)
+      return fail(TFX_ERR_MISALIGNED, "%s: workspace 256-byte alignment", fn);
+    if (workspace_bytes < static_cast<size_t>(pl.bytes))
+      return fail(TFX_ERR_WORKSPACE, "%s: workspace %zu < required %lld bytes", fn,
+                  workspace_bytes, static_cast<long long>(pl.bytes));
+  }
+  if (pl.rows == 0) return TFX_OK;  // no new token
+  PagedAttn a{};
+  a.q = reinterpret_cast<const __half*>(q);
+  a.ld_q = ld_q;
+  a.out = reinterpret_cast<__half*>(out);
+  a.ld_out = ld_out;
+  a.group = q_heads / cache->kv_heads;
+  a.scale_log2 = scale_log2;
+  a.causal = causal != 0;
+  a.splits = pl.splits;
+  a.kps = pl.kps;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + pl.ml_offset);
+  const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  const int hd = cache->head_dim;
+  st = cache->dtype == TFX_CACHE_F16
+           ? launch_paged_rows<kCodeF16>(p, a, hd, pl.block_rows, pl.rows, stream)
+       : cache->dtype == TFX_CACHE_INT8
+           ? launch_paged_rows<kCodeI8>(p, a, hd, pl.block_rows, pl.rows, stream)
+           : launch_paged_rows<kCodeE4M3>(p, a, hd, pl.block_rows, pl.rows, stream);
+  if (st != TFX_OK || pl.splits == 1) return st;
+  return join_hd(p, a, hd, stream);
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
+from .paged import PagedBatch, PagedKVCache
 
 
 def _stream(device: torch.device) -> int:
@@ -233,6 +234,135 @@ def attention(
         ),
         "tfx_attention",
     )
+    return out
+
+
+def _packed_rows(t: torch.Tensor, what: str, tokens: int, heads: int, hd: int,
+                 device: torch.device) -> int:
+    """Checks a packed [T, heads, head_dim] fp16 tensor; its row stride in elements."""
+    if t.dtype != torch.float16 or t.shape != (tokens, heads, hd):
+        raise ValueError(f"{what} must be float16 [{tokens}, {heads}, {hd}]")
+    if t.device != device:
+        raise ValueError(f"{what} must be on the cache's device")
+    st = t.stride()
+    if st[2] != 1 or (heads > 1 and st[1] != hd):
+        raise ValueError(f"{what} must have contiguous heads (any row stride)")
+    return st[0] if tokens > 1 else heads * hd
+
+
+def _paged_stream(cache: PagedKVCache, batch: PagedBatch) -> int:
+    dev = cache.device
+    if dev.type != "cuda":
+        raise ValueError("the paged cache requires CUDA tensors")
+    if batch.device != dev:
+        raise ValueError("batch and cache must be on one device")
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _call_on(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args) with ``device`` as the current one (the library launches there)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.check(fn(*args), what)
+        return
+    with torch.cuda.device(device):
+        _lib.check(fn(*args), what)
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: PagedBatch) -> None:
+    """Write the batch's new keys and values into their pages.
+
+    k, v: fp16 [num_tokens, kv_heads, head_dim] with contiguous heads (slices of
+    the packed projection qualify). 8-bit caches quantise here, one scale per
+    token and head (max|x| / 127 or / 448): codes are those of exact
+    arithmetic, ties to even; a row of zeros gets scale 0, a row with an
+    infinity or NaN gets scale NaN and reads back as NaN. Tokens whose page is
+    outside the pool are dropped. Where two tokens of a batch share a slot, one
+    of them is kept. The paged form of the reference's ``_append_kv_cache``
+    (torch_transformer_benchmark.py:426-462).
+    """
+    stream = _paged_stream(cache, batch)
+    n, heads, hd = batch.num_tokens, cache.kv_heads, cache.head_dim
+    ld_k = _packed_rows(k, "k", n, heads, hd, cache.device)
+    ld_v = _packed_rows(v, "v", n, heads, hd, cache.device)
+    if n == 0:
+        return
+    _call_on(cache.device, "tfx_paged_append", _lib.load().tfx_paged_append, k.data_ptr(), ld_k,
+             v.data_ptr(), ld_v, cache._ref, batch._ref, stream)
+
+
+def paged_read(
+    cache: PagedKVCache,
+    batch: PagedBatch,
+    out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cached keys and values of the batch's tokens, fp16 [num_tokens, kv_heads, head_dim].
+
+    The same tokens that ``paged_append`` writes: the last ones of each
+    sequence, all of it where query_start counts kv_len tokens. 8-bit caches
+    give code * scale, rounded once. Tokens without a page read as zeros; rows
+    that belong to no sequence are not written. ``out``: write into these two.
+    """
+    stream = _paged_stream(cache, batch)
+    n, heads, hd = batch.num_tokens, cache.kv_heads, cache.head_dim
+    if out is None:
+        out = tuple(torch.empty((n, heads, hd), dtype=torch.float16, device=cache.device)
+                    for _ in range(2))
+    k, v = out
+    ld_k = _packed_rows(k, "out[0]", n, heads, hd, cache.device)
+    ld_v = _packed_rows(v, "out[1]", n, heads, hd, cache.device)
+    if n:
+        _call_on(cache.device, "tfx_paged_read", _lib.load().tfx_paged_read, cache._ref,
+                 batch._ref, k.data_ptr(), ld_k, v.data_ptr(), ld_v, stream)
+    return k, v
+
+
+def paged_attention(
+    q: torch.Tensor,
+    cache: PagedKVCache,
+    batch: PagedBatch,
+    is_causal: bool = True,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of the batch's new tokens over their sequences' cached ones.
+
+    q: fp16 [num_tokens, q_heads, head_dim] with contiguous heads; q_heads a
+    multiple of the cache's kv_heads (query head h reads key/value head
+    h // (q_heads // kv_heads)). The new tokens' own keys and values are in the
+    cache already (``paged_append``). ``is_causal``: a token sees the positions up
+    to its own; otherwise all of its sequence. ``scale`` (default
+    head_dim ** -0.5) is positive. Returns ctx [num_tokens, q_heads * head_dim]
+    fp16 (``out`` if given); a row that sees no key is zero, rows that belong to
+    no sequence are not written. Single tokens, drafts of a few and chunks of a
+    prompt may share a batch. The paged form of the cached attention of
+    torch_transformer_benchmark.py:747-765.
+    """
+    stream = _paged_stream(cache, batch)
+    n, hd = batch.num_tokens, cache.head_dim
+    if q.ndim != 3:
+        raise ValueError("q must be [num_tokens, q_heads, head_dim]")
+    heads = q.shape[1]
+    ld_q = _packed_rows(q, "q", n, heads, hd, cache.device)
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError(f"q_heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
+    if out is None:
+        out = torch.empty((n, heads * hd), dtype=torch.float16, device=cache.device)
+    elif out.shape != (n, heads * hd) or out.dtype != torch.float16 or \
+            out.device != cache.device or (n > 0 and out.stride(1) != 1):
+        raise ValueError("out must be float16 [num_tokens, q_heads * head_dim] with contiguous rows")
+    if n == 0:
+        return out
+    lib = _lib.load()
+    need = lib.tfx_paged_attention_workspace_bytes(cache._ref, batch._ref, heads)
+    if need < 0:
+        raise ValueError("tfx_paged_attention: " + lib.tfx_last_error_message().decode())
+    # A workspace of its own for each call, from the stream's allocator: calls on
+    # different streams, and graphs captured apart, never share one.
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    _call_on(cache.device, "tfx_paged_attention", lib.tfx_paged_attention, q.data_ptr(), ld_q,
+             cache._ref, batch._ref, out.data_ptr(), out.stride(0) if n > 1 else heads * hd, heads,
+             hd ** -0.5 if scale is None else float(scale), int(is_causal),
+             ws.data_ptr() if need else None, need, stream)
     return out
 
 

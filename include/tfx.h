@@ -270,6 +270,119 @@ TFX_API int tfx_forward_kv(const tfx_model* model, const float* x, float* y, int
                            tfx_stream_t stream);
 
 /*
+ * ------------------------------------------------------------ paged KV cache
+ * Keys and values of many sequences in one pool of pages, for batches whose
+ * sequences differ in length (the contiguous caches of tfx_forward_kv hold
+ * sequences of one length). Three operators share the cache and the batch:
+ * tfx_paged_append writes the new tokens, tfx_paged_read reads the same tokens
+ * back, tfx_paged_attention lets them attend everything cached. No counterpart
+ * in the reference, whose cache is contiguous fp16
+ * (torch_transformer_benchmark.py:409-462).
+ */
+
+/* What a cache holds. The 8-bit types have one fp32 scale for each token and
+ * head, of K and of V: value = code * scale. */
+typedef enum tfx_cache_dtype {
+  TFX_CACHE_F16 = 0,
+  TFX_CACHE_INT8 = 1, /* codes -127..127, scale = max|x| / 127          */
+  TFX_CACHE_E4M3 = 2  /* 8-bit floats (448 at most), scale = max|x| / 448 */
+} tfx_cache_dtype;
+
+/*
+ * The pool. Element e of head h of the token in slot t of page p is at
+ * k[p*page_stride + t*token_stride + h*head_stride + e] (in elements of the
+ * dtype; the same strides for v), so a page may hold its tokens head by head
+ * or its heads token by token. Scales (8-bit types; NULL for fp16):
+ * k_scale[(p*kv_heads + h)*page_size + t].
+ * page_size: 16, 32, 64, 128 or 256; head_dim: 8, 16, 32, 64, 128 or 256 (8-bit
+ * types: 16 and up); k and v 16-byte aligned, each stride a multiple of 16
+ * bytes and at least head_dim.
+ */
+typedef struct tfx_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int dtype; /* tfx_cache_dtype */
+  int num_pages;
+  int page_size;
+  int kv_heads;
+  int head_dim;
+  int64_t page_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+} tfx_paged_cache;
+
+/*
+ * A batch of sequences with their new tokens packed one behind the other:
+ * sequence b owns rows query_start[b] .. query_start[b+1] - 1 of the packed
+ * tensors, which are its LAST tokens, at positions kv_len[b] - n .. kv_len[b] - 1
+ * (n rows; kv_len counts the new tokens). The token at position p lives in
+ * slot p % page_size of page page_table[b*table_stride + p / page_size].
+ * Device arrays, read by the kernels when they run: a captured graph sees
+ * their contents at each replay. Values out of range are never followed: a page
+ * id outside [0, num_pages) is a page without tokens (writes to it are dropped,
+ * its keys are masked, reads give zeros), lengths and starts are clamped to
+ * the table's width and to num_tokens. Rows that no sequence owns are left as
+ * they are. Two sequences may share pages that neither writes.
+ */
+typedef struct tfx_paged_batch {
+  const int32_t* page_table;  /* [batch][max_pages], row pitch table_stride */
+  int64_t table_stride;
+  int max_pages;              /* max_pages * page_size <= 2^30 */
+  const int32_t* query_start; /* [batch + 1], from 0 up */
+  const int32_t* kv_len;      /* [batch] */
+  int batch;                  /* <= 65535 */
+  int num_tokens;             /* rows of the packed tensors */
+  int max_query_len;          /* no sequence has more new tokens (further ones stay unattended) */
+  int max_kv_len;             /* the longest kv_len, or a bound: sizes the split over keys only */
+} tfx_paged_batch;
+
+/*
+ * Writes k and v of the batch's new tokens into their slots, quantised in the
+ * 8-bit types: per token and head scale = max|x| / 127 (or / 448) in fp32 and
+ * code = x / scale rounded to nearest, ties to even, as if computed exactly;
+ * a row of zeros has scale 0, a row with an infinity or NaN has scale NaN (it
+ * reads back as NaN) and codes 0.
+ * k, v: fp16, element (row, h, e) at k[row*ld_k + h*head_dim + e]; 16-byte
+ * aligned, ld a multiple of 8.
+ */
+TFX_API int tfx_paged_append(const tfx_half* k, int64_t ld_k, const tfx_half* v, int64_t ld_v,
+                             const tfx_paged_cache* cache, const tfx_paged_batch* batch,
+                             tfx_stream_t stream);
+
+/*
+ * Reads k and v of the same tokens (the last n of each sequence: the whole
+ * sequence where n = kv_len) into fp16 rows laid out as tfx_paged_append's.
+ * Tokens without a page, and positions before 0, read as zeros.
+ */
+TFX_API int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* batch,
+                           tfx_half* k_out, int64_t ld_k, tfx_half* v_out, int64_t ld_v,
+                           tfx_stream_t stream);
+
+/*
+ * softmax(q . K^T * scale [+ causal mask]) . V of the batch's new tokens over
+ * their sequences' cached ones. Query head h reads key/value head
+ * h / (q_heads / kv_heads). causal: the token at position p sees positions
+ * 0..p; otherwise all kv_len of its sequence. A key that a query does not see
+ * has no part in its row, whatever its cached values are (NaN included); a
+ * row that sees no key is zero.
+ * q, out: fp16, element (row, h, e) at q[row*ld_q + h*head_dim + e], 16-byte
+ * aligned, ld a multiple of 8; scale > 0 and finite. q_heads is a multiple of
+ * cache->kv_heads. The new tokens' keys and values must be in the cache
+ * (tfx_paged_append before, on the same stream).
+ * workspace: tfx_paged_attention_workspace_bytes() of the same arguments (0:
+ * may be NULL), 256-byte aligned, for partial results of keys split over
+ * CTAs; calls that may overlap need one each.
+ */
+TFX_API int64_t tfx_paged_attention_workspace_bytes(const tfx_paged_cache* cache,
+                                                    const tfx_paged_batch* batch, int q_heads);
+TFX_API int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* cache,
+                                const tfx_paged_batch* batch, tfx_half* out, int64_t ld_out,
+                                int q_heads, float scale, int causal, void* workspace,
+                                size_t workspace_bytes, tfx_stream_t stream);
+
+/*
  * Reads and clears the calling device's kernel error word (synchronises the
  * device). *code receives 0 or a timeout code; returns TFX_OK or TFX_ERR_CUDA.
  * No reference counterpart (the reference's kernels have no waits).
