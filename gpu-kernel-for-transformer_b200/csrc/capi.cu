@@ -118,6 +118,28 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
   return TFX_OK;
 }
 
+int make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank,
+              const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+              CUtensorMapSwizzle swizzle) {
+  if (int st = resolve_encode()) return st;
+  cuuint64_t d[5], sb[4];
+  cuuint32_t bx[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    bx[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) sb[i] = strides[i];
+  }
+  const CUresult r = g_encode(map, dtype, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d,
+                              sb, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(TFX_ERR_CUDA, "cuTensorMapEncodeTiled (%d-D) failed (%d)", rank,
+                static_cast<int>(r));
+  return TFX_OK;
+}
+
 int make_tmap_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t batch, uint64_t cols,
                  uint64_t ld, uint64_t batch_stride, uint32_t box_cols, uint32_t box_rows) {
   if (int st = resolve_encode()) return st;

@@ -65,6 +65,12 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, 
 int make_tmap_3d(CUtensorMap* map, const void* base, uint64_t rows, uint64_t batch, uint64_t cols,
                  uint64_t ld, uint64_t batch_stride, uint32_t box_cols, uint32_t box_rows);
 
+// A row-major view of `rank` (2 to 5) dimensions, innermost first: sizes in
+// elements, strides of dimensions 1.. in bytes (multiples of 16).
+int make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, int rank,
+              const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+              CUtensorMapSwizzle swizzle);
+
 // Which keys of each sequence attention may use, and which output rows are
 // real tokens: all of them (both null), a prefix per sequence (len: [batch]
 // int32 valid lengths), or any pattern (bits: [batch][key_words(seq)] uint32,

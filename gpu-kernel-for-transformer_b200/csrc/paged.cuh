@@ -109,6 +109,22 @@ __device__ __forceinline__ bool h2_not_finite(uint32_t w) {
   return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
 }
 
+// Clears the halves that are infinities or NaN; true if there was one.
+__device__ __forceinline__ bool h2_clear(uint32_t& w) {
+  if (!h2_not_finite(w)) return false;
+  if ((w & 0x7c00u) == 0x7c00u) w &= 0xffff0000u;
+  if ((w & 0x7c000000u) == 0x7c000000u) w &= 0xffffu;
+  return true;
+}
+
+// Four elements of a row over the sum of its weights; no key seen: zeros (a
+// sum that is NaN stays).
+__device__ __forceinline__ void store_row4(__half* dst, float4 x, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(dst) =
+      make_uint2(pack_half2(x.x * inv, x.y * inv), pack_half2(x.z * inv, x.w * inv));
+}
+
 // One cached value (fp16 bits for kCodeF16, else a code and its scale).
 template <int CODE>
 __device__ __forceinline__ float paged_value(const void* base, int64_t at, float scale) {
@@ -119,10 +135,12 @@ __device__ __forceinline__ float paged_value(const void* base, int64_t at, float
 }
 
 // ------------------------------------------------------------- attention
-// One attention call as its kernels take it. `splits` CTAs share the keys of a
-// row block, kps keys each (a multiple of 256); with splits > 1 their
-// unnormalised results go to part_o [token][q_head][split][head_dim] with the
-// running (max, sum) in part_ml, and a second kernel joins them.
+// One attention call as its kernels take it. Sequences with more than
+// tc_rows rows (new tokens x group) belong to the tcgen05 kernel, the others to
+// the mma.sync kernel. `splits` CTAs share the keys of a row block, kps (or
+// kps_tc) keys each, a multiple of 256; with splits > 1 their unnormalised
+// results go to part_o [token][q_head][split][head_dim] with the (max, sum) in
+// part_ml, and a third kernel joins them.
 struct PagedAttn {
   const __half* q;
   int64_t ld_q;
@@ -131,15 +149,25 @@ struct PagedAttn {
   int group;  // query heads per key/value head
   float scale_log2;
   int causal;
-  int splits, kps;
+  int tc_rows;
+  int splits, kps, kps_tc;
+  int cluster;  // mma.sync kernel: CTAs of a cluster that share a row block's keys; 0: splits
   float* part_o;
   float2* part_ml;
 };
 
+__device__ __forceinline__ bool paged_is_tc(const PagedAttn& a, const PagedSeq& s) {
+  return s.n * a.group > a.tc_rows;  // below 2^31: checked on the host
+}
+
+__device__ __forceinline__ int paged_split_keys(const PagedAttn& a, const PagedSeq& s) {
+  return paged_is_tc(a, s) ? a.kps_tc : a.kps;
+}
+
 // Keys are split for this sequence (its partial results are joined later);
 // otherwise split 0 holds all of them and writes the rows itself.
 __device__ __forceinline__ bool paged_is_split(const PagedAttn& a, const PagedSeq& s) {
-  return a.splits > 1 && s.len > a.kps;
+  return a.splits > 1 && s.len > paged_split_keys(a, s);
 }
 
 // Rows of a CTA of the mma.sync kernel for rows = max_query_len * group.
@@ -147,5 +175,9 @@ int paged_rows_block(int head_dim, int64_t rows);
 template <int CODE>
 int launch_paged_rows(const Paged& p, const PagedAttn& a, int head_dim, int block_rows,
                       int64_t rows, cudaStream_t stream);
+// tokens: max_query_len.
+template <int CODE>
+int launch_paged_tc(const tfx_paged_cache* cache, const Paged& p, const PagedAttn& a,
+                    int64_t tokens, cudaStream_t stream);
 
 }  // namespace tfx

@@ -7,6 +7,9 @@ namespace {
 
 // Keys of a split: a multiple of every kernel's round of tiles over its warps.
 constexpr int kSplitKeys = 256;
+// Sequences with more rows (new tokens x query heads per key/value head) go to
+// the tcgen05 kernel, whose tiles have 128.
+constexpr int kTcRows = 64;
 
 // out[row] = sum over splits of partial O scaled to the common maximum, over
 // the sum of their sums. `wpr` warps of the CTA per (token, head) row: one when
@@ -31,7 +34,7 @@ __global__ void __launch_bounds__(128)
       const PagedSeq s = paged_seq(p, b);
       if (paged_is_split(a, s) && tok >= s.row0 && tok < s.row0 + s.n) {
         const int lim = a.causal ? min(s.len, max(0, s.pos0 + (tok - s.row0) + 1)) : s.len;
-        n = (lim + a.kps - 1) / a.kps;
+        n = (lim + paged_split_keys(a, s) - 1) / paged_split_keys(a, s);
         if (n == 0) n = -1;  // a split sequence's row that sees no key
       }
     }
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(128)
 template <int HD>
 int launch_join(const Paged& p, const PagedAttn& a, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_heads * a.group;
-  const int wpr = a.splits > 8 ? 4 : 1, per_cta = 4 / wpr;
+  const int wpr = a.splits > 16 ? 4 : 1, per_cta = 4 / wpr;
   launch_pdl(paged_join_kernel<HD>, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)),
              dim3(128), 0, stream, p, a, rows, wpr);
   return check_launch("paged_join_kernel");
@@ -96,38 +99,101 @@ int join_hd(const Paged& p, const PagedAttn& a, int head_dim, cudaStream_t strea
 }
 
 struct Plan {
-  int block_rows;
-  int64_t rows;  // of the longest sequence
-  int splits, kps;
+  int64_t q, rows;  // new tokens of the longest sequence, and their rows
+  int block_rows;   // of the mma.sync kernel
+  int tc_rows;      // sequences with more rows go to the tcgen05 kernel
+  bool tc, small;   // which kernels run
+  int splits, kps, kps_tc, cluster;
   int64_t ml_offset, bytes;  // workspace
 };
 
-// How the work is cut: row blocks, and ranges of keys where the blocks alone
-// leave SMs idle.
+// Into how many ranges the keys of `blocks` row blocks are cut, for `slots`
+// CTAs at a time, each of which costs `start` keys besides its own; `most`
+// ranges at most, of `least` keys at least. Sequences are taken to have any
+// length up to kv: the work per slot, and behind it the longest range (alone,
+// where all CTAs run at once).
+int64_t cut(int64_t blocks, int64_t slots, int64_t kv, int64_t start, int64_t least, int64_t most,
+            double* cost) {
+  int64_t best = 1;
+  *cost = 0.;
+  for (int64_t n = 1; n <= most; n += n < 8 ? 1 : n / 4) {
+    const int64_t keys = (kv + n - 1) / n;
+    if (n > 1 && keys < least) break;
+    const double waves = static_cast<double>(blocks) * n / slots;
+    const double c = waves <= 1. ? keys + start : 0.55 * waves * keys + waves * start + keys;
+    if (n == 1 || c < *cost) {
+      best = n;
+      *cost = c;
+    }
+  }
+  return best;
+}
+
+int round_keys(int64_t kv, int64_t parts) {
+  const int64_t keys = (kv + parts - 1) / parts;
+  return static_cast<int>((keys + kSplitKeys - 1) / kSplitKeys * kSplitKeys);
+}
+
+// How the work is cut: which kernel, row blocks, and ranges of keys where the
+// blocks alone leave SMs idle.
 Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) {
   Plan pl{};
-  const int group = q_heads / c->kv_heads;
-  const int q = b->max_query_len < b->num_tokens ? b->max_query_len : b->num_tokens;
-  pl.rows = static_cast<int64_t>(q) * group;
-  pl.block_rows = paged_rows_block(c->head_dim, pl.rows);
-  const int64_t blocks = static_cast<int64_t>(b->batch) * c->kv_heads *
-                         ((pl.rows + pl.block_rows - 1) / pl.block_rows);
-  // About four waves of CTAs, three to an SM: long and short sequences even out.
-  const int64_t want = blocks > 0 ? (12LL * num_sms() + blocks - 1) / blocks : 1;
+  const int group = q_heads / c->kv_heads, hd = c->head_dim;
+  pl.q = b->max_query_len < b->num_tokens ? b->max_query_len : b->num_tokens;
+  pl.rows = pl.q * group;
+  pl.tc_rows = 0x7fffffff;
+  if ((hd == 64 || hd == 128) && group <= 128) pl.tc_rows = kTcRows;
+  pl.tc = pl.rows > pl.tc_rows;
+  pl.small = !pl.tc || b->batch > 1;  // a single sequence has all the rows
+  if (!pl.tc) pl.tc_rows = 0x7fffffff;
+  if (!pl.small) pl.tc_rows = 0;
+  const int64_t small_rows = pl.rows < pl.tc_rows ? pl.rows : pl.tc_rows;
+  pl.block_rows = paged_rows_block(hd, small_rows);
+  const int64_t pairs = static_cast<int64_t>(b->batch) * c->kv_heads;
   int64_t kv = static_cast<int64_t>(b->max_pages) * c->page_size;
   if (b->max_kv_len < kv) kv = b->max_kv_len;
-  int64_t kps = want > 1 ? (kv + want - 1) / want : kv;
-  kps = (kps + kSplitKeys - 1) / kSplitKeys * kSplitKeys;
-  if (kps < kSplitKeys) kps = kSplitKeys;
-  pl.kps = static_cast<int>(kps);
-  pl.splits = static_cast<int>((kv + kps - 1) / kps);
-  if (pl.splits < 1) pl.splits = 1;
+  if (kv < 1) kv = 1;
+  // mma.sync: four CTAs to an SM (one at 512-byte rows); a start costs about
+  // as much as 400 keys, a second launch to join as much as 512.
+  const int64_t slots = num_sms() * (hd * (c->dtype == TFX_CACHE_F16 ? 2 : 1) >= 512 ? 1 : 4);
+  const int64_t blocks = pairs * ((small_rows + pl.block_rows - 1) / pl.block_rows);
+  double alone = 0., joined = 0.;
+  const int64_t share = cut(blocks, slots, kv, 400, 128, 8, &alone);
+  // (beside the tcgen05 kernel few splits: its many rows are joined by the same kernel)
+  const int64_t parts = cut(blocks, slots, kv, 400, kSplitKeys, pl.tc ? 8 : 1024, &joined);
+  if (!pl.tc && alone <= joined + 512.) {
+    pl.cluster = share > 1 ? static_cast<int>(share) : 0;
+    pl.kps = round_keys(kv, 1);
+  } else {
+    pl.kps = round_keys(kv, parts);
+  }
+  // tcgen05: one CTA to an SM; a start and the partial results of its 256 rows
+  // cost about as much as 6 tiles of 128 keys.
+  const int tokens = group <= 128 ? 2 * (128 / group) : 1;
+  double cost = 0.;
+  pl.kps_tc = round_keys(
+      kv, cut(pairs * ((pl.q + tokens - 1) / tokens), num_sms(), kv, 768, 1024, 16, &cost));
+  int64_t least = pl.tc ? pl.kps_tc : pl.kps;
+  if (pl.small && pl.kps < least) least = pl.kps;
+  pl.splits = static_cast<int>((kv + least - 1) / least);
+  if (pl.cluster > 0) pl.splits = 1;
   if (pl.splits > 1) {
-    const int64_t parts = static_cast<int64_t>(b->num_tokens) * q_heads * pl.splits;
-    pl.ml_offset = parts * c->head_dim;  // floats; head_dim is even: float2 stays aligned
-    pl.bytes = (parts * (c->head_dim + 2) * 4 + 255) / 256 * 256;
+    const int64_t part_rows = static_cast<int64_t>(b->num_tokens) * q_heads * pl.splits;
+    pl.ml_offset = part_rows * hd;  // floats; head_dim is even: float2 stays aligned
+    pl.bytes = (part_rows * (hd + 2) * 4 + 255) / 256 * 256;
   }
   return pl;
+}
+
+template <int CODE>
+int launch_attention_code(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a,
+                          const Plan& pl, cudaStream_t stream) {
+  int st = TFX_OK;
+  if (pl.tc) st = launch_paged_tc<CODE>(c, p, a, pl.q, stream);
+  if (st == TFX_OK && pl.small)
+    st = launch_paged_rows<CODE>(p, a, c->head_dim, pl.block_rows,
+                                 pl.rows < pl.tc_rows ? pl.rows : pl.tc_rows, stream);
+  return st;
 }
 
 int check_heads(const char* fn, const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) {
@@ -144,7 +210,7 @@ int check_heads(const char* fn, const tfx_paged_cache* c, const tfx_paged_batch*
 int paged_rows_block(int head_dim, int64_t rows) {
   // Registers hold 64 rows up to head_dim 64, 32 at 128, 16 at 256.
   const int most = head_dim <= 64 ? 64 : (head_dim == 128 ? 32 : 16);
-  const int need = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  const int need = rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 64));
   return need < most ? need : most;
 }
 
@@ -207,17 +273,19 @@ int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* 
   a.causal = causal != 0;
   a.splits = pl.splits;
   a.kps = pl.kps;
+  a.kps_tc = pl.kps_tc;
+  a.tc_rows = pl.tc_rows;
+  a.cluster = pl.cluster;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + pl.ml_offset);
   const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-  const int hd = cache->head_dim;
-  st = cache->dtype == TFX_CACHE_F16
-           ? launch_paged_rows<kCodeF16>(p, a, hd, pl.block_rows, pl.rows, stream)
-       : cache->dtype == TFX_CACHE_INT8
-           ? launch_paged_rows<kCodeI8>(p, a, hd, pl.block_rows, pl.rows, stream)
-           : launch_paged_rows<kCodeE4M3>(p, a, hd, pl.block_rows, pl.rows, stream);
+  switch (cache->dtype) {
+    case TFX_CACHE_F16: st = launch_attention_code<kCodeF16>(cache, p, a, pl, stream); break;
+    case TFX_CACHE_INT8: st = launch_attention_code<kCodeI8>(cache, p, a, pl, stream); break;
+    default: st = launch_attention_code<kCodeE4M3>(cache, p, a, pl, stream); break;
+  }
   if (st != TFX_OK || pl.splits == 1) return st;
-  return join_hd(p, a, hd, stream);
+  return join_hd(p, a, cache->head_dim, stream);
 }
 
 }  // extern "C"

@@ -4,26 +4,37 @@
 //
 // Rows: the `group` query heads that read one key/value head are rows of the
 // same block (row = token * group + head in group), so a cached key is read
-// once for all of them. A CTA takes 16 * MT rows of one (sequence, key/value
-// head) and one range of its keys. Its 4 warps take the range's KT-key tiles
-// in turn, each with a ring of NS tiles of its own in shared memory (cp.async,
+// once for all of them. A CTA takes 8 * NT rows of one (sequence, key/value
+// head) and one range of its keys. Its warps take the range's KT-key tiles in
+// turn, each with a ring of two tiles of its own in shared memory (cp.async,
 // no barrier between warps) and its own running maximum and sum per row; they
 // are merged through shared memory at the end.
 //
+// Keys are the products' M: S^T = K Q^T and O^T = V^T P^T, 16 keys (or dims) by
+// 8 rows at a time, so that a single row wastes 7 columns and not 15 rows, and
+// a cached value is expanded once for all rows. Bound by instructions, not
+// by the tensor cores; against rows as M: half the products, scores and
+// accumulators per key at up to 8 rows. P^T comes out of the first product with
+// keys along lanes and goes into the second with keys along k: movmatrix.
+//
+// The running maximum moves only when a score exceeds it by more than 2^8
+// (weights stay below 2^8, fine in fp16), so that most tiles need neither the
+// maximum over lanes nor a rescaled accumulator, only a vote.
+//
 // 8-bit caches are expanded to fp16 in registers, between ldmatrix and the
-// product, without the scales: a key's scale multiplies its column of scores,
-// a value's scale its column of weights, both in fp32. Weights are rounded to
-// fp16 for the second product; so that w * scale neither overflows nor loses
-// bits for scales far from 1, it is divided by the largest scale seen so far
-// (U, the accumulator's unit), which is put back at the end.
+// product, without the scales: a key's scale multiplies its row of scores, a
+// value's scale its row of weights, both in fp32. Weights are rounded to fp16
+// for the second product; so that w * scale neither overflows nor loses bits
+// for scales far from 1, it is divided by a unit U, the largest scale of an
+// earlier tile or at least 1/16 of the largest so far, which is put back at
+// the end.
 //
 // Fragment orders. An 8x8 ldmatrix block of 16-bit words holds 8 keys x 16
 // codes. Scores: thread (g, t) gets codes 4t..4t+3 of key g and uses (4t, 4t+1)
-// and (4t+2, 4t+3) as the B operand's k pairs; the sum over k does not depend
-// on the order as long as Q's fragments take the same one. Second product,
-// transposed load: the thread gets dims 2g and 2g+1 of keys 2t and 2t+1; the
-// even dims make one 8-wide column block of the product, the odd dims another,
-// and the thread ends up with dims 4t..4t+3 of each 16.
+// and (4t+2, 4t+3) as the k pairs; the sum over k does not depend on the order,
+// and Q is stored in the same one. Second product, transposed load: the thread
+// gets dims 2g and 2g+1 of keys 2t and 2t+1; the even dims are rows 0-7 of the
+// product, the odd dims rows 8-15.
 //
 // Masked keys. A weight of 0 does not hide an infinity or NaN among the values
 // (0 * inf), so values beyond the sequence are loaded as zeros, and in tiles
@@ -31,15 +42,17 @@
 // (NaN codes) are cleared before the product and added at the end to the rows
 // that see them. (A scale that is not finite stays in its row: it multiplies
 // weights, which are 0 where masked.)
+//
+// Keys over CTAs: either ranges of kps keys whose unnormalised results a second
+// kernel joins, or, where 8 ranges are enough, a cluster of CTAs with equal
+// shares that reads each other's results from shared memory: one launch and
+// no workspace.
 #pragma once
 
 #include "paged.cuh"
 
 namespace tfx {
 namespace {
-
-constexpr int kRowsWarps = 4;
-constexpr int kRowsThreads = 32 * kRowsWarps;
 
 __device__ __forceinline__ void rows_cp16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;  // zero-fill where there is no key
@@ -66,9 +79,19 @@ __device__ __forceinline__ void rows_ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ void rows_ldsm2(uint32_t addr, uint32_t& r0, uint32_t& r1) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];"
+               : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
+}
 __device__ __forceinline__ void rows_ldsm2_t(uint32_t addr, uint32_t& r0, uint32_t& r1) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
                : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
+}
+// Transposes an 8x8 block of 16-bit words held two to a lane.
+__device__ __forceinline__ uint32_t rows_movm_t(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
 }
 // D(16x8, f32) += A(16x16, f16, row) * B(16x8, f16, col)
 __device__ __forceinline__ void rows_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -79,9 +102,28 @@ __device__ __forceinline__ void rows_mma(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float4 rows_peer4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 rows_peer2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr)
+               : "memory");
+  return v;
+}
 
-template <int CODE, int HD, int MT>
+constexpr float kRowsRescale = 8.0f;  // log2 units, see the file's comment
+constexpr float kRowsUnit = 16.0f;
+
+template <int CODE, int HD, int NT>
 struct RowsCfg {
+  static constexpr int kRows = 8 * NT;
+  // One CTA to an SM at 512-byte rows: more warps in it.
+  static constexpr int kWarps = HD * code_bytes(CODE) >= 512 ? 6 : 4;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kHDP = HD < 16 ? 16 : HD;  // width of the first product (zero padded)
   static constexpr int kRowBytes = HD * code_bytes(CODE);
   static constexpr int kU = kRowBytes / 16;  // 16-byte chunks of a cached row
@@ -89,39 +131,46 @@ struct RowsCfg {
   static constexpr int kPitch = ((kHDP * code_bytes(CODE) / 16) | 1) * 16;
   static constexpr int kQPitch = (kHDP + 8) * 2;
   // Keys of a warp's tile: about 2 KB of K (small tiles keep more warps on an
-  // SM), at most 64 / MT (registers: the scores), at least what one x4
-  // ldmatrix of codes covers.
+  // SM), at most 64, and 128 scores to a column of lanes (registers).
+  static constexpr int kMost = 128 / NT < 64 ? 128 / NT : 64;
   static constexpr int kWant = 2048 / kRowBytes < 16 ? 16 : 2048 / kRowBytes;
-  static constexpr int kMost = 64 / MT;
-  static constexpr int kLeast = (CODE != kCodeF16 && HD == 16) ? 32 : 16;
-  static constexpr int kKT0 = kWant < kMost ? kWant : kMost;
-  static constexpr int kKT = kKT0 < kLeast ? kLeast : kKT0;
-  static constexpr int NS = 3;
+  static constexpr int kKT = kWant < kMost ? kWant : kMost;
+  static constexpr int NS = 2;
   static constexpr int kTileBytes = kKT * kPitch;
   static constexpr int kScaleBytes = CODE == kCodeF16 ? 0 : 2 * kKT * 4;
   // K, V, their scales, the bits of keys that exist
   static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes + 16;
-  static constexpr int kQBytes = 16 * MT * kQPitch;
-  static constexpr int kRing = kRowsWarps * NS * kStageBytes;
-  static constexpr int kMerge = kRowsWarps * 16 * (HD + 4) * 4;  // one 16-row block at a time
+  static constexpr int kQBytes = kRows * kQPitch;
+  static constexpr int kRing = kWarps * NS * kStageBytes;
+  // After the loop, over the ring: 8 rows of every warp; the CTA's rows.
+  static constexpr int kMP = HD + 4;  // row pitch in floats: spreads the banks
+  static constexpr int kMergeRows = kWarps * 8 * kMP * 4;
+  static constexpr int kMergeMl = kMergeRows + kWarps * 8 * 8;
+  static constexpr int kPart = kMergeMl + kRows * HD * 4;
+  static constexpr int kMerge = kPart + kRows * 8;
   static constexpr int kFlag = kQBytes + (kRing > kMerge ? kRing : kMerge);
   static constexpr int kSmem = kFlag + 16;
   static_assert(kSmem <= 227 * 1024, "shared-memory budget");
-  static_assert(kKT <= 64 && kKT % 16 == 0, "tile of 16 to 64 keys");
+  static_assert(kKT >= 16 && kKT % 16 == 0, "tile of 16 to 64 keys");
 };
 
-template <int CODE, int HD, int MT>
-__global__ void __launch_bounds__(kRowsThreads)
+template <int CODE, int HD, int NT>
+__global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
     paged_rows_kernel(const __grid_constant__ Paged p, const __grid_constant__ PagedAttn a,
                       int row_blocks) {
   grid_dep_wait();
   grid_dep_launch();
-  using C = RowsCfg<CODE, HD, MT>;
-  constexpr int KT = C::kKT, NS = C::NS, HDP = C::kHDP, U = C::kU;
-  constexpr int NT_S = KT / 8;                        // 8-key column blocks of the scores
-  constexpr int NT_O = HD / 8;                        // 8-dim column blocks of the output
-  constexpr int KS = HDP / 16;                        // 16-wide steps of the first product
+  using C = RowsCfg<CODE, HD, NT>;
+  constexpr int KT = C::kKT, NS = C::NS, HDP = C::kHDP, U = C::kU, W = C::kWarps;
+  constexpr int KB = KT / 16;                // 16-key blocks of a tile
+  constexpr int KS = HDP / 16;               // 16-wide steps of the first product
+  constexpr int DB = HD < 16 ? 1 : HD / 16;  // 16-dim blocks of the output
+  constexpr int KW = (KT + 31) / 32;         // 32-bit words of key bits
   constexpr bool kQuant = CODE != kCodeF16;
+  // Chains of dependent products: several accumulators where there are few.
+  constexpr int kAcc0 = NT * KB >= 4 ? 1 : 4 / (NT * KB);
+  constexpr int ACC = kAcc0 < KS ? kAcc0 : KS;
+  constexpr bool kQInRegs = NT * KS <= 16;
   extern __shared__ __align__(16) uint8_t smem_rows[];
   uint8_t* sQ = smem_rows;
   int* flag = reinterpret_cast<int*>(smem_rows + C::kFlag);
@@ -129,39 +178,54 @@ __global__ void __launch_bounds__(kRowsThreads)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int b = blockIdx.z, hk = blockIdx.y;
-  const int split = blockIdx.x / row_blocks;
+  const int parts = a.cluster > 0 ? a.cluster : a.splits;
+  const int split = static_cast<int>(blockIdx.x) % parts;  // cluster: also the CTA's rank
   // The last rows see the most keys: they go first.
-  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.x) % row_blocks;
+  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.x) / parts;
   const PagedSeq seq = paged_seq(p, b);
   const int rows = seq.n * a.group;  // below 2^31: checked on the host
-  const int r0 = rb * 16 * MT;
-  if (r0 >= rows) return;
+  const int r0 = rb * C::kRows;
+  if (r0 >= rows || paged_is_tc(a, seq)) return;  // the same for a whole cluster
   // Keys that row r sees: [0, lim(r)).
   auto lim_of = [&](int r) {
     return a.causal ? min(seq.len, max(0, seq.pos0 + r / a.group + 1)) : seq.len;
   };
-  const int lim_first = lim_of(r0), lim_last = lim_of(min(r0 + 16 * MT, rows) - 1);
-  const bool is_split = paged_is_split(a, seq);
-  if (!is_split && split > 0) return;
-  const int k_begin = is_split ? split * a.kps : 0;
-  const int k_end = is_split ? min(lim_last, k_begin + a.kps) : lim_last;
-  if (is_split && k_begin >= lim_last) return;  // not looked at when the splits are joined
-
-  // ---- queries, zero rows behind the last one
-  for (int i = threadIdx.x; i < 16 * MT * (HD / 8); i += kRowsThreads) {
-    const int r = i / (HD / 8), c = i % (HD / 8), row = r0 + r;
-    const bool ok = row < rows;
-    const int tok = seq.row0 + (ok ? row / a.group : 0);
-    const int head = hk * a.group + (ok ? row % a.group : 0);
-    rows_cp16(smem_u32(sQ + r * C::kQPitch + c * 16),
-              a.q + static_cast<int64_t>(tok) * a.ld_q + head * HD + c * 8, ok);
+  const int lim_first = lim_of(r0), lim_last = lim_of(min(r0 + C::kRows, rows) - 1);
+  const bool is_split = a.cluster == 0 && paged_is_split(a, seq);
+  int k_begin = 0, k_end = lim_last;
+  if (a.cluster > 0) {
+    const int share = ((lim_last + parts - 1) / parts + KT - 1) / KT * KT;
+    k_begin = min(split * share, lim_last);
+    k_end = min(k_begin + share, lim_last);
+  } else {
+    // Splits behind the sequence (64 bits: splits is the larger kernel's number).
+    if (is_split ? static_cast<int64_t>(split) * a.kps >= lim_last : split > 0) return;
+    if (is_split) {
+      k_begin = split * a.kps;
+      k_end = min(lim_last, k_begin + a.kps);
+    }
   }
-  if constexpr (HD < 16) {
-    for (int i = threadIdx.x; i < 16 * MT; i += kRowsThreads)
-      *reinterpret_cast<uint4*>(sQ + i * C::kQPitch + HD * 2) = make_uint4(0, 0, 0, 0);
+
+  // ---- queries as the product's B operand, zero rows behind the last one.
+  // 8 bits: dims in the order of the codes' k pairs (see the file's comment).
+  for (int i = threadIdx.x; i < C::kRows * (HD / 8); i += C::kThreads) {
+    const int r = i / (HD / 8), c = i % (HD / 8), row = r0 + r;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows)
+      x = *reinterpret_cast<const uint4*>(a.q +
+                                          static_cast<int64_t>(seq.row0 + row / a.group) * a.ld_q +
+                                          (hk * a.group + row % a.group) * HD + c * 8);
+    uint8_t* dst = sQ + r * C::kQPitch;
+    if constexpr (!kQuant) {
+      *reinterpret_cast<uint4*>(dst + c * 16) = x;
+      if (HD < 16) *reinterpret_cast<uint4*>(dst + 16) = make_uint4(0u, 0u, 0u, 0u);
+    } else {  // words 0, 2 of the 4 here to the first half of the 16, 1, 3 to the second
+      uint8_t* at = dst + (c >> 1) * 32 + (c & 1) * 8;
+      *reinterpret_cast<uint2*>(at) = make_uint2(x.x, x.z);
+      *reinterpret_cast<uint2*>(at + 16) = make_uint2(x.y, x.w);
+    }
   }
   if (threadIdx.x == 0) *flag = 0;
-  rows_commit();
 
   // ---- this warp's ring
   uint8_t* ring = smem_rows + C::kQBytes + warp * NS * C::kStageBytes;
@@ -170,12 +234,11 @@ __global__ void __launch_bounds__(kRowsThreads)
       *reinterpret_cast<uint4*>(ring + (i / (2 * KT)) * C::kStageBytes + (i % (2 * KT)) * C::kPitch +
                                 HD * 2) = make_uint4(0, 0, 0, 0);
   }
-  const int n_tiles = k_end > k_begin + warp * KT
-                          ? (k_end - k_begin - warp * KT + kRowsWarps * KT - 1) / (kRowsWarps * KT)
-                          : 0;
+  const int n_tiles =
+      k_end > k_begin + warp * KT ? (k_end - k_begin - warp * KT + W * KT - 1) / (W * KT) : 0;
   const uint8_t* kb = static_cast<const uint8_t*>(p.k) + hk * p.head_stride * code_bytes(CODE);
   const uint8_t* vb = static_cast<const uint8_t*>(p.v) + hk * p.head_stride * code_bytes(CODE);
-  auto tile_key = [&](int i) { return k_begin + (i * kRowsWarps + warp) * KT; };
+  auto tile_key = [&](int i) { return k_begin + (i * W + warp) * KT; };
   // Page of this lane's keys of tile i (lane and lane + 32), one tile ahead.
   int pg[2];
   auto look_up = [&](int i) {
@@ -188,7 +251,7 @@ __global__ void __launch_bounds__(kRowsThreads)
     uint8_t* st = ring + (i % NS) * C::kStageBytes;
     const int k0 = tile_key(i);
 #pragma unroll
-    for (int it = 0; it < KT * U / 32 + (KT * U % 32 != 0); ++it) {
+    for (int it = 0; it < (KT * U + 31) / 32; ++it) {
       const int c = it * 32 + lane, r = c / U, col = c % U;
       int page = __shfl_sync(0xffffffffu, pg[0], r & 31);
       if constexpr (KT > 32) {
@@ -205,7 +268,7 @@ __global__ void __launch_bounds__(kRowsThreads)
     if constexpr (kQuant) {
       float* sc = reinterpret_cast<float*>(st + 2 * C::kTileBytes);
 #pragma unroll
-      for (int u = 0; u < (KT + 31) / 32; ++u) {
+      for (int u = 0; u < KW; ++u) {
         if (lane + 32 * u < KT) {
           const bool ok = pg[u] >= 0;
           const int64_t so = ok ? paged_scale_offset(p, pg[u], hk, k0 + 32 * u + lane) : 0;
@@ -216,7 +279,7 @@ __global__ void __launch_bounds__(kRowsThreads)
     }
     uint32_t* bits = reinterpret_cast<uint32_t*>(st + 2 * C::kTileBytes + C::kScaleBytes);
 #pragma unroll
-    for (int u = 0; u < (KT + 31) / 32; ++u) {
+    for (int u = 0; u < KW; ++u) {
       const uint32_t m = __ballot_sync(0xffffffffu, pg[u] >= 0);
       if (lane == 0) bits[u] = m;
     }
@@ -228,45 +291,38 @@ __global__ void __launch_bounds__(kRowsThreads)
     rows_commit();
     look_up(i + 1);
   }
-  rows_wait<NS - 1>();  // the queries (the oldest group)
-  __syncthreads();
+  __syncthreads();  // the queries
 
-  // Q fragments; with more than one 16-row block they are read again for each
-  // tile (registers).
-  uint32_t qf[MT == 1 ? KS : 1][4];
-  auto load_q = [&](int mt, int kk, uint32_t (&f)[4]) {
-    if constexpr (!kQuant) {
-      rows_ldsm4(smem_u32(sQ + (mt * 16 + (lane & 15)) * C::kQPitch + kk * 32 + (lane >> 4) * 16),
-                 f);
-    } else {  // columns 4t..4t+3 of each 16, see the file's comment
-      const uint2 lo = *reinterpret_cast<const uint2*>(sQ + (mt * 16 + g) * C::kQPitch + kk * 32 +
-                                                       t * 8);
-      const uint2 hi = *reinterpret_cast<const uint2*>(sQ + (mt * 16 + g + 8) * C::kQPitch +
-                                                       kk * 32 + t * 8);
-      f[0] = lo.x;
-      f[1] = hi.x;
-      f[2] = lo.y;
-      f[3] = hi.y;
-    }
+  // Q fragments of two steps at a time (b0, b1 of each).
+  auto load_q = [&](int nt, int kk, uint32_t (&f)[4]) {
+    const uint32_t row = smem_u32(sQ + (nt * 8 + (lane & 7)) * C::kQPitch + kk * 32);
+    if constexpr (KS == 1)
+      rows_ldsm2(row + ((lane >> 3) & 1) * 16, f[0], f[1]);
+    else
+      rows_ldsm4(row + (lane >> 4) * 32 + ((lane >> 3) & 1) * 16, f);
   };
-  if constexpr (MT == 1) {
+  uint32_t qf[kQInRegs ? NT : 1][kQInRegs ? (KS + 1) / 2 : 1][4];
+  if constexpr (kQInRegs) {
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) load_q(0, kk, qf[kk]);
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int kk = 0; kk < KS; kk += 2) load_q(nt, kk, qf[nt][kk / 2]);
   }
 
-  float o[MT][NT_O][4];
-  float m_run[MT][2], l_run[MT][2];
-  int lim[MT][2];
+  // Rows 2t and 2t+1 of each 8 are this thread's.
+  float o[NT][DB][4];
+  float m_ref[NT][2], l_run[NT][2];
+  int lim[NT][2];
   float unit = 1e-37f;  // U (its reciprocal stays finite)
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int i = 0; i < NT_O; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
+    for (int n = 0; n < DB; ++n) o[nt][n][0] = o[nt][n][1] = o[nt][n][2] = o[nt][n][3] = 0.f;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      m_run[mt][r] = -INFINITY;
-      l_run[mt][r] = 0.f;
-      lim[mt][r] = lim_of(min(r0 + mt * 16 + g + 8 * r, rows - 1));
+      m_ref[nt][r] = -INFINITY;  // no key seen yet
+      l_run[nt][r] = 0.f;
+      lim[nt][r] = lim_of(min(r0 + nt * 8 + 2 * t + r, rows - 1));
     }
   }
   bool cleared = false;
@@ -283,90 +339,82 @@ __global__ void __launch_bounds__(kRowsThreads)
     const float* sc = reinterpret_cast<const float*>(st + 2 * C::kTileBytes);
     const int k0 = tile_key(i);
 
-    // ---- S = Q K^T
-    float s[MT][NT_S][4];
+    // ---- S^T = K Q^T: key g (values 0, 1) and g + 8 (2, 3) of each 16, rows 2t, 2t+1
+    float s[NT][KB][4];
+    {
+      float part[ACC][NT][KB][4];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int x = 0; x < ACC; ++x)
 #pragma unroll
-      for (int j = 0; j < NT_S; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
-    auto product = [&](int j, int kk, uint32_t b0, uint32_t b1) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if constexpr (MT == 1) {
-          rows_mma(s[0][j], qf[kk], b0, b1);
-        } else {
-          uint32_t f[4];
-          load_q(mt, kk, f);
-          rows_mma(s[mt][j], f, b0, b1);
-        }
-      }
-    };
-    if constexpr (!kQuant) {
+          for (int j = 0; j < KB; ++j)
+            part[x][nt][j][0] = part[x][nt][j][1] = part[x][nt][j][2] = part[x][nt][j][3] = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        uint32_t f[MT][4];
-        if constexpr (MT > 1) {
+      for (int kk = 0; kk < KS; kk += 2) {
+        uint32_t f[NT][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) load_q(mt, kk, f[mt]);
+        for (int nt = 0; nt < NT; ++nt) {
+          if constexpr (kQInRegs) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[nt][e] = qf[nt][kk / 2][e];
+          } else {
+            load_q(nt, kk, f[nt]);
+          }
         }
 #pragma unroll
-        for (int j = 0; j < NT_S; j += 2) {
-          uint32_t r[4];
-          rows_ldsm4(smem_u32(st + (j * 8 + (lane >> 4) * 8 + (lane & 7)) * C::kPitch + kk * 32 +
-                              ((lane >> 3) & 1) * 16),
-                     r);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            if constexpr (MT == 1) {
-              rows_mma(s[0][j], qf[kk], r[0], r[1]);
-              rows_mma(s[0][j + 1], qf[kk], r[2], r[3]);
-            } else {
-              rows_mma(s[mt][j], f[mt], r[0], r[1]);
-              rows_mma(s[mt][j + 1], f[mt], r[2], r[3]);
+        for (int j = 0; j < KB; ++j) {
+          const uint32_t row =
+              smem_u32(st + (j * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * C::kPitch);
+          uint32_t k1[4], k2[4];  // steps kk and kk + 1
+          if constexpr (!kQuant) {
+            rows_ldsm4(row + kk * 32 + (lane >> 4) * 16, k1);
+            if constexpr (KS > 1) rows_ldsm4(row + (kk + 1) * 32 + (lane >> 4) * 16, k2);
+          } else {
+            uint32_t w[4];
+            if constexpr (KS > 1)
+              rows_ldsm4(row + (kk + (lane >> 4)) * 16, w);
+            else
+              rows_ldsm2(row, w[0], w[1]);
+            k1[0] = codes_to_h2<CODE, 0, 1>(w[0]);
+            k1[1] = codes_to_h2<CODE, 0, 1>(w[1]);
+            k1[2] = codes_to_h2<CODE, 2, 3>(w[0]);
+            k1[3] = codes_to_h2<CODE, 2, 3>(w[1]);
+            if constexpr (KS > 1) {
+              k2[0] = codes_to_h2<CODE, 0, 1>(w[2]);
+              k2[1] = codes_to_h2<CODE, 0, 1>(w[3]);
+              k2[2] = codes_to_h2<CODE, 2, 3>(w[2]);
+              k2[3] = codes_to_h2<CODE, 2, 3>(w[3]);
             }
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            rows_mma(part[kk % ACC][nt][j], k1, f[nt][0], f[nt][1]);
+            if constexpr (KS > 1) rows_mma(part[(kk + 1) % ACC][nt][j], k2, f[nt][2], f[nt][3]);
           }
         }
       }
-    } else {
-      // Blocks of 8 keys x 16 codes, four at a time: block n is column block
-      // n / KS, step n % KS.
 #pragma unroll
-      for (int n = 0; n < NT_S * KS; n += 4) {
-        uint32_t r[4];
-        const int mine = n + (lane >> 3);
-        rows_ldsm4(smem_u32(st + ((mine / KS) * 8 + (lane & 7)) * C::kPitch + (mine % KS) * 16), r);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
-          product((n + m) / KS, (n + m) % KS, codes_to_h2<CODE, 0, 1>(r[m]),
-                  codes_to_h2<CODE, 2, 3>(r[m]));
-      }
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[nt][j][e] = part[0][nt][j][e];
+#pragma unroll
+            for (int x = 1; x < ACC; ++x) s[nt][j][e] += part[x][nt][j][e];
+          }
     }
 
-    // ---- keys that exist; the accumulator's unit; values that must not leak
-    uint32_t bits[(KT + 31) / 32];
+    // ---- keys that exist; values that must not leak
+    uint32_t bits[KW];
     bool full = true;
 #pragma unroll
-    for (int u = 0; u < (KT + 31) / 32; ++u) {
+    for (int u = 0; u < KW; ++u) {
       bits[u] = reinterpret_cast<const uint32_t*>(st + 2 * C::kTileBytes + C::kScaleBytes)[u];
       full = full && bits[u] == (KT < 32 ? (1u << (KT & 31)) - 1u : 0xffffffffu);
     }
     const bool need_mask = !full || k0 + KT > lim_first;  // warp-uniform
-    float unit_corr = 1.f, inv_unit = 0.f;
-    if constexpr (kQuant) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int u = 0; u < (KT + 31) / 32; ++u) {
-        const uint32_t x = lane + 32 * u < KT ? __float_as_uint(sc[KT + 32 * u + lane]) & 0x7fffffffu
-                                              : 0u;
-        top = max(top, x < 0x7f800000u ? x : 0u);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);  // non-negative floats order as integers
-      if (__uint_as_float(top) > unit) {
-        unit_corr = unit / __uint_as_float(top);
-        unit = __uint_as_float(top);
-      }
-      inv_unit = 1.f / unit;
-    }
     if constexpr (CODE != kCodeI8) {
       if (k0 + KT > lim_first && lim_first < lim_last) {
         bool found = false;
@@ -378,11 +426,7 @@ __global__ void __launch_bounds__(kRowsThreads)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if constexpr (CODE == kCodeF16) {
-              if (h2_not_finite(w[e])) {
-                hit = true;
-                if ((w[e] & 0x7c00u) == 0x7c00u) w[e] &= 0xffff0000u;
-                if ((w[e] & 0x7c000000u) == 0x7c000000u) w[e] &= 0xffffu;
-              }
+              hit |= h2_clear(w[e]);
             } else {
               const uint32_t nan = __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
               hit = hit || nan != 0u;
@@ -399,125 +443,141 @@ __global__ void __launch_bounds__(kRowsThreads)
       }
     }
 
-    // ---- mask and running softmax (scores in the log2 domain)
+    // ---- scores in the log2 domain, masked; does a maximum or the unit grow?
+    float vs[kQuant ? KB : 1][2];
+    uint32_t top = 0;
+    if constexpr (kQuant) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      float mx[2] = {-INFINITY, -INFINITY};
+      for (int j = 0; j < KB; ++j)
 #pragma unroll
-      for (int j = 0; j < NT_S; ++j) {
-        float f0 = a.scale_log2, f1 = a.scale_log2;
-        if constexpr (kQuant) {
-          const float2 ks = *reinterpret_cast<const float2*>(sc + j * 8 + 2 * t);
-          f0 *= ks.x;
-          f1 *= ks.y;
+        for (int r = 0; r < 2; ++r) {
+          vs[j][r] = sc[KT + j * 16 + g + 8 * r];
+          const uint32_t x = __float_as_uint(vs[j][r]) & 0x7fffffffu;
+          top = max(top, x < 0x7f800000u ? x : 0u);  // non-negative floats order as integers
         }
+    }
+    bool grow = kQuant && __uint_as_float(top) > unit * kRowsUnit;
+    float mx[NT][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float val = s[mt][j][e] * ((e & 1) ? f1 : f0);
-          if (need_mask) {
-            const int kk = j * 8 + 2 * t + (e & 1);
-            if (k0 + kk >= lim[mt][e >> 1] || !((bits[kk >> 5] >> (kk & 31)) & 1u)) val = -INFINITY;
-          }
-          s[mt][j][e] = val;
-          mx[e >> 1] = fmaxf(mx[e >> 1], val);
-        }
-      }
-      float corr[2];
+    for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-        const float m_new = fmaxf(m_run[mt][r], mx[r]);
-        const float m_ref = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet: weights 0, no NaN
-        corr[r] = fast_exp2(m_run[mt][r] - m_ref);
-        m_run[mt][r] = m_new;
-        mx[r] = m_ref;
+        const int kk = j * 16 + g + 8 * r;
+        float f = a.scale_log2;
+        if constexpr (kQuant) f *= sc[kk];
+        const bool there = !need_mask || ((bits[kk >> 5] >> (kk & 31)) & 1u);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float val = s[nt][j][2 * r + e] * f;
+            if (need_mask && (!there || k0 + kk >= lim[nt][e])) val = -INFINITY;
+            s[nt][j][2 * r + e] = val;
+            mx[nt][e] = fmaxf(mx[nt][e], val);
+          }
       }
-      float rs[2] = {0.f, 0.f};
+    }
 #pragma unroll
-      for (int j = 0; j < NT_S; ++j) {
-        float v0 = 1.f, v1 = 1.f;
-        if constexpr (kQuant) {
-          const float2 vs = *reinterpret_cast<const float2*>(sc + KT + j * 8 + 2 * t);
-          v0 = vs.x * inv_unit;
-          v1 = vs.y * inv_unit;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float w = fast_exp2(s[mt][j][e] - mx[e >> 1]);
-          rs[e >> 1] += w;
-          if constexpr (kQuant)  // a masked key's scale may be anything
-            s[mt][j][e] = w == 0.f ? 0.f : w * ((e & 1) ? v1 : v0);
-          else
-            s[mt][j][e] = w;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) l_run[mt][r] = l_run[mt][r] * corr[r] + rs[r];
+    for (int nt = 0; nt < NT; ++nt)
+      grow = grow || mx[nt][0] > m_ref[nt][0] + kRowsRescale || mx[nt][1] > m_ref[nt][1] + kRowsRescale;
+    if (__any_sync(0xffffffffu, grow)) {
+      float unit_corr = 1.f;
       if constexpr (kQuant) {
-        corr[0] *= unit_corr;
-        corr[1] *= unit_corr;
+        const float now = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+        if (now > unit) {
+          unit_corr = unit / now;
+          unit = now;
+        }
       }
 #pragma unroll
-      for (int n = 0; n < NT_O; ++n) {
-        o[mt][n][0] *= corr[0];
-        o[mt][n][1] *= corr[0];
-        o[mt][n][2] *= corr[1];
-        o[mt][n][3] *= corr[1];
+      for (int nt = 0; nt < NT; ++nt) {
+        float corr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = mx[nt][e];
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+          m = fmaxf(m, m_ref[nt][e]);
+          corr[e] = m == m_ref[nt][e] ? 1.f : fast_exp2(m_ref[nt][e] - m);  // from -inf: 0
+          m_ref[nt][e] = m;
+          l_run[nt][e] *= corr[e];
+          corr[e] *= unit_corr;
+        }
+#pragma unroll
+        for (int n = 0; n < DB; ++n) {
+          o[nt][n][0] *= corr[0];
+          o[nt][n][1] *= corr[1];
+          o[nt][n][2] *= corr[0];
+          o[nt][n][3] *= corr[1];
+        }
       }
     }
 
-    // ---- O += P V, 16 keys at a time
+    // ---- weights, as the second product's B operand
+    uint32_t pf[NT][KB][2];
+    const float inv_unit = kQuant ? 1.f / unit : 1.f;
 #pragma unroll
-    for (int kk = 0; kk < KT / 16; ++kk) {
-      uint32_t pf[MT][4];
+    for (int nt = 0; nt < NT; ++nt) {
+      float m_use[2];  // nothing seen yet: weights 0, no NaN
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        pf[mt][0] = pack_half2(s[mt][2 * kk][0], s[mt][2 * kk][1]);
-        pf[mt][1] = pack_half2(s[mt][2 * kk][2], s[mt][2 * kk][3]);
-        pf[mt][2] = pack_half2(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
-        pf[mt][3] = pack_half2(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
-      }
-      const uint32_t row = smem_u32(sv + (kk * 16 + (lane & 15)) * C::kPitch);
+      for (int e = 0; e < 2; ++e) m_use[e] = m_ref[nt][e] == -INFINITY ? 0.f : m_ref[nt][e];
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            w[e] = fast_exp2(s[nt][j][2 * r + e] - m_use[e]);
+            l_run[nt][e] += w[e];
+            // a masked key's scale may be anything
+            if constexpr (kQuant) w[e] = w[e] == 0.f ? 0.f : w[e] * (vs[j][r] * inv_unit);
+          }
+          pf[nt][j][r] = rows_movm_t(pack_half2(w[0], w[1]));
+        }
+    }
+
+    // ---- O^T += V^T P^T: 16 dims by 16 keys
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+      const uint32_t row = smem_u32(sv + j * 16 * C::kPitch);
       if constexpr (!kQuant) {
-        if constexpr (NT_O == 1) {
-          uint32_t b0, b1;
-          rows_ldsm2_t(row, b0, b1);
+        if constexpr (HD < 16) {
+          uint32_t v[4] = {0u, 0u, 0u, 0u};
+          rows_ldsm2_t(row + (lane & 15) * C::kPitch, v[0], v[2]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) rows_mma(o[mt][0], pf[mt], b0, b1);
+          for (int nt = 0; nt < NT; ++nt) rows_mma(o[nt][0], v, pf[nt][j][0], pf[nt][j][1]);
         } else {
 #pragma unroll
-          for (int n = 0; n < NT_O; n += 2) {
-            uint32_t r[4];
-            rows_ldsm4_t(row + n * 16 + (lane >> 4) * 16, r);
+          for (int n = 0; n < DB; ++n) {
+            uint32_t v[4];
+            rows_ldsm4_t(row + ((lane >> 4) * 8 + (lane & 7)) * C::kPitch + n * 32 +
+                             ((lane >> 3) & 1) * 16,
+                         v);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              rows_mma(o[mt][n], pf[mt], r[0], r[1]);
-              rows_mma(o[mt][n + 1], pf[mt], r[2], r[3]);
-            }
+            for (int nt = 0; nt < NT; ++nt) rows_mma(o[nt][n], v, pf[nt][j][0], pf[nt][j][1]);
           }
         }
       } else {
-        auto block = [&](int n, uint32_t lo, uint32_t hi) {  // 16 dims; lo, hi: keys 0-7, 8-15
+        auto block = [&](int n, uint32_t lo, uint32_t hi) {  // 16 dims; keys 0-7, 8-15
+          const uint32_t v[4] = {codes_to_h2<CODE, 0, 2>(lo), codes_to_h2<CODE, 1, 3>(lo),
+                                 codes_to_h2<CODE, 0, 2>(hi), codes_to_h2<CODE, 1, 3>(hi)};
 #pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
-            const uint32_t b0 = odd ? codes_to_h2<CODE, 1, 3>(lo) : codes_to_h2<CODE, 0, 2>(lo);
-            const uint32_t b1 = odd ? codes_to_h2<CODE, 1, 3>(hi) : codes_to_h2<CODE, 0, 2>(hi);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) rows_mma(o[mt][2 * n + odd], pf[mt], b0, b1);
-          }
+          for (int nt = 0; nt < NT; ++nt) rows_mma(o[nt][n], v, pf[nt][j][0], pf[nt][j][1]);
         };
         if constexpr (HD == 16) {
           uint32_t lo, hi;
-          rows_ldsm2_t(row, lo, hi);
+          rows_ldsm2_t(row + (lane & 15) * C::kPitch, lo, hi);
           block(0, lo, hi);
         } else {
 #pragma unroll
-          for (int n = 0; n < HD / 16; n += 2) {
-            uint32_t r[4];
-            rows_ldsm4_t(row + n * 16 + (lane >> 4) * 16, r);
-            block(n, r[0], r[1]);
-            block(n + 1, r[2], r[3]);
+          for (int n = 0; n < DB; n += 2) {
+            uint32_t w[4];
+            rows_ldsm4_t(row + (lane & 15) * C::kPitch + (n + (lane >> 4)) * 16, w);
+            block(n, w[0], w[1]);
+            block(n + 1, w[2], w[3]);
           }
         }
       }
@@ -528,55 +588,53 @@ __global__ void __launch_bounds__(kRowsThreads)
   __syncthreads();
   const bool fix = *flag != 0;
 
-  // ---- merge the warps, one 16-row block at a time
-  float* mo = reinterpret_cast<float*>(smem_rows + C::kQBytes);  // [warp][16][HD]
-  float* mm = mo + kRowsWarps * 16 * HD;                         // [warp][16]
-  float* ml = mm + kRowsWarps * 16;
+  // ---- merge the warps, 8 rows at a time
+  uint8_t* area = smem_rows + C::kQBytes;
+  float* mo = reinterpret_cast<float*>(area);                      // [warp][8][kMP]
+  float2* ml = reinterpret_cast<float2*>(area + C::kMergeRows);    // [warp][8] (max, sum)
+  float* cta_o = reinterpret_cast<float*>(area + C::kMergeMl);     // cluster: [kRows][HD]
+  float2* cta_ml = reinterpret_cast<float2*>(area + C::kPart);     // cluster: [kRows]
   const float back = kQuant ? unit : 1.f;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    if (r0 + mt * 16 >= rows) break;  // uniform
+  for (int nt = 0; nt < NT; ++nt) {
+    if (r0 + nt * 8 >= rows) break;  // uniform
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l_run[mt][r] += __shfl_xor_sync(0xffffffffu, l_run[mt][r], 1);
-      l_run[mt][r] += __shfl_xor_sync(0xffffffffu, l_run[mt][r], 2);
-      float* dst = mo + (warp * 16 + g + 8 * r) * HD;
-      if constexpr (!kQuant) {
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int n = 0; n < NT_O; ++n)
-          *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) =
-              make_float2(o[mt][n][2 * r], o[mt][n][2 * r + 1]);
-      } else {
+      for (int d = 4; d < 32; d <<= 1)
+        l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], d);
+      float* dst = mo + (warp * 8 + 2 * t + e) * C::kMP;
 #pragma unroll
-        for (int n = 0; n < HD / 16; ++n)
-          *reinterpret_cast<float4*>(dst + n * 16 + 4 * t) =
-              make_float4(o[mt][2 * n][2 * r] * back, o[mt][2 * n + 1][2 * r] * back,
-                          o[mt][2 * n][2 * r + 1] * back, o[mt][2 * n + 1][2 * r + 1] * back);
+      for (int n = 0; n < DB; ++n) {
+        if constexpr (kQuant) {
+          *reinterpret_cast<float2*>(dst + n * 16 + 2 * g) =
+              make_float2(o[nt][n][e] * back, o[nt][n][2 + e] * back);
+        } else {
+          dst[n * 16 + g] = o[nt][n][e];
+          if constexpr (HD >= 16) dst[n * 16 + 8 + g] = o[nt][n][2 + e];
+        }
       }
-      if (t == 0) {
-        mm[warp * 16 + g + 8 * r] = m_run[mt][r];
-        ml[warp * 16 + g + 8 * r] = l_run[mt][r];
-      }
+      if (g == 0) ml[warp * 8 + 2 * t + e] = make_float2(m_ref[nt][e], l_run[nt][e]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += kRowsThreads) {
-      const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, row = r0 + mt * 16 + r;
+    for (int i = threadIdx.x; i < 8 * (HD / 4); i += C::kThreads) {
+      const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, row = r0 + nt * 8 + r;
       if (row >= rows) continue;
       float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) m = fmaxf(m, mm[w * 16 + r]);
+      for (int w = 0; w < W; ++w) m = fmaxf(m, ml[w * 8 + r].x);
       float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
-        const float mw = mm[w * 16 + r];
-        if (mw == -INFINITY && ml[w * 16 + r] == 0.f) continue;  // this warp saw no key
-        const float f = fast_exp2(mw - m);
-        const float4 x = *reinterpret_cast<const float4*>(mo + (w * 16 + r) * HD + d);
-        acc[0] += f * x.x;
-        acc[1] += f * x.y;
-        acc[2] += f * x.z;
-        acc[3] += f * x.w;
-        l += f * ml[w * 16 + r];
+      for (int w = 0; w < W; ++w) {
+        const float2 x = ml[w * 8 + r];
+        if (x.x == -INFINITY && x.y == 0.f) continue;  // this warp saw no key
+        const float f = fast_exp2(x.x - m);
+        const float4 y = *reinterpret_cast<const float4*>(mo + (w * 8 + r) * C::kMP + d);
+        acc[0] += f * y.x;
+        acc[1] += f * y.y;
+        acc[2] += f * y.z;
+        acc[3] += f * y.w;
+        l += f * x.y;
       }
       if (fix) {  // non-finite values cleared from shared tiles: to the rows that see them
         const int hi = min(lim_of(row), k_end);
@@ -584,55 +642,103 @@ __global__ void __launch_bounds__(kRowsThreads)
           const int page = paged_page(p, b, key);
           if (page < 0) continue;
           const int64_t at = paged_offset(p, page, key) + hk * p.head_stride + d;
-          const float vs = kQuant ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
+          const float sv = kQuant ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = paged_value<CODE>(p.v, at + e, vs);
+            const float x = paged_value<CODE>(p.v, at + e, sv);
             if (!isfinite(x)) acc[e] += x;
           }
         }
       }
       const int tok = seq.row0 + row / a.group, head = hk * a.group + row % a.group;
-      if (is_split) {
-        const int64_t at = (static_cast<int64_t>(tok) * (p.kv_heads * a.group) + head) * a.splits +
-                           split;
-        *reinterpret_cast<float4*>(a.part_o + at * HD + d) =
-            make_float4(acc[0], acc[1], acc[2], acc[3]);
+      const float4 y = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      if (a.cluster > 0) {
+        *reinterpret_cast<float4*>(cta_o + (nt * 8 + r) * HD + d) = y;
+        if (d == 0) cta_ml[nt * 8 + r] = make_float2(m, l);
+      } else if (is_split) {
+        const int64_t at =
+            (static_cast<int64_t>(tok) * (p.kv_heads * a.group) + head) * a.splits + split;
+        *reinterpret_cast<float4*>(a.part_o + at * HD + d) = y;
         if (d == 0) a.part_ml[at] = make_float2(m, l);
       } else {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // no key seen: zero (NaN sums stay NaN)
-        *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(tok) * a.ld_out + head * HD + d) =
-            make_uint2(pack_half2(acc[0] * inv, acc[1] * inv), pack_half2(acc[2] * inv, acc[3] * inv));
+        store_row4(a.out + static_cast<int64_t>(tok) * a.ld_out + head * HD + d, y, l);
       }
     }
     __syncthreads();
   }
+  if (a.cluster == 0) return;
+
+  // ---- join the cluster: every CTA a share of the rows' elements
+  cluster_sync_all();
+  const int count = min(C::kRows, rows - r0) * (HD / 4);
+  for (int i = split * C::kThreads + threadIdx.x; i < count; i += parts * C::kThreads) {
+    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, row = r0 + r;
+    const uint32_t at_ml = smem_u32(cta_ml + r), at_o = smem_u32(cta_o + r * HD + d);
+    float m = -INFINITY;
+    for (int c = 0; c < parts; ++c) m = fmaxf(m, rows_peer2(mapa_shared(at_ml, c)).x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    for (int c = 0; c < parts; ++c) {
+      const float2 x = rows_peer2(mapa_shared(at_ml, c));
+      if (x.x == -INFINITY && x.y == 0.f) continue;  // this CTA saw no key
+      const float f = fast_exp2(x.x - m);
+      const float4 y = rows_peer4(mapa_shared(at_o, c));
+      acc.x += f * y.x;
+      acc.y += f * y.y;
+      acc.z += f * y.z;
+      acc.w += f * y.w;
+      l += f * x.y;
+    }
+    store_row4(a.out + static_cast<int64_t>(seq.row0 + row / a.group) * a.ld_out +
+                   (hk * a.group + row % a.group) * HD + d,
+               acc, l);
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its results
 }
 
-template <int CODE, int HD, int MT>
+template <int CODE, int HD, int NT>
 int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t stream) {
-  using C = RowsCfg<CODE, HD, MT>;
+  using C = RowsCfg<CODE, HD, NT>;
   static int done[kMaxDevices] = {0};
-  auto kern = paged_rows_kernel<CODE, HD, MT>;
+  auto kern = paged_rows_kernel<CODE, HD, NT>;
   int st = ensure_smem(reinterpret_cast<const void*>(kern), C::kSmem, done);
   if (st != TFX_OK) return st;
-  const int64_t blocks = (rows + 16 * MT - 1) / (16 * MT);
-  if (blocks * a.splits > 0x7fffffffLL)
+  const int64_t blocks = (rows + C::kRows - 1) / C::kRows;
+  const int parts = a.cluster > 0 ? a.cluster : a.splits;
+  if (blocks * parts > 0x7fffffffLL)
     return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: too many rows");
-  launch_pdl(kern, dim3(static_cast<unsigned>(blocks * a.splits), p.kv_heads, p.batch),
-             dim3(kRowsThreads), C::kSmem, stream, p, a, static_cast<int>(blocks));
-  return check_launch("paged_rows_kernel");
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(parts);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks * parts), p.kv_heads, p.batch);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.cluster > 0 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, a, static_cast<int>(blocks));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TFX_ERR_CUDA, "paged_rows_kernel: %s", cudaGetErrorString(e));
+  }
+  return TFX_OK;
 }
 
 template <int CODE, int HD>
 int launch_rows_hd(const Paged& p, const PagedAttn& a, int block_rows, int64_t rows,
                    cudaStream_t stream) {
   if constexpr (HD <= 64) {
-    if (block_rows == 64) return launch_rows<CODE, HD, 4>(p, a, rows, stream);
+    if (block_rows == 64) return launch_rows<CODE, HD, 8>(p, a, rows, stream);
   }
   if constexpr (HD <= 128) {
-    if (block_rows == 32) return launch_rows<CODE, HD, 2>(p, a, rows, stream);
+    if (block_rows == 32) return launch_rows<CODE, HD, 4>(p, a, rows, stream);
   }
+  if (block_rows == 16) return launch_rows<CODE, HD, 2>(p, a, rows, stream);
   return launch_rows<CODE, HD, 1>(p, a, rows, stream);
 }
 

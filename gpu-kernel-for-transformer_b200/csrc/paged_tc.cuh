@@ -1,0 +1,780 @@
+// Attention of many query rows (chunks of prompts) over a paged cache on the
+// 5th-generation tensor cores, head_dim 64 and 128. Included by one
+// translation unit per cache type.
+//
+// The `group` query heads that read one key/value head are rows of the same
+// tile: a 128-row tile holds 128 / group tokens x group heads (TMA box of q;
+// the last 128 % group rows stay unused). CTA = two such tiles A and B of one
+// (sequence, key/value head) that share every 128-key tile, and one range of
+// the keys; 12 warps, one CTA per SM:
+//   warps 2..5, 6..9  softmax of A and of B; thread = row = TMEM lane
+//   warps 1, 10       MMA issuers of A and of B (one lane)
+//   fp16:  warp 0 loads K and V, a TMA box per page and 64 columns (lane =
+//          box); warp 11 looks after V tiles that hold keys which not every
+//          row sees
+//   8 bit: warps 0 and 11 each expand half of every K and V tile from a ring
+//          of raw tiles (TMA, a box per page; warp 0 issues it) to fp16
+// A key tile is 128 consecutive positions, 128 / page_size pages or half of
+// one; pages outside the pool are boxes outside the tensor map and read as
+// zeros.
+//
+// Products, TMEM columns and the lazy rescaling of O are those of the
+// contiguous kernel (attention_tc.cu): S = Q K^T and O += P V with P from TMEM
+// and V MN-major from the row-major tile. S needs 128x128xHD products for every
+// exponential row of 128, which the softmax warps bound at head_dim 64; MN-major
+// V costs tensor time that is hidden behind them.
+//
+// 8-bit values are expanded as code * scale in fp16. The scale s is used as
+// m * 2^k with an fp16 m: int8 codes are placed behind the exponent of
+// 2^(10+k) (as 1024 + u in units of 2^k), so that subtracting 1152 * 2^k gives
+// code * 2^k exactly, and one multiplication by m follows; e4m3 codes convert
+// exactly and are multiplied by m and by 2^k. m's rounding and the product's
+// are each half an fp16 step, small scales lose nothing more.
+//
+// What a row does not see must not reach it, and 0 * inf does: V rows behind
+// the sequence are cleared; in tiles that some rows of the CTA see and others
+// do not, non-finite values are cleared before the product and added at the
+// end to the rows that see them. Rows whose scores hold a NaN or +inf are NaN
+// (the polynomial exponential would lose them).
+#pragma once
+
+#include "paged.cuh"
+
+namespace tfx {
+namespace {
+
+constexpr int kPtThreads = 384;
+constexpr int kPtTile = 128;
+constexpr float kPtRescale = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8
+constexpr int kPtPoly = 2;          // of 8 pairs of exponentials, on the FMA pipe
+constexpr uint32_t kPtCols = 512;
+
+template <int CODE, int HD>
+struct PtCfg {
+  static constexpr bool kQuant = CODE != kCodeF16;
+  static constexpr int kStages = HD == 64 ? 4 : 2;
+  static constexpr int kBlocks = HD / 64;
+  static constexpr int kBlockBytes = kPtTile * 128;
+  static constexpr int kTileBytes = kPtTile * HD * 2;
+  static constexpr int kRaws = kQuant ? (HD == 64 ? 4 : 2) : 0;  // raw tiles: K and V in turn
+  static constexpr int kRawBytes = kPtTile * HD;
+  static constexpr int kQ = 0;
+  static constexpr int kK = 2 * kTileBytes;
+  static constexpr int kV = kK + kStages * kTileBytes;
+  static constexpr int kR = kV + kStages * kTileBytes;
+  static constexpr int kBar = kR + kRaws * kRawBytes;
+  static constexpr int kSmem = kBar + 512 + 1024;  // barriers + alignment slack
+  static constexpr bool kSepP = HD == 64;          // P has its own TMEM columns
+  static constexpr uint32_t kColP = kSepP ? 2 * kPtTile : 0;
+  static constexpr uint32_t kPStride = kSepP ? kPtTile / 2 : kPtTile;
+  static constexpr uint32_t kColO = kSepP ? 3 * kPtTile : 2 * kPtTile;
+  static_assert(kColO + 2 * HD <= kPtCols, "TMEM budget");
+  static_assert(kSmem <= 227 * 1024, "shared-memory budget");
+};
+
+__device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
+                                           int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// max(a, b, c), NaN if one is.
+__device__ __forceinline__ float pt_max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// A row's scale as the expansion uses it: fp16 bits of m (low half), k + 64 (high).
+template <int CODE>
+__device__ __forceinline__ uint32_t pt_scale(float s) {
+  const int e = static_cast<int>((__float_as_uint(s) >> 23) & 0xff) - 127;
+  const int k = min(max(e, CODE == kCodeI8 ? -24 : -14), CODE == kCodeI8 ? 5 : 8);
+  const float m = s * __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  return static_cast<uint32_t>(__half_as_ushort(__float2half_rn(m))) |
+         (static_cast<uint32_t>(k + 64) << 16);
+}
+
+// Four codes to two fp16 pairs, times the row's scale.
+template <int CODE>
+struct PtExpand {
+  uint32_t m, a, c;  // m twice; int8: high byte x 4, 1152 * 2^k; e4m3: 2^k
+  __device__ __forceinline__ explicit PtExpand(uint32_t packed) {
+    const int k = static_cast<int>(packed >> 16) - 64;
+    m = __byte_perm(packed, 0u, 0x1010);
+    if constexpr (CODE == kCodeI8) {
+      a = (0x64u + 4u * static_cast<uint32_t>(k)) * 0x01010101u;
+      c = (0x6480u + (static_cast<uint32_t>(k) << 10)) * 0x00010001u;
+    } else {
+      a = 0u;
+      c = (static_cast<uint32_t>(k + 15) << 10) * 0x00010001u;
+    }
+  }
+  __device__ __forceinline__ void operator()(uint32_t x, uint32_t& lo, uint32_t& hi) const {
+    if constexpr (CODE == kCodeI8) {
+      const uint32_t u = x ^ 0x80808080u;
+      lo = h2_bits(__hmul2(__hsub2(bits_h2(__byte_perm(u, a, 0x4140)), bits_h2(c)), bits_h2(m)));
+      hi = h2_bits(__hmul2(__hsub2(bits_h2(__byte_perm(u, a, 0x4342)), bits_h2(c)), bits_h2(m)));
+    } else {
+      lo = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_to_h2(x)), bits_h2(m)), bits_h2(c)));
+      hi = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_to_h2(x >> 16)), bits_h2(m)), bits_h2(c)));
+    }
+  }
+};
+
+template <int CODE, int HD>
+__global__ void __launch_bounds__(kPtThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Paged p,
+                    const __grid_constant__ PagedAttn a, int row_blocks, int* err) {
+  grid_dep_wait();
+  grid_dep_launch();
+  using L = PtCfg<CODE, HD>;
+  constexpr int S = L::kStages;
+  constexpr bool kQuant = L::kQuant;
+  constexpr int R = L::kRaws > 0 ? L::kRaws : 1;
+
+  // ---- this CTA's work
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.x, b = blockIdx.y;
+  const int split = static_cast<int>(blockIdx.z) % a.splits;
+  // The last rows of all sequences and heads see the most keys: they go first.
+  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.z) / a.splits;
+  const int group = a.group, tile_tokens = kPtTile / group;
+  const PagedSeq seq = paged_seq(p, b);
+  const int i0 = rb * 2 * tile_tokens;  // first token
+  if (i0 >= seq.n || !paged_is_tc(a, seq)) return;
+  auto lim_of = [&](int i) {  // token i sees keys [0, lim)
+    return a.causal ? min(seq.len, max(0, seq.pos0 + i + 1)) : seq.len;
+  };
+  const bool is_split = paged_is_split(a, seq);
+  // Splits behind the sequence (64 bits: splits is the larger kernel's number).
+  if (is_split ? static_cast<int64_t>(split) * a.kps_tc >= seq.len : split > 0) return;
+  const int k_begin = is_split ? split * a.kps_tc : 0;
+  const int k_stop = is_split ? k_begin + a.kps_tc : seq.len;  // of the split
+  auto tiles_of = [&](int x) {
+    const int first = i0 + x * tile_tokens;
+    if (first >= seq.n) return 0;
+    const int lim = min(lim_of(min(first + tile_tokens, seq.n) - 1), k_stop);
+    return lim > k_begin ? (lim - k_begin + kPtTile - 1) / kPtTile : 0;
+  };
+  const int nA = tiles_of(0), nB = tiles_of(1), n_iter = max(nA, nB);
+  if (is_split && n_iter == 0) return;  // not looked at when the splits are joined
+  // Tiles from this key on hold keys that not every row sees.
+  const int lim_first = lim_of(i0);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* k_full = q_full + 1;
+  uint64_t* v_full = k_full + S;        // fp16: V loaded
+  uint64_t* v_ready = v_full + S;       // V may be multiplied
+  uint64_t* k_empty = v_ready + S;      // [2][S]
+  uint64_t* v_empty = k_empty + 2 * S;  // [2][S]
+  uint64_t* s_full = v_empty + 2 * S;   // [2]
+  uint64_t* s_free = s_full + 2;        // [2], separate P only
+  uint64_t* p_full = s_free + 2;        // [2]
+  uint64_t* o_done = p_full + 2;        // [2]
+  uint64_t* drain = o_done + 2;         // [2]
+  uint64_t* r_full = drain + 2;         // [R] raw tile loaded
+  uint64_t* r_empty = r_full + R;       // [R] raw tile read by both warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + R);
+  volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
+  static_assert((1 + 7 * S + 10 + 2 * R) * 8 + 8 <= 512, "barrier space");
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_q);
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+    mbar_init(q_full, 1);
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&k_full[s], kQuant ? 2 : 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_ready[s], kQuant ? 2 : 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&k_empty[x * S + s], 1);
+        mbar_init(&v_empty[x * S + s], 1);
+      }
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&s_full[x], 1);
+      mbar_init(&s_free[x], 4);
+      mbar_init(&p_full[x], 4);
+      mbar_init(&o_done[x], 1);
+      mbar_init(&drain[x], 1);
+    }
+    for (int r = 0; r < R; ++r) {
+      mbar_init(&r_full[r], 1);
+      mbar_init(&r_empty[r], 2);
+    }
+    *cleared = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kPtCols);
+    tmem_relinquish();
+  }
+  // Pages of the range that are outside the pool: rare, so looked for once.
+  int hole = 0;
+  {
+    const int last = min(k_stop, min(seq.len, lim_of(min(i0 + 2 * tile_tokens, seq.n) - 1)));
+    for (int pos = k_begin + (static_cast<int>(threadIdx.x) << p.page_shift); pos < last;
+         pos += kPtThreads << p.page_shift)
+      hole |= paged_page(p, b, pos) < 0;
+  }
+  tc_fence_before();
+  const bool holes = __syncthreads_or(hole);
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int page_rows = min(1 << p.page_shift, kPtTile);  // of a tile in one page
+  const int tile_pages = kPtTile / page_rows;
+
+  // Page of a tile's part, as a coordinate (outside the map: zeros).
+  auto page_coord = [&](int j, int part) {
+    const int pos = k_begin + j * kPtTile + part * page_rows;
+    const int page = j < n_iter && pos < seq.len ? paged_page(p, b, pos) : -1;
+    return page < 0 ? p.num_pages : page;
+  };
+  auto slot_coord = [&](int j, int part) {
+    return (k_begin + j * kPtTile + part * page_rows) & ((1 << p.page_shift) - 1);
+  };
+  auto stage_free = [&](uint64_t* empty, int j) {  // stage of tile j, which held tile j - S
+    const uint32_t par = ((j / S) - 1) & 1;
+    bool ok = true;
+    if (j >= S) {
+      if (j - S < nA) ok = mbar_wait(&empty[j % S], par, err, kDevTimeoutEmpty);
+      if (ok && j - S < nB) ok = mbar_wait(&empty[S + j % S], par, err, kDevTimeoutEmpty);
+    }
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
+  auto load_q = [&]() {
+    if (lane == 0) {
+      const int rows = tile_tokens * group;
+      mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(2 * L::kBlocks * rows * 128));
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int cb = 0; cb < L::kBlocks; ++cb)
+          tma_load_3d(smem + L::kQ + x * L::kTileBytes + cb * L::kBlockBytes, &tm_q, q_full,
+                      64 * cb, hk * group, seq.row0 + i0 + x * tile_tokens);
+    }
+  };
+
+  if (warp == 0 || warp == 11) {
+    if constexpr (!kQuant) {
+      if (warp == 0) {
+        // -------------------------------------------------- TMA of K and V
+        load_q();
+        // Lane = (part of the tile, 64-column block).
+        const int part = lane % tile_pages, cb = lane / tile_pages;
+        const bool mine = cb < L::kBlocks;
+        const uint32_t dst = smem_u32(smem) + cb * L::kBlockBytes + part * page_rows * 128;
+        int page = page_coord(0, part), k_issued = 0, issued = 0;
+        for (int j = 0; j < n_iter; ++j) {
+          const int st = j % S;
+          const int next = page_coord(j + 1, part);
+          if (!stage_free(k_empty, j)) break;
+          if (lane == 0) mbar_arrive_expect_tx(&k_full[st], L::kTileBytes);
+          __syncwarp();
+          if (mine)
+            pt_load_4d(dst + L::kK + st * L::kTileBytes, &tm_k, &k_full[st], 64 * cb,
+                       slot_coord(j, part), hk, page);
+          k_issued = j + 1;
+          if (!stage_free(v_empty, j)) break;
+          if (lane == 0) mbar_arrive_expect_tx(&v_full[st], L::kTileBytes);
+          __syncwarp();
+          if (mine)
+            pt_load_4d(dst + L::kV + st * L::kTileBytes, &tm_v, &v_full[st], 64 * cb,
+                       slot_coord(j, part), hk, page);
+          issued = j + 1;
+          page = next;
+        }
+        // Our own copies land before the CTA may exit.
+        mbar_wait(q_full, 0, nullptr, 0);
+        for (int j = max(0, k_issued - S); j < k_issued; ++j)
+          mbar_wait(&k_full[j % S], (j / S) & 1, nullptr, 0);
+        for (int j = max(0, issued - S); j < issued; ++j)
+          mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, 0);
+      } else {
+        // ---------------------------------------------- V tiles not all see
+        for (int j = 0; j < n_iter; ++j) {
+          const int st = j % S, key0 = k_begin + j * kPtTile;
+          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / S) & 1, err, kDevTimeoutFull)))
+            break;
+          if (key0 + kPtTile > lim_first) {
+            uint8_t* tile = smem + L::kV + st * L::kTileBytes;
+            bool found = false;
+            for (int c = lane; c < L::kTileBytes / 16; c += 32) {
+              // 16-byte chunk c lies in row (c / 8) % 128 of its 64-column block
+              uint4* at = reinterpret_cast<uint4*>(tile) + c;
+              const bool behind = key0 + ((c >> 3) & (kPtTile - 1)) >= seq.len;
+              uint4 x = *at;
+              bool hit = h2_clear(x.x);
+              hit |= h2_clear(x.y);
+              hit |= h2_clear(x.z);
+              hit |= h2_clear(x.w);
+              if (behind) *at = make_uint4(0u, 0u, 0u, 0u);
+              else if (hit) *at = x;
+              found |= hit && !behind;
+            }
+            if (found) *cleared = 1;
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&v_ready[st]);
+        }
+      }
+    } else {
+      // ------------------------------------------- raw tiles, expanded to fp16
+      const int half = warp == 0 ? 0 : 1;  // rows 64 * half .. + 63 of every tile
+      const int total = 2 * n_iter;
+      int raw_issued = 0;
+      int part_page = 0, part_next = 0;  // warp 0: this lane's page of the next raw tiles
+      if (warp == 0) {
+        load_q();
+        part_page = page_coord(0, lane % tile_pages);
+        part_next = page_coord(1, lane % tile_pages);
+      }
+      auto issue_raw = [&]() {  // warp 0: tile raw_issued / 2, K if even
+        const int e = raw_issued++, j = e >> 1;
+        if (lane == 0) mbar_arrive_expect_tx(&r_full[e % R], L::kRawBytes);
+        __syncwarp();
+        if (lane < tile_pages)
+          pt_load_4d(smem_u32(smem + L::kR + (e % R) * L::kRawBytes) + lane * page_rows * HD,
+                     (e & 1) ? &tm_v : &tm_k, &r_full[e % R], 0, slot_coord(j, lane), hk, part_page);
+        if (e & 1) {
+          part_page = part_next;
+          part_next = page_coord(j + 2, lane % tile_pages);
+        }
+      };
+      if (warp == 0)
+        while (raw_issued < min(R, total)) issue_raw();
+      // Scales of this lane's two rows (lane, lane + 32 of the warp's half) of
+      // tile j, K and V; loaded a tile ahead.
+      float sc[2][2];
+      auto load_scales = [&](int j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int key = k_begin + j * kPtTile + half * 64 + 32 * u + lane;
+          const int page = j < n_iter && key < seq.len ? paged_page(p, b, key) : -1;
+          const int64_t so = page >= 0 ? paged_scale_offset(p, page, hk, key) : 0;
+          sc[0][u] = page >= 0 ? p.k_scale[so] : 0.f;
+          sc[1][u] = page >= 0 ? p.v_scale[so] : 0.f;
+        }
+      };
+      load_scales(0);
+      bool ok = true;
+      for (int j = 0; ok && j < n_iter; ++j) {
+        const int st = j % S, key0 = k_begin + j * kPtTile;
+        uint32_t pk[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          pk[0][u] = pt_scale<CODE>(sc[0][u]);
+          pk[1][u] = pt_scale<CODE>(sc[1][u]);
+        }
+        load_scales(j + 1);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const int e = 2 * j + kv;
+          // Refill the raw tile before this one (both warps are through with it).
+          if (warp == 0 && e > 0 && raw_issued < total) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&r_empty[(e - 1) % R], ((e - 1) / R) & 1, err,
+                                                   kDevTimeoutEmpty));
+            if (!ok) break;
+            issue_raw();
+          }
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) &&
+               stage_free(kv ? v_empty : k_empty, j);
+          if (!ok) break;
+          const uint8_t* raw = smem + L::kR + (e % R) * L::kRawBytes;
+          uint8_t* tile = smem + (kv ? L::kV : L::kK) + st * L::kTileBytes;
+          const bool partly = kv == 1 && key0 + kPtTile > lim_first;  // not every row sees all
+          constexpr int CPR = HD / 16;            // 16-code chunks of a row
+          constexpr int RPP = 32 / CPR;           // rows of a pass
+          const int c = lane % CPR;
+          bool found = false;
+#pragma unroll 4
+          for (int ps = 0; ps < 64 / RPP; ++ps) {
+            const int rl = ps * RPP + lane / CPR;  // row of the warp's half
+            const int r = half * 64 + rl;
+            const uint32_t lo = __shfl_sync(0xffffffffu, pk[kv][0], rl & 31);
+            const uint32_t hi = __shfl_sync(0xffffffffu, pk[kv][1], rl & 31);
+            const PtExpand<CODE> expand(ps * RPP < 32 ? lo : hi);
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + r * HD + c * 16);
+            uint32_t w[8];
+            expand(x.x, w[0], w[1]);
+            expand(x.y, w[2], w[3]);
+            expand(x.z, w[4], w[5]);
+            expand(x.w, w[6], w[7]);
+            if (partly) {
+              const bool behind = key0 + r >= seq.len;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const bool hit = h2_clear(w[i]);
+                found |= hit && !behind;
+                if (behind) w[i] = 0u;
+              }
+            }
+            // fp16 chunks 2c and 2c+1 of the row, swizzled; lanes of the second
+            // 64-column block store theirs in the other order (banks).
+            uint8_t* row = tile + (c >> 2) * L::kBlockBytes + r * 128;
+            const int sub = c >> 2;
+            const uint4 y0 = make_uint4(w[0], w[1], w[2], w[3]), y1 = make_uint4(w[4], w[5], w[6], w[7]);
+            const int ch = 2 * (c & 3);
+            *reinterpret_cast<uint4*>(row + (((ch + sub) ^ (r & 7)) << 4)) = sub ? y1 : y0;
+            *reinterpret_cast<uint4*>(row + (((ch + 1 - sub) ^ (r & 7)) << 4)) = sub ? y0 : y1;
+          }
+          if (found) *cleared = 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(kv ? &v_ready[st] : &k_full[st]);
+            mbar_arrive(&r_empty[e % R]);
+          }
+        }
+      }
+      if (warp == 0) {  // our own copies land before the CTA may exit
+        mbar_wait(q_full, 0, nullptr, 0);
+        for (int e = max(0, raw_issued - R); e < raw_issued; ++e)
+          mbar_wait(&r_full[e % R], (e / R) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == 1 || warp == 10) {
+    // ------------------------------------------------ MMA issuer of tile x
+    if (lane == 0) {
+      const int x = warp == 1 ? 0 : 1;
+      const int nx = x == 0 ? nA : nB;
+      uint64_t* k_free = k_empty + x * S;
+      uint64_t* v_free = v_empty + x * S;
+      constexpr uint32_t id_qk = idesc_f16_f32(kPtTile, kPtTile);
+      constexpr uint32_t id_pv = idesc_f16_f32_bmn(kPtTile, HD);
+      const uint64_t dq0 = sdesc_k_sw128(smem_u32(smem + L::kQ));
+      const uint64_t dk0 = sdesc_k_sw128(smem_u32(smem + L::kK));
+      const uint64_t dv0 = sdesc_mn_sw128(smem_u32(smem + L::kV), L::kBlockBytes);
+      auto issue_qk = [&](int st) {
+        const uint64_t da = dq0 + static_cast<uint64_t>(x * (L::kTileBytes >> 4));
+        const uint64_t db = dk0 + static_cast<uint64_t>(st * (L::kTileBytes >> 4));
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint64_t off = static_cast<uint64_t>(((k >> 2) * L::kBlockBytes + (k & 3) * 32) >> 4);
+          mma_f16_ss(tmem + x * kPtTile, da + off, db + off, id_qk, k > 0 ? 1u : 0u);
+        }
+      };
+      auto issue_pv = [&](int st, bool accumulate) {
+        const uint64_t db = dv0 + static_cast<uint64_t>(st * (L::kTileBytes >> 4));
+#pragma unroll
+        for (int k = 0; k < kPtTile / 16; ++k)
+          mma_f16_ts(tmem + L::kColO + x * HD, tmem + L::kColP + x * L::kPStride + 8 * k,
+                     db + static_cast<uint64_t>((k * 2048) >> 4), id_pv,
+                     (accumulate || k > 0) ? 1u : 0u);
+      };
+      bool ok = mbar_wait(q_full, 0, err, kDevTimeoutFull);
+      if (ok && nx > 0) {
+        ok = mbar_wait(&k_full[0], 0, err, kDevTimeoutFull);
+        if (ok) {
+          tc_fence_after();
+          issue_qk(0);
+          mma_commit(&s_full[x]);
+          mma_commit(&k_free[0]);
+        }
+      }
+      for (int j = 0; ok && j < nx; ++j) {
+        const int st = j % S, st1 = (j + 1) % S;
+        const uint32_t par = (j / S) & 1, par1 = ((j + 1) / S) & 1;
+        const uint32_t jp = j & 1;
+        if constexpr (L::kSepP) {
+          if (j + 1 < nx) {
+            if (!mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) break;
+            if (!mbar_wait(&s_free[x], jp, err, kDevTimeoutOther)) break;
+            tc_fence_after();
+            issue_qk(st1);
+            mma_commit(&s_full[x]);
+            mma_commit(&k_free[st1]);
+          }
+          if (!mbar_wait(&v_ready[st], par, err, kDevTimeoutFull)) break;
+          if (!mbar_wait(&p_full[x], jp, err, kDevTimeoutOther)) break;
+          tc_fence_after();
+          issue_pv(st, j > 0);
+          mma_commit(&o_done[x]);
+          mma_commit(&v_free[st]);
+        } else {
+          if (!mbar_wait(&v_ready[st], par, err, kDevTimeoutFull)) break;
+          if (!mbar_wait(&p_full[x], jp, err, kDevTimeoutOther)) break;
+          tc_fence_after();
+          issue_pv(st, j > 0);
+          mma_commit(&o_done[x]);
+          mma_commit(&v_free[st]);
+          if (j + 1 < nx) {
+            // S(j+1) overwrites P(j): after the product that reads it.
+            if (!mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) break;
+            if (!mbar_wait(&o_done[x], jp, err, kDevTimeoutAccum)) break;
+            tc_fence_after();
+            issue_qk(st1);
+            mma_commit(&s_full[x]);
+            mma_commit(&k_free[st1]);
+          }
+        }
+      }
+      mma_commit(&drain[x]);
+      mbar_wait(&drain[x], 0, nullptr, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int x = (warp - 2) >> 2;
+    const int quarter = warp & 3;  // this warp's TMEM lanes [32*quarter, +32)
+    const int row = quarter * 32 + lane;
+    const int first = i0 + x * tile_tokens;
+    const int tok = first + row / group;
+    const bool owned = row < tile_tokens * group && tok < seq.n;  // a row of the batch
+    const int nx = x == 0 ? nA : nB;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + x * kPtTile;
+    const uint32_t t_p = tmem + lane_off + L::kColP + x * L::kPStride;
+    const uint32_t t_o = tmem + lane_off + L::kColO + x * HD;
+    const int lim_row = lim_of(min(tok, seq.n - 1));
+    const int lim_tile = lim_of(min(first, seq.n - 1));  // smallest of the tile
+    float m_ref = -INFINITY;  // -inf: no key seen yet
+    bool bad = false;         // a NaN or +inf among the row's scores
+    uint64_t lsum0 = 0, lsum1 = 0;
+    bool ok = true;
+    for (int j = 0; j < nx; ++j) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1, err, kDevTimeoutAccum))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int key0 = k_begin + j * kPtTile;
+      uint32_t s[kPtTile];
+#pragma unroll
+      for (int c = 0; c < kPtTile / 32; ++c)
+        tmem_ld32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+      tmem_ld_wait();
+      if constexpr (L::kSepP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[x]);
+      }
+      if (key0 + kPtTile > lim_tile) {  // warp-uniform
+        const int c0 = lim_row - key0;
+#pragma unroll
+        for (int c = 0; c < kPtTile; ++c)
+          if (c >= c0) s[c] = 0xff800000u;  // -inf
+      }
+      if (holes) {
+        uint32_t there = 0;  // bit i: keys 16 i .. 16 i + 15 exist
+#pragma unroll 1
+        for (int i = 0; i < kPtTile / 16; ++i)
+          there |= static_cast<uint32_t>(key0 + 16 * i < seq.len &&
+                                         paged_page(p, b, key0 + 16 * i) >= 0) << i;
+        if (there != 0xffu) {
+#pragma unroll
+          for (int c = 0; c < kPtTile; ++c)
+            if (!((there >> (c >> 4)) & 1u)) s[c] = 0xff800000u;
+        }
+      }
+      float mm[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        mm[i] = pt_max3(__uint_as_float(s[i]), __uint_as_float(s[i + 8]), -INFINITY);
+#pragma unroll
+      for (int c = 16; c < kPtTile; c += 16)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          mm[i] = pt_max3(mm[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
+      const float mx = pt_max3(pt_max3(mm[0], mm[1], mm[2]), pt_max3(mm[3], mm[4], mm[5]),
+                               pt_max3(mm[6], mm[7], -INFINITY));
+      const float m_new = mx * a.scale_log2;
+      bad = bad || !(m_new < INFINITY);
+      bool rescale = false;
+      float f = 1.f;
+      // (a NaN maximum compares false and leaves m_ref)
+      if (j == 0) {
+        m_ref = m_new;
+      } else if (__any_sync(0xffffffffu, m_new > m_ref + kPtRescale)) {
+        const float m_up = fmaxf(m_ref, m_new);
+        f = m_ref == m_up ? 1.f : fast_exp2(m_ref - m_up);  // m_ref -inf: 0
+        m_ref = m_up;
+        const uint64_t f2v = f2_pack(f, f);
+        lsum0 = f2_fma(lsum0, f2v, 0);
+        lsum1 = f2_fma(lsum1, f2v, 0);
+        rescale = true;
+      }
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+      const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2);
+      const uint64_t negm2 = f2_pack(-m_use, -m_use);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pr[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = 64 * half + 2 * i;
+          const uint64_t arg =
+              f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, negm2);
+          uint64_t e;
+          if ((i & 7) < kPtPoly) {
+            e = exp2_poly_f2(arg);
+          } else {
+            float a0, a1;
+            f2_unpack(arg, a0, a1);
+            e = f2_pack(fast_exp2(a0), fast_exp2(a1));
+          }
+          if (i & 1) lsum1 = f2_add(lsum1, e); else lsum0 = f2_add(lsum0, e);
+          float e0, e1;
+          f2_unpack(e, e0, e1);
+          pr[i] = pack_half2(e0, e1);
+        }
+        if (half == 0) {
+          if constexpr (L::kSepP) {
+            if (j > 0 && !__all_sync(0xffffffffu,
+                                     mbar_wait(&o_done[x], (j - 1) & 1, err, kDevTimeoutAccum))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          if (rescale) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(t_o + c, o);
+            }
+          }
+        }
+        tmem_st32(t_p + 32 * half, pr);
+      }
+      if (!ok) break;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
+    }
+    if (ok && nx > 0)
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], (nx - 1) & 1, err, kDevTimeoutAccum));
+    float la, lb, lc, ld;
+    f2_unpack(lsum0, la, lb);
+    f2_unpack(lsum1, lc, ld);
+    float l = (la + lb) + (lc + ld);
+    if (m_ref == -INFINITY) l = 0.f;  // no key seen
+    if (bad) l = __uint_as_float(0x7fc00000u);
+    if (ok) {
+      const bool fix = *cleared != 0;  // the writer arrived before the last product
+      const int head = hk * group + row % group;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = (static_cast<int64_t>(seq.row0 + tok) * (p.kv_heads * group) + head) *
+                             a.splits + split;
+      __half* dst = a.out + static_cast<int64_t>(seq.row0 + tok) * a.ld_out + head * HD;
+      if (nx > 0) tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (nx > 0) {
+          tmem_ld32(t_o + c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        float* of = reinterpret_cast<float*>(o);
+        if (owned) {
+          if (fix) {
+            for (int key = max(k_begin, lim_first - kPtTile); key < min(lim_row, k_stop); ++key) {
+              const int page = paged_page(p, b, key);
+              if (page < 0) continue;
+              const int64_t va = paged_offset(p, page, key) + hk * p.head_stride + c;
+              const float vs = kQuant ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float y = paged_value<CODE>(p.v, va + i, vs);
+                if (!isfinite(y)) of[i] += y;
+              }
+            }
+          }
+          if (is_split) {
+            float4* d4 = reinterpret_cast<float4*>(a.part_o + at * HD + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              d4[i] = make_float4(of[4 * i], of[4 * i + 1], of[4 * i + 2], of[4 * i + 3]);
+            if (c == 0) a.part_ml[at] = make_float2(m_ref, l);
+          } else {
+            uint4* d4 = reinterpret_cast<uint4*>(dst + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float* g = of + 8 * i;
+              d4[i] =
+                  make_uint4(pack_half2(g[0] * inv, g[1] * inv), pack_half2(g[2] * inv, g[3] * inv),
+                             pack_half2(g[4] * inv, g[5] * inv), pack_half2(g[6] * inv, g[7] * inv));
+            }
+          }
+        }
+        __syncwarp();  // the next tmem_ld is warp-collective
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, kPtCols);
+  }
+}
+
+template <int CODE, int HD>
+int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, int64_t tokens,
+                 cudaStream_t stream) {
+  using L = PtCfg<CODE, HD>;
+  static int done[kMaxDevices] = {0};
+  auto kern = paged_tc_kernel<CODE, HD>;
+  int st = ensure_smem(reinterpret_cast<const void*>(kern), L::kSmem, done);
+  if (st != TFX_OK) return st;
+  const int eb = code_bytes(CODE), page_rows = c->page_size < kPtTile ? c->page_size : kPtTile;
+  const uint32_t tile_tokens = static_cast<uint32_t>(kPtTile / a.group);
+  CUtensorMap tq, tk, tv;
+  const uint64_t qd[3] = {HD, static_cast<uint64_t>(p.kv_heads) * a.group,
+                          static_cast<uint64_t>(p.num_tokens)};
+  const uint64_t qs[2] = {HD * 2, static_cast<uint64_t>(a.ld_q) * 2};
+  const uint32_t qb[3] = {64, static_cast<uint32_t>(a.group), tile_tokens};
+  st = make_tmap(&tq, a.q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, qd, qs, qb,
+                 CU_TENSOR_MAP_SWIZZLE_128B);
+  // fp16: 64-column boxes in the layout of the products; 8 bit: plain rows.
+  const uint64_t kd[4] = {HD, static_cast<uint64_t>(c->page_size),
+                          static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.num_pages)};
+  const uint64_t ks[3] = {static_cast<uint64_t>(p.token_stride) * eb,
+                          static_cast<uint64_t>(p.head_stride) * eb,
+                          static_cast<uint64_t>(p.page_stride) * eb};
+  const uint32_t kb[4] = {L::kQuant ? HD : 64, static_cast<uint32_t>(page_rows), 1, 1};
+  const CUtensorMapDataType dt =
+      L::kQuant ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapSwizzle sw = L::kQuant ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+  if (st == TFX_OK) st = make_tmap(&tk, p.k, dt, 4, kd, ks, kb, sw);
+  if (st == TFX_OK) st = make_tmap(&tv, p.v, dt, 4, kd, ks, kb, sw);
+  if (st != TFX_OK) return st;
+  const int64_t blocks = (tokens + 2 * tile_tokens - 1) / (2 * tile_tokens);
+  if (blocks * a.splits > 65535)
+    return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: max_query_len is too long for the grid");
+  launch_pdl(kern, dim3(p.kv_heads, p.batch, static_cast<unsigned>(blocks * a.splits)),
+             dim3(kPtThreads), L::kSmem, stream, tq, tk, tv, p, a, static_cast<int>(blocks),
+             device_error_word());
+  return check_launch("paged_tc_kernel");
+}
+
+}  // namespace
+
+template <int CODE>
+int launch_paged_tc(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, int64_t tokens,
+                    cudaStream_t stream) {
+  return c->head_dim == 64 ? launch_tc_hd<CODE, 64>(c, p, a, tokens, stream)
+                           : launch_tc_hd<CODE, 128>(c, p, a, tokens, stream);
+}
+
+}  // namespace tfx

@@ -1,0 +1,7 @@
+// The tcgen05 paged attention kernel for e4m3 caches (paged_tc.cuh).
+#include "paged_tc.cuh"
+
+namespace tfx {
+template int launch_paged_tc<kCodeE4M3>(const tfx_paged_cache*, const Paged&, const PagedAttn&, int64_t,
+                                 cudaStream_t);
+}  // namespace tfx

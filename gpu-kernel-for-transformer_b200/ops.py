@@ -250,22 +250,26 @@ def _packed_rows(t: torch.Tensor, what: str, tokens: int, heads: int, hd: int,
     return st[0] if tokens > 1 else heads * hd
 
 
-def _paged_stream(cache: PagedKVCache, batch: PagedBatch) -> int:
-    dev = cache.device
-    if dev.type != "cuda":
+def _paged_device(cache: PagedKVCache, batch: PagedBatch) -> int:
+    """Index of the device that both live on."""
+    if not cache.device.type == "cuda":
         raise ValueError("the paged cache requires CUDA tensors")
-    if batch.device != dev:
+    if batch.device != cache.device:
         raise ValueError("batch and cache must be on one device")
-    return torch.cuda.current_stream(dev).cuda_stream
+    return cache.device.index
 
 
-def _call_on(device: torch.device, what: str, fn, *args) -> None:
-    """fn(*args) with ``device`` as the current one (the library launches there)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        _lib.check(fn(*args), what)
-        return
-    with torch.cuda.device(device):
-        _lib.check(fn(*args), what)
+def _call_on(index: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) on device ``index`` and its current stream. (The raw
+    handle: a decode step's calls are short, and a Stream object costs 2 us.)"""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status, what)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: PagedBatch) -> None:
@@ -280,14 +284,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: P
     of them is kept. The paged form of the reference's ``_append_kv_cache``
     (torch_transformer_benchmark.py:426-462).
     """
-    stream = _paged_stream(cache, batch)
-    n, heads, hd = batch.num_tokens, cache.kv_heads, cache.head_dim
-    ld_k = _packed_rows(k, "k", n, heads, hd, cache.device)
-    ld_v = _packed_rows(v, "v", n, heads, hd, cache.device)
-    if n == 0:
-        return
-    _call_on(cache.device, "tfx_paged_append", _lib.load().tfx_paged_append, k.data_ptr(), ld_k,
-             v.data_ptr(), ld_v, cache._ref, batch._ref, stream)
+    index = _paged_device(cache, batch)
+    n, heads, hd, dev = batch.num_tokens, cache.kv_heads, cache.head_dim, cache.device
+    ld_k = _packed_rows(k, "k", n, heads, hd, dev)
+    ld_v = _packed_rows(v, "v", n, heads, hd, dev)
+    if n:
+        _call_on(index, "tfx_paged_append", _lib.load().tfx_paged_append, k.data_ptr(), ld_k,
+                 v.data_ptr(), ld_v, cache._ref, batch._ref)
 
 
 def paged_read(
@@ -302,17 +305,19 @@ def paged_read(
     give code * scale, rounded once. Tokens without a page read as zeros; rows
     that belong to no sequence are not written. ``out``: write into these two.
     """
-    stream = _paged_stream(cache, batch)
-    n, heads, hd = batch.num_tokens, cache.kv_heads, cache.head_dim
+    index = _paged_device(cache, batch)
+    n, heads, hd, dev = batch.num_tokens, cache.kv_heads, cache.head_dim, cache.device
     if out is None:
-        out = tuple(torch.empty((n, heads, hd), dtype=torch.float16, device=cache.device)
-                    for _ in range(2))
-    k, v = out
-    ld_k = _packed_rows(k, "out[0]", n, heads, hd, cache.device)
-    ld_v = _packed_rows(v, "out[1]", n, heads, hd, cache.device)
+        k = torch.empty((n, heads, hd), dtype=torch.float16, device=dev)
+        v = torch.empty_like(k)
+        ld_k = ld_v = heads * hd
+    else:
+        k, v = out
+        ld_k = _packed_rows(k, "out[0]", n, heads, hd, dev)
+        ld_v = _packed_rows(v, "out[1]", n, heads, hd, dev)
     if n:
-        _call_on(cache.device, "tfx_paged_read", _lib.load().tfx_paged_read, cache._ref,
-                 batch._ref, k.data_ptr(), ld_k, v.data_ptr(), ld_v, stream)
+        _call_on(index, "tfx_paged_read", _lib.load().tfx_paged_read, cache._ref, batch._ref,
+                 k.data_ptr(), ld_k, v.data_ptr(), ld_v)
     return k, v
 
 
@@ -337,32 +342,34 @@ def paged_attention(
     prompt may share a batch. The paged form of the cached attention of
     torch_transformer_benchmark.py:747-765.
     """
-    stream = _paged_stream(cache, batch)
-    n, hd = batch.num_tokens, cache.head_dim
+    index = _paged_device(cache, batch)
+    n, hd, dev = batch.num_tokens, cache.head_dim, cache.device
     if q.ndim != 3:
         raise ValueError("q must be [num_tokens, q_heads, head_dim]")
     heads = q.shape[1]
-    ld_q = _packed_rows(q, "q", n, heads, hd, cache.device)
+    ld_q = _packed_rows(q, "q", n, heads, hd, dev)
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"q_heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
+    ld_out = heads * hd
     if out is None:
-        out = torch.empty((n, heads * hd), dtype=torch.float16, device=cache.device)
-    elif out.shape != (n, heads * hd) or out.dtype != torch.float16 or \
-            out.device != cache.device or (n > 0 and out.stride(1) != 1):
+        out = torch.empty((n, ld_out), dtype=torch.float16, device=dev)
+    elif out.shape != (n, ld_out) or out.dtype != torch.float16 or out.device != dev or \
+            (n > 0 and out.stride(1) != 1):
         raise ValueError("out must be float16 [num_tokens, q_heads * head_dim] with contiguous rows")
+    elif n > 1:
+        ld_out = out.stride(0)
     if n == 0:
         return out
     lib = _lib.load()
     need = lib.tfx_paged_attention_workspace_bytes(cache._ref, batch._ref, heads)
-    if need < 0:
-        raise ValueError("tfx_paged_attention: " + lib.tfx_last_error_message().decode())
-    # A workspace of its own for each call, from the stream's allocator: calls on
-    # different streams, and graphs captured apart, never share one.
-    ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
-    _call_on(cache.device, "tfx_paged_attention", lib.tfx_paged_attention, q.data_ptr(), ld_q,
-             cache._ref, batch._ref, out.data_ptr(), out.stride(0) if n > 1 else heads * hd, heads,
-             hd ** -0.5 if scale is None else float(scale), int(is_causal),
-             ws.data_ptr() if need else None, need, stream)
+    ws = None
+    if need > 0:
+        # A workspace of its own for each call, from the stream's allocator: calls
+        # on different streams, and graphs captured apart, never share one.
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call_on(index, "tfx_paged_attention", lib.tfx_paged_attention, q.data_ptr(), ld_q, cache._ref,
+             batch._ref, out.data_ptr(), ld_out, heads, hd ** -0.5 if scale is None else float(scale),
+             int(is_causal), None if ws is None else ws.data_ptr(), max(need, 0))
     return out
 
 
