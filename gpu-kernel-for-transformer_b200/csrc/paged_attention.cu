@@ -153,15 +153,18 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   int64_t kv = static_cast<int64_t>(b->max_pages) * c->page_size;
   if (b->max_kv_len < kv) kv = b->max_kv_len;
   if (kv < 1) kv = 1;
-  // mma.sync: four CTAs to an SM (one at 512-byte rows); a start costs about
+  // mma.sync: CTAs to an SM by registers and shared memory; a start costs about
   // as much as 400 keys, a second launch to join as much as 512.
-  const int64_t slots = num_sms() * (hd * (c->dtype == TFX_CACHE_F16 ? 2 : 1) >= 512 ? 1 : 4);
+  const int row_bytes = hd * (c->dtype == TFX_CACHE_F16 ? 2 : 1);
+  const int64_t slots = num_sms() * (row_bytes >= 512 ? 1 : pl.block_rows >= 32 ? 2 :
+                                     pl.block_rows == 16 || row_bytes == 256 ? 3 : 4);
   const int64_t blocks = pairs * ((small_rows + pl.block_rows - 1) / pl.block_rows);
   double alone = 0., joined = 0.;
   const int64_t share = cut(blocks, slots, kv, 400, 128, 8, &alone);
   // (beside the tcgen05 kernel few splits: its many rows are joined by the same kernel)
   const int64_t parts = cut(blocks, slots, kv, 400, kSplitKeys, pl.tc ? 8 : 1024, &joined);
-  if (!pl.tc && alone <= joined + 512.) {
+  // (CTAs of a cluster wait for one another at its end: for one wave only)
+  if (!pl.tc && alone <= joined + 512. && (share == 1 || 4 * blocks * share <= 5 * slots)) {
     pl.cluster = share > 1 ? static_cast<int>(share) : 0;
     pl.kps = round_keys(kv, 1);
   } else {

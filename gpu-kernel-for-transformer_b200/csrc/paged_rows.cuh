@@ -239,49 +239,62 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
   const uint8_t* kb = static_cast<const uint8_t*>(p.k) + hk * p.head_stride * code_bytes(CODE);
   const uint8_t* vb = static_cast<const uint8_t*>(p.v) + hk * p.head_stride * code_bytes(CODE);
   auto tile_key = [&](int i) { return k_begin + (i * W + warp) * KT; };
-  // Page of this lane's keys of tile i (lane and lane + 32), one tile ahead.
-  int pg[2];
+  // Pages of this lane's keys of tile i (lane and lane + 32), one tile ahead.
+  const int32_t* table = p.table + b * p.table_stride;
+  int pg[KW];
   auto look_up = [&](int i) {
-    const int key = tile_key(i) + lane;
-    pg[0] = i < n_tiles && key < k_end && lane < KT ? paged_page(p, b, key) : -1;
-    if constexpr (KT > 32)
-      pg[1] = i < n_tiles && key + 32 < k_end ? paged_page(p, b, key + 32) : -1;
-  };
-  auto load = [&](int i) {
-    uint8_t* st = ring + (i % NS) * C::kStageBytes;
-    const int k0 = tile_key(i);
 #pragma unroll
-    for (int it = 0; it < (KT * U + 31) / 32; ++it) {
-      const int c = it * 32 + lane, r = c / U, col = c % U;
-      int page = __shfl_sync(0xffffffffu, pg[0], r & 31);
-      if constexpr (KT > 32) {
-        const int hi = __shfl_sync(0xffffffffu, pg[1], r & 31);
-        page = r < 32 ? page : hi;
-      }
-      if (KT * U % 32 == 0 || c < KT * U) {
-        const int64_t off = page >= 0 ? paged_offset(p, page, k0 + r) * code_bytes(CODE) : 0;
-        rows_cp16(smem_u32(st + r * C::kPitch + col * 16), kb + off + col * 16, page >= 0);
-        rows_cp16(smem_u32(st + C::kTileBytes + r * C::kPitch + col * 16), vb + off + col * 16,
-                  page >= 0);
+    for (int u = 0; u < KW; ++u) {
+      const int key = tile_key(i) + 32 * u + lane;
+      int page = -1;
+      if (i < n_tiles && key < k_end && (KT % 32 == 0 || lane < KT)) page = table[key >> p.page_shift];
+      pg[u] = static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages) ? page : -1;
+    }
+  };
+  // 16 keys lie in one page. Lane = (row of it, 16-byte chunk); a pass covers
+  // 32 / U rows.
+  constexpr int RP = 32 / U;  // rows of a pass
+  const int64_t row_step = p.token_stride * code_bytes(CODE);
+  const int64_t lane_off = (lane / U) % 16 * row_step + (lane % U) * 16;
+  const uint32_t lane_dst = smem_u32(ring) + (lane / U) * C::kPitch + (lane % U) * 16;
+  auto load = [&](int i) {
+    const uint32_t st = (i % NS) * C::kStageBytes;
+    const int k0 = tile_key(i);
+    // Byte offset of this lane's group of 16 keys, negative without a page.
+    int64_t base[KW];
+#pragma unroll
+    for (int u = 0; u < KW; ++u)
+      base[u] = pg[u] < 0 ? -1
+                          : paged_offset(p, pg[u], (k0 + 32 * u + lane) & ~15) * code_bytes(CODE);
+#pragma unroll
+    for (int it = 0; it < KT / RP + (KT % RP != 0); ++it) {
+      const int first = it * RP;  // row of lane 0
+      // (a pass of 32 rows holds two groups)
+      const int src = RP == 32 ? lane & 16 : (first & 16);
+      const int64_t from = __shfl_sync(0xffffffffu, base[first / 32], src);
+      const bool ok = from >= 0 && k0 + first + lane / U < k_end;
+      const int64_t off = (ok ? from + (first % 16) * row_step : 0) + lane_off;
+      if (KT % RP == 0 || lane / U < KT) {
+        rows_cp16(lane_dst + st + first * C::kPitch, kb + off, ok);
+        rows_cp16(lane_dst + st + C::kTileBytes + first * C::kPitch, vb + off, ok);
       }
     }
+    uint8_t* at = ring + st + 2 * C::kTileBytes;
     if constexpr (kQuant) {
-      float* sc = reinterpret_cast<float*>(st + 2 * C::kTileBytes);
 #pragma unroll
       for (int u = 0; u < KW; ++u) {
-        if (lane + 32 * u < KT) {
+        if (KT % 32 == 0 || lane < KT) {
           const bool ok = pg[u] >= 0;
           const int64_t so = ok ? paged_scale_offset(p, pg[u], hk, k0 + 32 * u + lane) : 0;
-          rows_cp4(smem_u32(sc + 32 * u + lane), p.k_scale + so, ok);
-          rows_cp4(smem_u32(sc + KT + 32 * u + lane), p.v_scale + so, ok);
+          rows_cp4(smem_u32(at) + (32 * u + lane) * 4, p.k_scale + so, ok);
+          rows_cp4(smem_u32(at) + (KT + 32 * u + lane) * 4, p.v_scale + so, ok);
         }
       }
     }
-    uint32_t* bits = reinterpret_cast<uint32_t*>(st + 2 * C::kTileBytes + C::kScaleBytes);
 #pragma unroll
     for (int u = 0; u < KW; ++u) {
       const uint32_t m = __ballot_sync(0xffffffffu, pg[u] >= 0);
-      if (lane == 0) bits[u] = m;
+      if (lane == 0) reinterpret_cast<uint32_t*>(at + C::kScaleBytes)[u] = m;
     }
   };
   look_up(0);
@@ -457,28 +470,42 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
         }
     }
     bool grow = kQuant && __uint_as_float(top) > unit * kRowsUnit;
-    float mx[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int kk = j * 16 + g + 8 * r;
         float f = a.scale_log2;
-        if constexpr (kQuant) f *= sc[kk];
-        const bool there = !need_mask || ((bits[kk >> 5] >> (kk & 31)) & 1u);
+        if constexpr (kQuant) f *= sc[j * 16 + g + 8 * r];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float val = s[nt][j][2 * r + e] * f;
-            if (need_mask && (!there || k0 + kk >= lim[nt][e])) val = -INFINITY;
-            s[nt][j][2 * r + e] = val;
-            mx[nt][e] = fmaxf(mx[nt][e], val);
-          }
+        for (int nt = 0; nt < NT; ++nt) {
+          s[nt][j][2 * r] *= f;
+          s[nt][j][2 * r + 1] *= f;
+        }
       }
     }
+    if (need_mask) {
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int kk = j * 16 + g + 8 * r;
+          const int key = (bits[kk >> 5] >> (kk & 31)) & 1u ? k0 + kk : 0x7fffffff;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (key >= lim[nt][e]) s[nt][j][2 * r + e] = -INFINITY;
+        }
+    }
+    float mx[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[nt][e] = fmaxf(s[nt][0][e], s[nt][0][2 + e]);
+#pragma unroll
+        for (int j = 1; j < KB; ++j) mx[nt][e] = fmax3(mx[nt][e], s[nt][j][e], s[nt][j][2 + e]);
+      }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
       grow = grow || mx[nt][0] > m_ref[nt][0] + kRowsRescale || mx[nt][1] > m_ref[nt][1] + kRowsRescale;
@@ -532,8 +559,16 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
           for (int e = 0; e < 2; ++e) {
             w[e] = fast_exp2(s[nt][j][2 * r + e] - m_use[e]);
             l_run[nt][e] += w[e];
-            // a masked key's scale may be anything
-            if constexpr (kQuant) w[e] = w[e] == 0.f ? 0.f : w[e] * (vs[j][r] * inv_unit);
+            if constexpr (kQuant) {
+              s[nt][j][2 * r + e] = w[e];
+              w[e] *= vs[j][r] * inv_unit;
+            }
+          }
+          if constexpr (kQuant) {
+            if (need_mask) {  // a masked key's scale may be anything
+              if (s[nt][j][2 * r] == 0.f) w[0] = 0.f;
+              if (s[nt][j][2 * r + 1] == 0.f) w[1] = 0.f;
+            }
           }
           pf[nt][j][r] = rows_movm_t(pack_half2(w[0], w[1]));
         }

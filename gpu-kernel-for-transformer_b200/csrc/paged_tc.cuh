@@ -6,23 +6,28 @@
 // tile: a 128-row tile holds 128 / group tokens x group heads (TMA box of q;
 // the last 128 % group rows stay unused). CTA = two such tiles A and B of one
 // (sequence, key/value head) that share every 128-key tile, and one range of
-// the keys; 12 warps, one CTA per SM:
+// the keys; 12 warps (8 bit: 16), one CTA per SM:
 //   warps 2..5, 6..9  softmax of A and of B; thread = row = TMEM lane
 //   warps 1, 10       MMA issuers of A and of B (one lane)
 //   fp16:  warp 0 loads K and V, a TMA box per page and 64 columns (lane =
 //          box); warp 11 looks after V tiles that hold keys which not every
 //          row sees
-//   8 bit: warps 0 and 11 each expand half of every K and V tile from a ring
-//          of raw tiles (TMA, a box per page; warp 0 issues it) to fp16
+//   8 bit: warp 0 loads raw tiles (a box per page), warps 11..14 expand 32 rows
+//          each of every K and V tile to fp16, a lane per row (both tiles are
+//          swizzled: no bank conflicts)
 // A key tile is 128 consecutive positions, 128 / page_size pages or half of
 // one; pages outside the pool are boxes outside the tensor map and read as
 // zeros.
 //
-// Products, TMEM columns and the lazy rescaling of O are those of the
-// contiguous kernel (attention_tc.cu): S = Q K^T and O += P V with P from TMEM
-// and V MN-major from the row-major tile. S needs 128x128xHD products for every
-// exponential row of 128, which the softmax warps bound at head_dim 64; MN-major
-// V costs tensor time that is hidden behind them.
+// S = Q K^T (128 x N keys) goes to TMEM, the softmax warps write P over it or
+// beside it, O += P V takes P from TMEM and V MN-major from the row-major tile.
+// A row's reference maximum moves only when it is exceeded by more than 2^8
+// (O is then rescaled in TMEM). head_dim 64: N = 128 and P has columns of its
+// own (S 2 x 128, P 2 x 64, O 2 x 64), so the next S is computed while this one's
+// P is. head_dim 128: O fills half of TMEM and P lies over S; N = 64, so that
+// one half of a tile's S is being exponentiated while the other is multiplied
+// and replaced (with N = 128 each tile's chain S - P - PV - S was serial: 5000
+// against 2800 cycles of products for a pair of tiles).
 //
 // 8-bit values are expanded as code * scale in fp16. The scale s is used as
 // m * 2^k with an fp16 m: int8 codes are placed behind the exponent of
@@ -43,7 +48,7 @@
 namespace tfx {
 namespace {
 
-constexpr int kPtThreads = 384;
+constexpr int kPtConvert = 4;  // 8 bit: warps that expand
 constexpr int kPtTile = 128;
 constexpr float kPtRescale = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8
 constexpr int kPtPoly = 2;          // of 8 pairs of exponentials, on the FMA pipe
@@ -52,6 +57,7 @@ constexpr uint32_t kPtCols = 512;
 template <int CODE, int HD>
 struct PtCfg {
   static constexpr bool kQuant = CODE != kCodeF16;
+  static constexpr int kThreads = kQuant ? 512 : 384;
   static constexpr int kStages = HD == 64 ? 4 : 2;
   static constexpr int kBlocks = HD / 64;
   static constexpr int kBlockBytes = kPtTile * 128;
@@ -64,7 +70,9 @@ struct PtCfg {
   static constexpr int kR = kV + kStages * kTileBytes;
   static constexpr int kBar = kR + kRaws * kRawBytes;
   static constexpr int kSmem = kBar + 512 + 1024;  // barriers + alignment slack
-  static constexpr bool kSepP = HD == 64;          // P has its own TMEM columns
+  static constexpr bool kSepP = false;          // P has its own TMEM columns
+  static constexpr int kParts = kSepP ? 1 : 2;     // a tile's S in so many parts
+  static constexpr int kKeys = kPtTile / kParts;   // keys of one
   static constexpr uint32_t kColP = kSepP ? 2 * kPtTile : 0;
   static constexpr uint32_t kPStride = kSepP ? kPtTile / 2 : kPtTile;
   static constexpr uint32_t kColO = kSepP ? 3 * kPtTile : 2 * kPtTile;
@@ -126,7 +134,7 @@ struct PtExpand {
 };
 
 template <int CODE, int HD>
-__global__ void __launch_bounds__(kPtThreads, 1)
+__global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Paged p,
                     const __grid_constant__ PagedAttn a, int row_blocks, int* err) {
@@ -175,16 +183,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* v_ready = v_full + S;       // V may be multiplied
   uint64_t* k_empty = v_ready + S;      // [2][S]
   uint64_t* v_empty = k_empty + 2 * S;  // [2][S]
-  uint64_t* s_full = v_empty + 2 * S;   // [2]
-  uint64_t* s_free = s_full + 2;        // [2], separate P only
-  uint64_t* p_full = s_free + 2;        // [2]
-  uint64_t* o_done = p_full + 2;        // [2]
-  uint64_t* drain = o_done + 2;         // [2]
+  constexpr int N = L::kParts;
+  uint64_t* s_full = v_empty + 2 * S;   // [2][N]
+  uint64_t* s_free = s_full + 2 * N;    // [2], separate P only
+  uint64_t* p_full = s_free + 2;        // [2][N]
+  uint64_t* o_done = p_full + 2 * N;    // [2][N]
+  uint64_t* drain = o_done + 2 * N;     // [2]
   uint64_t* r_full = drain + 2;         // [R] raw tile loaded
-  uint64_t* r_empty = r_full + R;       // [R] raw tile read by both warps
+  uint64_t* r_empty = r_full + R;       // [R] raw tile expanded by all its warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + R);
   volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
-  static_assert((1 + 7 * S + 10 + 2 * R) * 8 + 8 <= 512, "barrier space");
+  static_assert((1 + 7 * S + 4 + 6 * N + 2 * R) * 8 + 8 <= 512, "barrier space");
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q);
@@ -192,24 +201,26 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     prefetch_tmap(&tm_v);
     mbar_init(q_full, 1);
     for (int s = 0; s < S; ++s) {
-      mbar_init(&k_full[s], kQuant ? 2 : 1);
+      mbar_init(&k_full[s], kQuant ? kPtConvert : 1);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_ready[s], kQuant ? 2 : 1);
+      mbar_init(&v_ready[s], kQuant ? kPtConvert : 1);
       for (int x = 0; x < 2; ++x) {
         mbar_init(&k_empty[x * S + s], 1);
         mbar_init(&v_empty[x * S + s], 1);
       }
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_full[x], 1);
       mbar_init(&s_free[x], 4);
-      mbar_init(&p_full[x], 4);
-      mbar_init(&o_done[x], 1);
       mbar_init(&drain[x], 1);
+      for (int h = 0; h < N; ++h) {
+        mbar_init(&s_full[x * N + h], 1);
+        mbar_init(&p_full[x * N + h], 4);
+        mbar_init(&o_done[x * N + h], 1);
+      }
     }
     for (int r = 0; r < R; ++r) {
       mbar_init(&r_full[r], 1);
-      mbar_init(&r_empty[r], 2);
+      mbar_init(&r_empty[r], kPtConvert);
     }
     *cleared = 0;
     fence_mbar_init();
@@ -223,7 +234,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   {
     const int last = min(k_stop, min(seq.len, lim_of(min(i0 + 2 * tile_tokens, seq.n) - 1)));
     for (int pos = k_begin + (static_cast<int>(threadIdx.x) << p.page_shift); pos < last;
-         pos += kPtThreads << p.page_shift)
+         pos += L::kThreads << p.page_shift)
       hole |= paged_page(p, b, pos) < 0;
   }
   tc_fence_before();
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
   };
 
-  if (warp == 0 || warp == 11) {
+  if (warp == 0 || warp >= 11) {
     if constexpr (!kQuant) {
       if (warp == 0) {
         // -------------------------------------------------- TMA of K and V
@@ -299,7 +310,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           mbar_wait(&k_full[j % S], (j / S) & 1, nullptr, 0);
         for (int j = max(0, issued - S); j < issued; ++j)
           mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, 0);
-      } else {
+      } else if (warp == 11) {
         // ---------------------------------------------- V tiles not all see
         for (int j = 0; j < n_iter; ++j) {
           const int st = j % S, key0 = k_begin + j * kPtTile;
@@ -329,105 +340,89 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       }
     } else {
-      // ------------------------------------------- raw tiles, expanded to fp16
-      const int half = warp == 0 ? 0 : 1;  // rows 64 * half .. + 63 of every tile
-      const int total = 2 * n_iter;
-      int raw_issued = 0;
-      int part_page = 0, part_next = 0;  // warp 0: this lane's page of the next raw tiles
+      const int total = 2 * n_iter;  // raw tiles: K and V in turn
       if (warp == 0) {
+        // ------------------------------------------------ TMA of raw tiles
         load_q();
-        part_page = page_coord(0, lane % tile_pages);
-        part_next = page_coord(1, lane % tile_pages);
-      }
-      auto issue_raw = [&]() {  // warp 0: tile raw_issued / 2, K if even
-        const int e = raw_issued++, j = e >> 1;
-        if (lane == 0) mbar_arrive_expect_tx(&r_full[e % R], L::kRawBytes);
-        __syncwarp();
-        if (lane < tile_pages)
-          pt_load_4d(smem_u32(smem + L::kR + (e % R) * L::kRawBytes) + lane * page_rows * HD,
-                     (e & 1) ? &tm_v : &tm_k, &r_full[e % R], 0, slot_coord(j, lane), hk, part_page);
-        if (e & 1) {
-          part_page = part_next;
-          part_next = page_coord(j + 2, lane % tile_pages);
+        const int part = lane % tile_pages;
+        const uint32_t dst = smem_u32(smem + L::kR) + part * page_rows * HD;
+        int page = page_coord(0, part), next = page_coord(1, part), issued = 0;
+        for (int e = 0; e < total; ++e) {
+          const int j = e >> 1;
+          if (e >= R && !__all_sync(0xffffffffu, mbar_wait(&r_empty[e % R], ((e / R) - 1) & 1, err,
+                                                           kDevTimeoutEmpty)))
+            break;
+          if (lane == 0) mbar_arrive_expect_tx(&r_full[e % R], L::kRawBytes);
+          __syncwarp();
+          if (lane < tile_pages)
+            pt_load_4d(dst + (e % R) * L::kRawBytes, (e & 1) ? &tm_v : &tm_k, &r_full[e % R], 0,
+                       slot_coord(j, part), hk, page);
+          issued = e + 1;
+          if (e & 1) {
+            page = next;
+            next = page_coord(j + 2, part);
+          }
         }
-      };
-      if (warp == 0)
-        while (raw_issued < min(R, total)) issue_raw();
-      // Scales of this lane's two rows (lane, lane + 32 of the warp's half) of
-      // tile j, K and V; loaded a tile ahead.
-      float sc[2][2];
-      auto load_scales = [&](int j) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int key = k_begin + j * kPtTile + half * 64 + 32 * u + lane;
+        // Our own copies land before the CTA may exit.
+        mbar_wait(q_full, 0, nullptr, 0);
+        for (int e = max(0, issued - R); e < issued; ++e)
+          mbar_wait(&r_full[e % R], (e / R) & 1, nullptr, 0);
+      } else if (warp < 11 + kPtConvert) {
+        // ------------------------------------------------- expansion to fp16
+        const int r = (warp - 11) * 32 + lane;  // this lane's row of every tile
+        float sc[2];                            // its scales in K and V, a tile ahead
+        auto load_scales = [&](int j) {
+          const int key = k_begin + j * kPtTile + r;
           const int page = j < n_iter && key < seq.len ? paged_page(p, b, key) : -1;
           const int64_t so = page >= 0 ? paged_scale_offset(p, page, hk, key) : 0;
-          sc[0][u] = page >= 0 ? p.k_scale[so] : 0.f;
-          sc[1][u] = page >= 0 ? p.v_scale[so] : 0.f;
-        }
-      };
-      load_scales(0);
-      bool ok = true;
-      for (int j = 0; ok && j < n_iter; ++j) {
-        const int st = j % S, key0 = k_begin + j * kPtTile;
-        uint32_t pk[2][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          pk[0][u] = pt_scale<CODE>(sc[0][u]);
-          pk[1][u] = pt_scale<CODE>(sc[1][u]);
-        }
-        load_scales(j + 1);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const int e = 2 * j + kv;
-          // Refill the raw tile before this one (both warps are through with it).
-          if (warp == 0 && e > 0 && raw_issued < total) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&r_empty[(e - 1) % R], ((e - 1) / R) & 1, err,
-                                                   kDevTimeoutEmpty));
-            if (!ok) break;
-            issue_raw();
-          }
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) &&
-               stage_free(kv ? v_empty : k_empty, j);
-          if (!ok) break;
-          const uint8_t* raw = smem + L::kR + (e % R) * L::kRawBytes;
-          uint8_t* tile = smem + (kv ? L::kV : L::kK) + st * L::kTileBytes;
-          const bool partly = kv == 1 && key0 + kPtTile > lim_first;  // not every row sees all
-          constexpr int CPR = HD / 16;            // 16-code chunks of a row
-          constexpr int RPP = 32 / CPR;           // rows of a pass
-          const int c = lane % CPR;
+          sc[0] = page >= 0 ? p.k_scale[so] : 0.f;
+          sc[1] = page >= 0 ? p.v_scale[so] : 0.f;
+        };
+        load_scales(0);
+        // Raw rows of 128 bytes: 16-byte chunk c at c ^ (r & 7); of 64 bytes: at
+        // c ^ (r >> 1 & 3). fp16 rows: chunk c of a 64-column block at c ^ (r & 7).
+        const uint32_t rx = HD == 128 ? (r & 7) << 4 : ((r >> 1) & 3) << 4;
+        const uint32_t dx = (r & 7) << 4;
+        for (int e = 0; e < total; ++e) {
+          const int j = e >> 1, kv = e & 1, st = j % S, key0 = k_begin + j * kPtTile;
+          const PtExpand<CODE> expand(pt_scale<CODE>(kv ? sc[1] : sc[0]));
+          if (kv) load_scales(j + 1);
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) ||
+              !stage_free(kv ? v_empty : k_empty, j))
+            break;
+          const uint8_t* src = smem + L::kR + (e % R) * L::kRawBytes + r * HD;
+          uint8_t* dst = smem + (kv ? L::kV : L::kK) + st * L::kTileBytes + r * 128;
+          const bool partly = kv && key0 + kPtTile > lim_first;  // not every row sees all
+          const bool behind = partly && key0 + r >= seq.len;
           bool found = false;
-#pragma unroll 4
-          for (int ps = 0; ps < 64 / RPP; ++ps) {
-            const int rl = ps * RPP + lane / CPR;  // row of the warp's half
-            const int r = half * 64 + rl;
-            const uint32_t lo = __shfl_sync(0xffffffffu, pk[kv][0], rl & 31);
-            const uint32_t hi = __shfl_sync(0xffffffffu, pk[kv][1], rl & 31);
-            const PtExpand<CODE> expand(ps * RPP < 32 ? lo : hi);
-            const uint4 x = *reinterpret_cast<const uint4*>(raw + r * HD + c * 16);
-            uint32_t w[8];
-            expand(x.x, w[0], w[1]);
-            expand(x.y, w[2], w[3]);
-            expand(x.z, w[4], w[5]);
-            expand(x.w, w[6], w[7]);
-            if (partly) {
-              const bool behind = key0 + r >= seq.len;
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const bool hit = h2_clear(w[i]);
-                found |= hit && !behind;
-                if (behind) w[i] = 0u;
+          for (int c0 = 0; c0 < HD / 16; c0 += 4) {
+            uint4 x[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              x[c] = *reinterpret_cast<const uint4*>(src + (((c0 + c) << 4) ^ rx));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t w[8];
+              expand(x[c].x, w[0], w[1]);
+              expand(x[c].y, w[2], w[3]);
+              expand(x[c].z, w[4], w[5]);
+              expand(x[c].w, w[6], w[7]);
+              if (partly) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const bool hit = h2_clear(w[i]);
+                  found |= hit && !behind;
+                  if (behind) w[i] = 0u;
+                }
               }
+              uint8_t* row = dst + (c0 >> 2) * L::kBlockBytes;
+              *reinterpret_cast<uint4*>(row + (((2 * c) << 4) ^ dx)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(row + (((2 * c + 1) << 4) ^ dx)) =
+                  make_uint4(w[4], w[5], w[6], w[7]);
             }
-            // fp16 chunks 2c and 2c+1 of the row, swizzled; lanes of the second
-            // 64-column block store theirs in the other order (banks).
-            uint8_t* row = tile + (c >> 2) * L::kBlockBytes + r * 128;
-            const int sub = c >> 2;
-            const uint4 y0 = make_uint4(w[0], w[1], w[2], w[3]), y1 = make_uint4(w[4], w[5], w[6], w[7]);
-            const int ch = 2 * (c & 3);
-            *reinterpret_cast<uint4*>(row + (((ch + sub) ^ (r & 7)) << 4)) = sub ? y1 : y0;
-            *reinterpret_cast<uint4*>(row + (((ch + 1 - sub) ^ (r & 7)) << 4)) = sub ? y0 : y1;
           }
           if (found) *cleared = 1;
           fence_proxy_async_smem();
@@ -438,11 +433,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
         }
       }
-      if (warp == 0) {  // our own copies land before the CTA may exit
-        mbar_wait(q_full, 0, nullptr, 0);
-        for (int e = max(0, raw_issued - R); e < raw_issued; ++e)
-          mbar_wait(&r_full[e % R], (e / R) & 1, nullptr, 0);
-      }
     }
   } else if (warp == 1 || warp == 10) {
     // ------------------------------------------------ MMA issuer of tile x
@@ -451,35 +441,41 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const int nx = x == 0 ? nA : nB;
       uint64_t* k_free = k_empty + x * S;
       uint64_t* v_free = v_empty + x * S;
-      constexpr uint32_t id_qk = idesc_f16_f32(kPtTile, kPtTile);
+      constexpr uint32_t id_qk = idesc_f16_f32(kPtTile, L::kKeys);
       constexpr uint32_t id_pv = idesc_f16_f32_bmn(kPtTile, HD);
       const uint64_t dq0 = sdesc_k_sw128(smem_u32(smem + L::kQ));
       const uint64_t dk0 = sdesc_k_sw128(smem_u32(smem + L::kK));
       const uint64_t dv0 = sdesc_mn_sw128(smem_u32(smem + L::kV), L::kBlockBytes);
-      auto issue_qk = [&](int st) {
+      // Part h of a tile: rows 64 h .. of K and of V, columns 64 h .. of S.
+      auto issue_qk = [&](int st, int h) {
         const uint64_t da = dq0 + static_cast<uint64_t>(x * (L::kTileBytes >> 4));
-        const uint64_t db = dk0 + static_cast<uint64_t>(st * (L::kTileBytes >> 4));
+        const uint64_t db =
+            dk0 + static_cast<uint64_t>((st * L::kTileBytes + h * L::kKeys * 128) >> 4);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint64_t off = static_cast<uint64_t>(((k >> 2) * L::kBlockBytes + (k & 3) * 32) >> 4);
-          mma_f16_ss(tmem + x * kPtTile, da + off, db + off, id_qk, k > 0 ? 1u : 0u);
+          mma_f16_ss(tmem + x * kPtTile + h * L::kKeys, da + off, db + off, id_qk, k > 0 ? 1u : 0u);
         }
+        mma_commit(&s_full[x * N + h]);
       };
-      auto issue_pv = [&](int st, bool accumulate) {
-        const uint64_t db = dv0 + static_cast<uint64_t>(st * (L::kTileBytes >> 4));
+      auto issue_pv = [&](int st, int h, bool accumulate) {
+        const uint64_t db =
+            dv0 + static_cast<uint64_t>((st * L::kTileBytes + h * L::kKeys * 128) >> 4);
 #pragma unroll
-        for (int k = 0; k < kPtTile / 16; ++k)
-          mma_f16_ts(tmem + L::kColO + x * HD, tmem + L::kColP + x * L::kPStride + 8 * k,
+        for (int k = 0; k < L::kKeys / 16; ++k)
+          mma_f16_ts(tmem + L::kColO + x * HD,
+                     tmem + L::kColP + x * L::kPStride + h * L::kKeys + 8 * k,
                      db + static_cast<uint64_t>((k * 2048) >> 4), id_pv,
                      (accumulate || k > 0) ? 1u : 0u);
+        mma_commit(&o_done[x * N + h]);
       };
       bool ok = mbar_wait(q_full, 0, err, kDevTimeoutFull);
       if (ok && nx > 0) {
         ok = mbar_wait(&k_full[0], 0, err, kDevTimeoutFull);
         if (ok) {
           tc_fence_after();
-          issue_qk(0);
-          mma_commit(&s_full[x]);
+#pragma unroll
+          for (int h = 0; h < N; ++h) issue_qk(0, h);
           mma_commit(&k_free[0]);
         }
       }
@@ -492,31 +488,32 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (!mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) break;
             if (!mbar_wait(&s_free[x], jp, err, kDevTimeoutOther)) break;
             tc_fence_after();
-            issue_qk(st1);
-            mma_commit(&s_full[x]);
+            issue_qk(st1, 0);
             mma_commit(&k_free[st1]);
           }
           if (!mbar_wait(&v_ready[st], par, err, kDevTimeoutFull)) break;
           if (!mbar_wait(&p_full[x], jp, err, kDevTimeoutOther)) break;
           tc_fence_after();
-          issue_pv(st, j > 0);
-          mma_commit(&o_done[x]);
+          issue_pv(st, 0, j > 0);
           mma_commit(&v_free[st]);
         } else {
           if (!mbar_wait(&v_ready[st], par, err, kDevTimeoutFull)) break;
-          if (!mbar_wait(&p_full[x], jp, err, kDevTimeoutOther)) break;
-          tc_fence_after();
-          issue_pv(st, j > 0);
-          mma_commit(&o_done[x]);
-          mma_commit(&v_free[st]);
-          if (j + 1 < nx) {
-            // S(j+1) overwrites P(j): after the product that reads it.
-            if (!mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) break;
-            if (!mbar_wait(&o_done[x], jp, err, kDevTimeoutAccum)) break;
+#pragma unroll
+          for (int h = 0; h < N; ++h) {
+            ok = mbar_wait(&p_full[x * N + h], jp, err, kDevTimeoutOther);
+            if (!ok) break;
             tc_fence_after();
-            issue_qk(st1);
-            mma_commit(&s_full[x]);
-            mma_commit(&k_free[st1]);
+            issue_pv(st, h, j > 0 || h > 0);
+            if (h == N - 1) mma_commit(&v_free[st]);
+            if (j + 1 < nx) {
+              // The next S overwrites this part's P: after the product that reads it.
+              ok = (h > 0 || mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) &&
+                   mbar_wait(&o_done[x * N + h], jp, err, kDevTimeoutAccum);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(st1, h);
+              if (h == N - 1) mma_commit(&k_free[st1]);
+            }
           }
         }
       }
@@ -542,38 +539,41 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     bool bad = false;         // a NaN or +inf among the row's scores
     uint64_t lsum0 = 0, lsum1 = 0;
     bool ok = true;
-    for (int j = 0; j < nx; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1, err, kDevTimeoutAccum))) {
+    for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
+      const int j = u / N, h = u % N;
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(&s_full[x * N + h], j & 1, err, kDevTimeoutAccum))) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const int key0 = k_begin + j * kPtTile;
-      uint32_t s[kPtTile];
+      constexpr int KC = L::kKeys;
+      const int key0 = k_begin + u * KC;
+      uint32_t s[KC];
 #pragma unroll
-      for (int c = 0; c < kPtTile / 32; ++c)
-        tmem_ld32(t_s + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+      for (int c = 0; c < KC / 32; ++c)
+        tmem_ld32(t_s + h * KC + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
       tmem_ld_wait();
       if constexpr (L::kSepP) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x]);
       }
-      if (key0 + kPtTile > lim_tile) {  // warp-uniform
+      if (key0 + KC > lim_tile) {  // warp-uniform
         const int c0 = lim_row - key0;
 #pragma unroll
-        for (int c = 0; c < kPtTile; ++c)
+        for (int c = 0; c < KC; ++c)
           if (c >= c0) s[c] = 0xff800000u;  // -inf
       }
       if (holes) {
         uint32_t there = 0;  // bit i: keys 16 i .. 16 i + 15 exist
 #pragma unroll 1
-        for (int i = 0; i < kPtTile / 16; ++i)
+        for (int i = 0; i < KC / 16; ++i)
           there |= static_cast<uint32_t>(key0 + 16 * i < seq.len &&
                                          paged_page(p, b, key0 + 16 * i) >= 0) << i;
-        if (there != 0xffu) {
+        if (there != (1u << (KC / 16)) - 1u) {
 #pragma unroll
-          for (int c = 0; c < kPtTile; ++c)
+          for (int c = 0; c < KC; ++c)
             if (!((there >> (c >> 4)) & 1u)) s[c] = 0xff800000u;
         }
       }
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       for (int i = 0; i < 8; ++i)
         mm[i] = pt_max3(__uint_as_float(s[i]), __uint_as_float(s[i + 8]), -INFINITY);
 #pragma unroll
-      for (int c = 16; c < kPtTile; c += 16)
+      for (int c = 16; c < KC; c += 16)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           mm[i] = pt_max3(mm[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       bool rescale = false;
       float f = 1.f;
       // (a NaN maximum compares false and leaves m_ref)
-      if (j == 0) {
+      if (u == 0) {
         m_ref = m_new;
       } else if (__any_sync(0xffffffffu, m_new > m_ref + kPtRescale)) {
         const float m_up = fmaxf(m_ref, m_new);
@@ -608,11 +608,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2);
       const uint64_t negm2 = f2_pack(-m_use, -m_use);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int q = 0; q < KC / 64; ++q) {
         uint32_t pr[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const int c = 64 * half + 2 * i;
+          const int c = 64 * q + 2 * i;
           const uint64_t arg =
               f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, negm2);
           uint64_t e;
@@ -628,10 +628,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           f2_unpack(e, e0, e1);
           pr[i] = pack_half2(e0, e1);
         }
-        if (half == 0) {
-          if constexpr (L::kSepP) {
-            if (j > 0 && !__all_sync(0xffffffffu,
-                                     mbar_wait(&o_done[x], (j - 1) & 1, err, kDevTimeoutAccum))) {
+        if (q == 0) {
+          // The previous part's product reads P (separate columns) and adds to O.
+          if ((L::kSepP || rescale) && u > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&o_done[x * N + (u - 1) % N], ((u - 1) / N) & 1,
+                                                   err, kDevTimeoutAccum))) {
               ok = false;
               break;
             }
@@ -649,16 +650,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             }
           }
         }
-        tmem_st32(t_p + 32 * half, pr);
+        tmem_st32(t_p + h * KC + 32 * q, pr);
       }
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      if (lane == 0) mbar_arrive(&p_full[x * N + h]);
     }
     if (ok && nx > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], (nx - 1) & 1, err, kDevTimeoutAccum));
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x * N + N - 1], (nx - 1) & 1, err,
+                                             kDevTimeoutAccum));
     float la, lb, lc, ld;
     f2_unpack(lsum0, la, lb);
     f2_unpack(lsum1, lc, ld);
@@ -746,7 +748,7 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   const uint32_t qb[3] = {64, static_cast<uint32_t>(a.group), tile_tokens};
   st = make_tmap(&tq, a.q, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, qd, qs, qb,
                  CU_TENSOR_MAP_SWIZZLE_128B);
-  // fp16: 64-column boxes in the layout of the products; 8 bit: plain rows.
+  // fp16: 64-column boxes in the layout of the products; 8 bit: whole rows.
   const uint64_t kd[4] = {HD, static_cast<uint64_t>(c->page_size),
                           static_cast<uint64_t>(p.kv_heads), static_cast<uint64_t>(p.num_pages)};
   const uint64_t ks[3] = {static_cast<uint64_t>(p.token_stride) * eb,
@@ -755,7 +757,8 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   const uint32_t kb[4] = {L::kQuant ? HD : 64, static_cast<uint32_t>(page_rows), 1, 1};
   const CUtensorMapDataType dt =
       L::kQuant ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const CUtensorMapSwizzle sw = L::kQuant ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
+  const CUtensorMapSwizzle sw =
+      L::kQuant && HD == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   if (st == TFX_OK) st = make_tmap(&tk, p.k, dt, 4, kd, ks, kb, sw);
   if (st == TFX_OK) st = make_tmap(&tv, p.v, dt, 4, kd, ks, kb, sw);
   if (st != TFX_OK) return st;
@@ -763,7 +766,7 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   if (blocks * a.splits > 65535)
     return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: max_query_len is too long for the grid");
   launch_pdl(kern, dim3(p.kv_heads, p.batch, static_cast<unsigned>(blocks * a.splits)),
-             dim3(kPtThreads), L::kSmem, stream, tq, tk, tv, p, a, static_cast<int>(blocks),
+             dim3(L::kThreads), L::kSmem, stream, tq, tk, tv, p, a, static_cast<int>(blocks),
              device_error_word());
   return check_launch("paged_tc_kernel");
 }
