@@ -170,12 +170,24 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   } else {
     pl.kps = round_keys(kv, parts);
   }
-  // tcgen05: one CTA to an SM; a start and the partial results of its 256 rows
-  // cost about as much as 6 tiles of 128 keys.
+  // tcgen05: one CTA to an SM, whose start costs about as much as 768 keys.
+  // Whole waves of equal CTAs, and what the partial results of every row cost
+  // (written and read once, in units of a key tile's time): cutting pays where
+  // there are few row blocks.
   const int tokens = group <= 128 ? 2 * (128 / group) : 1;
-  double cost = 0.;
-  pl.kps_tc = round_keys(
-      kv, cut(pairs * ((pl.q + tokens - 1) / tokens), num_sms(), kv, 768, 1024, 16, &cost));
+  const int64_t tc_blocks = pairs * ((pl.q + tokens - 1) / tokens);
+  int64_t tc_parts = 1;
+  double tc_cost = 0.;
+  for (int64_t n = 1; n <= 16 && (n == 1 || (kv + n - 1) / n >= 1024); ++n) {
+    const double waves = static_cast<double>((tc_blocks * n + num_sms() - 1) / num_sms());
+    const double join = n > 1 ? 500. + 1e-5 * 8. * b->num_tokens * q_heads * n * hd : 0.;
+    const double cost = waves * ((kv + n - 1) / n + 768) + join;
+    if (n == 1 || cost < tc_cost) {
+      tc_parts = n;
+      tc_cost = cost;
+    }
+  }
+  pl.kps_tc = round_keys(kv, tc_parts);
   int64_t least = pl.tc ? pl.kps_tc : pl.kps;
   if (pl.small && pl.kps < least) least = pl.kps;
   pl.splits = static_cast<int>((kv + least - 1) / least);

@@ -22,12 +22,13 @@
 // S = Q K^T (128 x N keys) goes to TMEM, the softmax warps write P over it or
 // beside it, O += P V takes P from TMEM and V MN-major from the row-major tile.
 // A row's reference maximum moves only when it is exceeded by more than 2^8
-// (O is then rescaled in TMEM). head_dim 64: N = 128 and P has columns of its
-// own (S 2 x 128, P 2 x 64, O 2 x 64), so the next S is computed while this one's
-// P is. head_dim 128: O fills half of TMEM and P lies over S; N = 64, so that
-// one half of a tile's S is being exponentiated while the other is multiplied
-// and replaced (with N = 128 each tile's chain S - P - PV - S was serial: 5000
-// against 2800 cycles of products for a pair of tiles).
+// (O is then rescaled in TMEM). A tile's S is two parts of N = 64 keys, so that
+// one is being exponentiated while the other is multiplied and replaced (with
+// N = 128 at head_dim 128 each tile's chain S - P - PV - S was serial: 870 against
+// 1029 TFLOP/s, one fp16 head_dim 128 sequence of 16k, not causal). head_dim 64:
+// P has columns of its own (S 2 x 128, P 2 x 64, O 2 x 64), so the next S is
+// computed as soon as this one is in registers; head_dim 128: O fills half of
+// TMEM and P lies over S.
 //
 // 8-bit values are expanded as code * scale in fp16. The scale s is used as
 // m * 2^k with an fp16 m: int8 codes are placed behind the exponent of
@@ -39,8 +40,7 @@
 // What a row does not see must not reach it, and 0 * inf does: V rows behind
 // the sequence are cleared; in tiles that some rows of the CTA see and others
 // do not, non-finite values are cleared before the product and added at the
-// end to the rows that see them. Rows whose scores hold a NaN or +inf are NaN
-// (the polynomial exponential would lose them).
+// end to the rows that see them. Rows whose scores hold a NaN or +inf are NaN.
 #pragma once
 
 #include "paged.cuh"
@@ -70,11 +70,12 @@ struct PtCfg {
   static constexpr int kR = kV + kStages * kTileBytes;
   static constexpr int kBar = kR + kRaws * kRawBytes;
   static constexpr int kSmem = kBar + 512 + 1024;  // barriers + alignment slack
-  static constexpr bool kSepP = false;          // P has its own TMEM columns
-  static constexpr int kParts = kSepP ? 1 : 2;     // a tile's S in so many parts
+  static constexpr bool kSepP = HD == 64 && !kQuant;  // P has its own TMEM columns
+  static constexpr int kParts = kSepP ? 1 : 2;        // a tile's S in so many parts
   static constexpr int kKeys = kPtTile / kParts;   // keys of one
   static constexpr uint32_t kColP = kSepP ? 2 * kPtTile : 0;
-  static constexpr uint32_t kPStride = kSepP ? kPtTile / 2 : kPtTile;
+  static constexpr uint32_t kPStride = kSepP ? kPtTile / 2 : kPtTile;  // of a tile
+  static constexpr uint32_t kPPart = kSepP ? kKeys / 2 : kKeys;        // of a part
   static constexpr uint32_t kColO = kSepP ? 3 * kPtTile : 2 * kPtTile;
   static_assert(kColO + 2 * HD <= kPtCols, "TMEM budget");
   static_assert(kSmem <= 227 * 1024, "shared-memory budget");
@@ -87,13 +88,6 @@ __device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map,
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
-}
-
-// max(a, b, c), NaN if one is.
-__device__ __forceinline__ float pt_max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
 }
 
 // A row's scale as the expansion uses it: fp16 bits of m (low half), k + 64 (high).
@@ -171,8 +165,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   };
   const int nA = tiles_of(0), nB = tiles_of(1), n_iter = max(nA, nB);
   if (is_split && n_iter == 0) return;  // not looked at when the splits are joined
-  // Tiles from this key on hold keys that not every row sees.
+  // Keys from here on are not seen by every row; the first tile that holds one.
   const int lim_first = lim_of(i0);
+  const int j_partly = max(0, lim_first - k_begin) / kPtTile;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -185,15 +180,15 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   uint64_t* v_empty = k_empty + 2 * S;  // [2][S]
   constexpr int N = L::kParts;
   uint64_t* s_full = v_empty + 2 * S;   // [2][N]
-  uint64_t* s_free = s_full + 2 * N;    // [2], separate P only
-  uint64_t* p_full = s_free + 2;        // [2][N]
+  uint64_t* s_free = s_full + 2 * N;    // [2][N], separate P only
+  uint64_t* p_full = s_free + 2 * N;    // [2][N]
   uint64_t* o_done = p_full + 2 * N;    // [2][N]
   uint64_t* drain = o_done + 2 * N;     // [2]
   uint64_t* r_full = drain + 2;         // [R] raw tile loaded
   uint64_t* r_empty = r_full + R;       // [R] raw tile expanded by all its warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + R);
   volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
-  static_assert((1 + 7 * S + 4 + 6 * N + 2 * R) * 8 + 8 <= 512, "barrier space");
+  static_assert((1 + 7 * S + 2 + 8 * N + 2 * R) * 8 + 8 <= 512, "barrier space");
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q);
@@ -210,9 +205,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       }
     }
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&s_free[x], 4);
       mbar_init(&drain[x], 1);
       for (int h = 0; h < N; ++h) {
+        mbar_init(&s_free[x * N + h], 4);
         mbar_init(&s_full[x * N + h], 1);
         mbar_init(&p_full[x * N + h], 4);
         mbar_init(&o_done[x * N + h], 1);
@@ -257,8 +252,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     const uint32_t par = ((j / S) - 1) & 1;
     bool ok = true;
     if (j >= S) {
-      if (j - S < nA) ok = mbar_wait(&empty[j % S], par, err, kDevTimeoutEmpty);
-      if (ok && j - S < nB) ok = mbar_wait(&empty[S + j % S], par, err, kDevTimeoutEmpty);
+      if (j - S < nA) ok = mbar_wait_sleep(&empty[j % S], par, err, kDevTimeoutEmpty);
+      if (ok && j - S < nB) ok = mbar_wait_sleep(&empty[S + j % S], par, err, kDevTimeoutEmpty);
     }
     return __all_sync(0xffffffffu, ok) != 0;
   };
@@ -314,28 +309,30 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         // ---------------------------------------------- V tiles not all see
         for (int j = 0; j < n_iter; ++j) {
           const int st = j % S, key0 = k_begin + j * kPtTile;
-          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (j / S) & 1, err, kDevTimeoutFull)))
+          // (every phase is waited for: a parity tells only neighbours apart)
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait_sleep(&v_full[st], (j / S) & 1, err, kDevTimeoutFull)))
             break;
-          if (key0 + kPtTile > lim_first) {
-            uint8_t* tile = smem + L::kV + st * L::kTileBytes;
-            bool found = false;
-            for (int c = lane; c < L::kTileBytes / 16; c += 32) {
-              // 16-byte chunk c lies in row (c / 8) % 128 of its 64-column block
-              uint4* at = reinterpret_cast<uint4*>(tile) + c;
-              const bool behind = key0 + ((c >> 3) & (kPtTile - 1)) >= seq.len;
-              uint4 x = *at;
-              bool hit = h2_clear(x.x);
-              hit |= h2_clear(x.y);
-              hit |= h2_clear(x.z);
-              hit |= h2_clear(x.w);
-              if (behind) *at = make_uint4(0u, 0u, 0u, 0u);
-              else if (hit) *at = x;
-              found |= hit && !behind;
-            }
-            if (found) *cleared = 1;
-            fence_proxy_async_smem();
-            __syncwarp();
+          if (j < j_partly) continue;
+          uint8_t* tile = smem + L::kV + st * L::kTileBytes;
+          bool found = false;
+#pragma unroll 4
+          for (int c = lane; c < L::kTileBytes / 16; c += 32) {
+            // 16-byte chunk c lies in row (c / 8) % 128 of its 64-column block
+            uint4* at = reinterpret_cast<uint4*>(tile) + c;
+            const bool behind = key0 + ((c >> 3) & (kPtTile - 1)) >= seq.len;
+            uint4 x = *at;
+            bool hit = h2_clear(x.x);
+            hit |= h2_clear(x.y);
+            hit |= h2_clear(x.z);
+            hit |= h2_clear(x.w);
+            if (behind) *at = make_uint4(0u, 0u, 0u, 0u);
+            else if (hit) *at = x;
+            found |= hit && !behind;
           }
+          if (found) *cleared = 1;
+          fence_proxy_async_smem();
+          __syncwarp();
           if (lane == 0) mbar_arrive(&v_ready[st]);
         }
       }
@@ -349,7 +346,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         int page = page_coord(0, part), next = page_coord(1, part), issued = 0;
         for (int e = 0; e < total; ++e) {
           const int j = e >> 1;
-          if (e >= R && !__all_sync(0xffffffffu, mbar_wait(&r_empty[e % R], ((e / R) - 1) & 1, err,
+          if (e >= R && !__all_sync(0xffffffffu, mbar_wait_sleep(&r_empty[e % R], ((e / R) - 1) & 1, err,
                                                            kDevTimeoutEmpty)))
             break;
           if (lane == 0) mbar_arrive_expect_tx(&r_full[e % R], L::kRawBytes);
@@ -388,7 +385,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           const PtExpand<CODE> expand(pt_scale<CODE>(kv ? sc[1] : sc[0]));
           if (kv) load_scales(j + 1);
           if (!__all_sync(0xffffffffu,
-                          mbar_wait(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) ||
+                          mbar_wait_sleep(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) ||
               !stage_free(kv ? v_empty : k_empty, j))
             break;
           const uint8_t* src = smem + L::kR + (e % R) * L::kRawBytes + r * HD;
@@ -464,10 +461,17 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
 #pragma unroll
         for (int k = 0; k < L::kKeys / 16; ++k)
           mma_f16_ts(tmem + L::kColO + x * HD,
-                     tmem + L::kColP + x * L::kPStride + h * L::kKeys + 8 * k,
+                     tmem + L::kColP + x * L::kPStride + h * L::kPPart + 8 * k,
                      db + static_cast<uint64_t>((k * 2048) >> 4), id_pv,
                      (accumulate || k > 0) ? 1u : 0u);
         mma_commit(&o_done[x * N + h]);
+      };
+      // fp16: V as loaded, where every row sees all of the tile.
+      auto wait_v = [&](int j) {
+        if (!kQuant && j < j_partly)
+          return mbar_wait(&v_full[j % S], (j / S) & 1, err, kDevTimeoutFull);
+        const int uses = kQuant ? j / S : (j - j_partly) / S;  // of v_ready's stage before
+        return mbar_wait(&v_ready[j % S], uses & 1, err, kDevTimeoutFull);
       };
       bool ok = mbar_wait(q_full, 0, err, kDevTimeoutFull);
       if (ok && nx > 0) {
@@ -481,23 +485,27 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       }
       for (int j = 0; ok && j < nx; ++j) {
         const int st = j % S, st1 = (j + 1) % S;
-        const uint32_t par = (j / S) & 1, par1 = ((j + 1) / S) & 1;
-        const uint32_t jp = j & 1;
+        const uint32_t par1 = ((j + 1) / S) & 1, jp = j & 1;
         if constexpr (L::kSepP) {
-          if (j + 1 < nx) {
-            if (!mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) break;
-            if (!mbar_wait(&s_free[x], jp, err, kDevTimeoutOther)) break;
+#pragma unroll
+          for (int h = 0; h < N; ++h) {
+            if (j + 1 < nx) {  // the next S, as soon as this one is in registers
+              ok = (h > 0 || mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) &&
+                   mbar_wait(&s_free[x * N + h], jp, err, kDevTimeoutOther);
+              if (!ok) break;
+              tc_fence_after();
+              issue_qk(st1, h);
+              if (h == N - 1) mma_commit(&k_free[st1]);
+            }
+            ok = (h > 0 || wait_v(j)) &&
+                 mbar_wait(&p_full[x * N + h], jp, err, kDevTimeoutOther);
+            if (!ok) break;
             tc_fence_after();
-            issue_qk(st1, 0);
-            mma_commit(&k_free[st1]);
+            issue_pv(st, h, j > 0 || h > 0);
+            if (h == N - 1) mma_commit(&v_free[st]);
           }
-          if (!mbar_wait(&v_ready[st], par, err, kDevTimeoutFull)) break;
-          if (!mbar_wait(&p_full[x], jp, err, kDevTimeoutOther)) break;
-          tc_fence_after();
-          issue_pv(st, 0, j > 0);
-          mma_commit(&v_free[st]);
         } else {
-          if (!mbar_wait(&v_ready[st], par, err, kDevTimeoutFull)) break;
+          if (!wait_v(j)) break;
 #pragma unroll
           for (int h = 0; h < N; ++h) {
             ok = mbar_wait(&p_full[x * N + h], jp, err, kDevTimeoutOther);
@@ -536,7 +544,6 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     const int lim_row = lim_of(min(tok, seq.n - 1));
     const int lim_tile = lim_of(min(first, seq.n - 1));  // smallest of the tile
     float m_ref = -INFINITY;  // -inf: no key seen yet
-    bool bad = false;         // a NaN or +inf among the row's scores
     uint64_t lsum0 = 0, lsum1 = 0;
     bool ok = true;
     for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
@@ -557,7 +564,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       if constexpr (L::kSepP) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[x]);
+        if (lane == 0) mbar_arrive(&s_free[x * N + h]);
       }
       if (key0 + KC > lim_tile) {  // warp-uniform
         const int c0 = lim_row - key0;
@@ -580,19 +587,17 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       float mm[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        mm[i] = pt_max3(__uint_as_float(s[i]), __uint_as_float(s[i + 8]), -INFINITY);
+        mm[i] = fmaxf(__uint_as_float(s[i]), __uint_as_float(s[i + 8]));
 #pragma unroll
       for (int c = 16; c < KC; c += 16)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          mm[i] = pt_max3(mm[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
-      const float mx = pt_max3(pt_max3(mm[0], mm[1], mm[2]), pt_max3(mm[3], mm[4], mm[5]),
-                               pt_max3(mm[6], mm[7], -INFINITY));
+          mm[i] = fmax3(mm[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
+      const float mx = fmaxf(fmax3(mm[0], mm[1], mm[2]),
+                             fmax3(fmax3(mm[3], mm[4], mm[5]), mm[6], mm[7]));
       const float m_new = mx * a.scale_log2;
-      bad = bad || !(m_new < INFINITY);
       bool rescale = false;
       float f = 1.f;
-      // (a NaN maximum compares false and leaves m_ref)
       if (u == 0) {
         m_ref = m_new;
       } else if (__any_sync(0xffffffffu, m_new > m_ref + kPtRescale)) {
@@ -617,7 +622,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
               f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, negm2);
           uint64_t e;
           if ((i & 7) < kPtPoly) {
-            e = exp2_poly_f2(arg);
+            uint64_t mant;
+            e = exp2_poly_nan_f2(arg, &mant);
+            lsum0 = f2_fma(mant, 0, lsum0);  // a NaN score makes the sum NaN
           } else {
             float a0, a1;
             f2_unpack(arg, a0, a1);
@@ -629,15 +636,18 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           pr[i] = pack_half2(e0, e1);
         }
         if (q == 0) {
-          // The previous part's product reads P (separate columns) and adds to O.
-          if ((L::kSepP || rescale) && u > 0) {
-            if (!__all_sync(0xffffffffu, mbar_wait(&o_done[x * N + (u - 1) % N], ((u - 1) / N) & 1,
-                                                   err, kDevTimeoutAccum))) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+          // P's columns are free once the product of this part of the last tile
+          // is through (P over S: it was before this S was computed); O may be
+          // rescaled once the previous part's is.
+          if (L::kSepP && j > 0)
+            ok = mbar_wait(&o_done[x * N + h], (j - 1) & 1, err, kDevTimeoutAccum);
+          if (rescale && u > 0 && ok)
+            ok = mbar_wait(&o_done[x * N + (u - 1) % N], ((u - 1) / N) & 1, err, kDevTimeoutAccum);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
           }
+          tc_fence_after();
           if (rescale) {
 #pragma unroll 1
             for (int c = 0; c < HD; c += 16) {
@@ -650,7 +660,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
             }
           }
         }
-        tmem_st32(t_p + h * KC + 32 * q, pr);
+        tmem_st32(t_p + h * L::kPPart + 32 * q, pr);
       }
       if (!ok) break;
       tmem_st_wait();
@@ -665,8 +675,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     f2_unpack(lsum0, la, lb);
     f2_unpack(lsum1, lc, ld);
     float l = (la + lb) + (lc + ld);
-    if (m_ref == -INFINITY) l = 0.f;  // no key seen
-    if (bad) l = __uint_as_float(0x7fc00000u);
+    if (m_ref == -INFINITY && l == l) l = 0.f;                  // no key seen
+    if (m_ref == INFINITY) l = __uint_as_float(0x7fc00000u);  // a score of +inf
     if (ok) {
       const bool fix = *cleared != 0;  // the writer arrived before the last product
       const int head = hk * group + row % group;

@@ -507,6 +507,30 @@ __device__ __forceinline__ uint64_t exp2_poly_f2(uint64_t x) {
   return f2_pack(__uint_as_float(r0), __uint_as_float(r1));
 }
 
+// exp2_poly_f2 that does not lose a NaN: *mant gets 2^f, in [0.7, 1.42] for
+// every other input (-inf included) and NaN for NaN (whose result's bits the
+// exponent step may turn into anything). 0 * mant added to a sum keeps it.
+__device__ __forceinline__ uint64_t exp2_poly_nan_f2(uint64_t x, uint64_t* mant) {
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
+  const uint64_t xc = f2_pack(x0, x1);
+  const uint64_t kRound = f2_pack(12582912.0f, 12582912.0f);  // 1.5 * 2^23
+  const uint64_t j = f2_add(xc, kRound);
+  const uint64_t f = f2_sub(xc, f2_sub(j, kRound));
+  uint64_t p = f2_fma(f, f2_pack(0.055171433836221695f, 0.055171433836221695f),
+                      f2_pack(0.24261081218719482f, 0.24261081218719482f));
+  p = f2_fma(p, f, f2_pack(0.6932609677314758f, 0.6932609677314758f));
+  p = f2_fma(p, f, f2_pack(0.9999281167984009f, 0.9999281167984009f));
+  *mant = p;
+  float p0, p1, j0, j1;
+  f2_unpack(p, p0, p1);
+  f2_unpack(j, j0, j1);
+  return f2_pack(__uint_as_float(__float_as_uint(p0) + (__float_as_uint(j0) << 23)),
+                 __uint_as_float(__float_as_uint(p1) + (__float_as_uint(j1) << 23)));
+}
+
 // ------------------------------------------------- thread-block clusters
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
