@@ -1,9 +1,11 @@
 // Writing new tokens into a paged KV cache (optionally in 8 bits with a scale
 // per token and head) and reading them back as fp16.
 //
-// Both are one pass over memory. A thread handles 8 consecutive elements
-// (16 bytes of fp16) of one (token, head) row of K and of V; the head_dim / 8
-// threads of a row sit in one warp and reduce max|x| with shuffles.
+// Both are one pass over memory. A CTA takes a few consecutive tokens: its first
+// threads look up where each lives (sequence, page, slot) into shared memory,
+// then a thread handles 8 consecutive elements (16 bytes of fp16) of one
+// (token, head) row of K and of V at a time, two such pieces in flight. The
+// head_dim / 8 threads of a row sit in one warp and reduce max|x| with shuffles.
 //
 // Quantisation rounds x / s as if in exact arithmetic, so that a code is the
 // nearest one even when the quotient lies within an fp32 rounding of the
@@ -15,6 +17,8 @@
 //  e4m3: the quotient's bits behind the 3 of the code decide unless they are
 //        within 4 ulp of a half (or the code is subnormal); then the quotient
 //        is divided out and rounded to odd, which rounds on correctly.
+// Eight elements are quantised without a branch, and again with these
+// corrections where one of them needs it (a few in 10^5 for int8).
 #include "paged.cuh"
 
 namespace tfx {
@@ -22,27 +26,25 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ int quant_i8(float x, float inv, float s, float half_s) {
+// The codes of x, exact (see the file's comment).
+__device__ __forceinline__ int exact_i8(float x, float inv, float s, float half_s) {
   float c = rintf(x * inv);
   const float e = fmaf(-c, s, x);
-  if (fabsf(e) >= half_s) {  // rare: next to a border
-    if (fabsf(e) > half_s || (static_cast<int>(c) & 1)) c += copysignf(1.0f, e);
-  }
+  if (fabsf(e) > half_s || (fabsf(e) == half_s && (static_cast<int>(c) & 1)))
+    c += copysignf(1.0f, e);
   return static_cast<int>(fminf(fmaxf(c, -127.0f), 127.0f));
 }
 
-// x / s for a conversion to e4m3 (see the file's comment).
-__device__ __forceinline__ float quot_e4m3(float x, float inv, float s) {
-  const float y = x * inv;
-  const uint32_t bits = __float_as_uint(y) & 0x7fffffffu;
-  if (((bits & 0xfffffu) - 0x7fffcu) <= 8u || (bits < 0x3c800000u && x != 0.f)) {  // 2^-6
-    const float ax = fabsf(x), q = __fdiv_rn(ax, s), r = fmaf(-q, s, ax);
-    uint32_t odd = __float_as_uint(q);
-    if (r < 0.f) --odd;
-    if (r != 0.f) odd |= 1u;
-    return copysignf(__uint_as_float(odd), x);
-  }
-  return y;
+__device__ __forceinline__ float exact_quot(float x, float s) {  // rounded to odd
+  const float ax = fabsf(x), q = __fdiv_rn(ax, s), r = fmaf(-q, s, ax);
+  uint32_t odd = __float_as_uint(q);
+  if (r < 0.f) --odd;
+  if (r != 0.f) odd |= 1u;
+  return copysignf(__uint_as_float(odd), x);
+}
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
 // max|x| of a row's elements as fp16 bits, over the CH threads of the row.
@@ -68,63 +70,145 @@ __device__ __forceinline__ uint2 quantise(const uint4& x, uint32_t top, float* s
   *scale = s;
   if (top == 0u) return make_uint2(0u, 0u);
   const float inv = __frcp_rn(s), half_s = 0.5f * s;
+  float f[8];
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t out[2] = {0u, 0u};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(bits_h2(w[i]));
-    uint32_t two;
-    if constexpr (CODE == kCodeI8) {
-      two = (quant_i8(f.x, inv, s, half_s) & 0xff) | ((quant_i8(f.y, inv, s, half_s) & 0xff) << 8);
-    } else {
-      two = __nv_cvt_float2_to_fp8x2(make_float2(quot_e4m3(f.x, inv, s), quot_e4m3(f.y, inv, s)),
-                                     __NV_SATFINITE, __NV_E4M3);
+    const float2 y = __half22float2(bits_h2(w[i]));
+    f[2 * i] = y.x;
+    f[2 * i + 1] = y.y;
+  }
+  uint32_t out[2];
+  bool border = false;
+  if constexpr (CODE == kCodeI8) {
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the code
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float m = fmaf(f[i], inv, kRound);
+      border |= fabsf(fmaf(kRound - m, s, f[i])) >= half_s;
+      c[i] = __float_as_uint(m);
     }
-    out[i >> 1] |= two << (16 * (i & 1));
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      out[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040),
+                           __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
+    if (border) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = exact_i8(f[i], inv, s, half_s) & 0xff;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        out[i] = c[4 * i] | (c[4 * i + 1] << 8) | (c[4 * i + 2] << 16) | (c[4 * i + 3] << 24);
+    }
+  } else {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = f[i] * inv;
+      const uint32_t bits = __float_as_uint(y[i]);
+      border |= ((bits & 0xfffffu) - 0x7fffcu) <= 8u;
+      border |= (bits & 0x7fffffffu) - 1u < 0x3c800000u - 1u;  // below 2^-6, not 0
+    }
+    if (border) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = exact_quot(f[i], s);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      out[i] = e4m3x2(y[4 * i], y[4 * i + 1]) | (e4m3x2(y[4 * i + 2], y[4 * i + 3]) << 16);
   }
   return make_uint2(out[0], out[1]);
+}
+
+// Where a CTA's tokens live: element offset of the token's first head in k and
+// v, and of its first head's scale; -1: no page; -2: a row of no sequence.
+constexpr int kMostTokens = 64;
+struct Places {
+  int64_t at[kMostTokens];
+  int64_t scale[kMostTokens];
+};
+
+__device__ __forceinline__ void look_up(const Paged& p, int t0, int tokens, Places& out) {
+  for (int i = threadIdx.x; i < tokens; i += kThreads) {
+    const int t = t0 + i, b = paged_seq_of_row(p, t);
+    int64_t at = -2, scale = 0;
+    if (b >= 0) {
+      const PagedSeq s = paged_seq(p, b);
+      if (t >= s.row0 && t < s.row0 + s.n) {
+        const int pos = s.pos0 + (t - s.row0), page = paged_page(p, b, pos);
+        at = page < 0 ? -1 : paged_offset(p, page, pos);
+        scale = page < 0 ? 0 : paged_scale_offset(p, page, 0, pos);
+      }
+    }
+    out.at[i] = at;
+    out.scale[i] = scale;
+  }
+  __syncthreads();
+}
+
+// One 8-element piece of the CTA's tokens: piece i is chunk i % CH of row i / CH,
+// a row being (token, head). `div`: 2^32 / kv_heads + 1, or 0 for one head (exact:
+// rows of a CTA times heads stay below 2^32).
+struct Piece {
+  int token, head, chunk;
+};
+template <int CH>
+__device__ __forceinline__ Piece piece_of(int i, int heads, uint32_t div) {
+  const int row = i / CH;
+  const int token = div == 0u ? row : static_cast<int>(__umulhi(static_cast<uint32_t>(row), div));
+  return Piece{token, row - token * heads, i % CH};
 }
 
 template <int CODE, int HD>
 __global__ void __launch_bounds__(kThreads)
     paged_append_kernel(const __half* __restrict__ k, int64_t ld_k, const __half* __restrict__ v,
-                        int64_t ld_v, Paged p) {
+                        int64_t ld_v, const __grid_constant__ Paged p, int cta_tokens,
+                        uint32_t div) {
   grid_dep_wait();
   grid_dep_launch();
-  constexpr int CH = HD / 8;
-  const int row = blockIdx.x * (kThreads / CH) + threadIdx.x / CH;  // (token, head)
-  const int c = threadIdx.x % CH;
-  const int t = row / p.kv_heads, h = row % p.kv_heads;
-  int page = -1, pos = 0;
-  if (t < p.num_tokens) {
-    const int b = paged_seq_of_row(p, t);
-    if (b >= 0) {
-      const PagedSeq s = paged_seq(p, b);
-      pos = s.pos0 + (t - s.row0);
-      if (t >= s.row0 && t < s.row0 + s.n) page = paged_page(p, b, pos);
+  constexpr int CH = HD / 8, U = 2;
+  __shared__ Places places;
+  const int t0 = blockIdx.x * cta_tokens, tokens = min(cta_tokens, p.num_tokens - t0);
+  look_up(p, t0, tokens, places);
+  const int pieces = tokens * p.kv_heads * CH;
+  const int64_t head_scale = static_cast<int64_t>(1) << p.page_shift;
+  // (whole warps go through the loop: the rows' threads reduce together)
+  for (int i0 = threadIdx.x; i0 - static_cast<int>(threadIdx.x) < pieces; i0 += U * kThreads) {
+    Piece pc[U];
+    int64_t at[U];
+    uint4 xk[U], xv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      pc[u] = piece_of<CH>(min(i, pieces - 1), p.kv_heads, div);
+      at[u] = i < pieces ? places.at[pc[u].token] : -1;
+      xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
+      if (at[u] >= 0) {
+        const int64_t t = t0 + pc[u].token;
+        xk[u] = __ldcs(reinterpret_cast<const uint4*>(k + t * ld_k + pc[u].head * HD) + pc[u].chunk);
+        xv[u] = __ldcs(reinterpret_cast<const uint4*>(v + t * ld_v + pc[u].head * HD) + pc[u].chunk);
+      }
     }
-  }
-  uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
-  if (page >= 0) {
-    xk = __ldcs(reinterpret_cast<const uint4*>(k + t * ld_k + h * HD + c * 8));
-    xv = __ldcs(reinterpret_cast<const uint4*>(v + t * ld_v + h * HD + c * 8));
-  }
-  const int64_t at = paged_offset(p, page, pos) + h * p.head_stride + c * 8;
-  if constexpr (CODE == kCodeF16) {
-    if (page >= 0) {
-      *reinterpret_cast<uint4*>(static_cast<__half*>(p.k) + at) = xk;
-      *reinterpret_cast<uint4*>(static_cast<__half*>(p.v) + at) = xv;
-    }
-  } else {
-    const uint32_t tk = row_absmax<CH>(xk), tv = row_absmax<CH>(xv);  // every lane takes part
-    if (page >= 0) {
-      float sk, sv;
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.k) + at) = quantise<CODE>(xk, tk, &sk);
-      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.v) + at) = quantise<CODE>(xv, tv, &sv);
-      if (c == 0) {
-        const int64_t so = paged_scale_offset(p, page, h, pos);
-        p.k_scale[so] = sk;
-        p.v_scale[so] = sv;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t to = at[u] + pc[u].head * p.head_stride + pc[u].chunk * 8;
+      if constexpr (CODE == kCodeF16) {
+        if (at[u] >= 0) {
+          *reinterpret_cast<uint4*>(static_cast<__half*>(p.k) + to) = xk[u];
+          *reinterpret_cast<uint4*>(static_cast<__half*>(p.v) + to) = xv[u];
+        }
+      } else {
+        const uint32_t tk = row_absmax<CH>(xk[u]), tv = row_absmax<CH>(xv[u]);  // every lane
+        if (at[u] >= 0) {
+          float sk, sv;
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.k) + to) = quantise<CODE>(xk[u], tk, &sk);
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.v) + to) = quantise<CODE>(xv[u], tv, &sv);
+          if (pc[u].chunk == 0) {
+            const int64_t so = places.scale[pc[u].token] + pc[u].head * head_scale;
+            p.k_scale[so] = sk;
+            p.v_scale[so] = sv;
+          }
+        }
       }
     }
   }
@@ -146,50 +230,77 @@ __device__ __forceinline__ uint4 dequantise(uint2 x, float s) {
 template <int CODE, int HD>
 __global__ void __launch_bounds__(kThreads)
     paged_read_kernel(__half* __restrict__ k, int64_t ld_k, __half* __restrict__ v, int64_t ld_v,
-                      Paged p) {
+                      const __grid_constant__ Paged p, int cta_tokens, uint32_t div) {
   grid_dep_wait();
   grid_dep_launch();
-  constexpr int CH = HD / 8;
-  const int row = blockIdx.x * (kThreads / CH) + threadIdx.x / CH;
-  const int c = threadIdx.x % CH;
-  const int t = row / p.kv_heads, h = row % p.kv_heads;
-  if (t >= p.num_tokens) return;
-  const int b = paged_seq_of_row(p, t);
-  if (b < 0) return;
-  const PagedSeq s = paged_seq(p, b);
-  if (t < s.row0 || t >= s.row0 + s.n) return;
-  const int pos = s.pos0 + (t - s.row0);
-  const int page = paged_page(p, b, pos);
-  uint4 xk = make_uint4(0, 0, 0, 0), xv = xk;
-  if (page >= 0) {
-    const int64_t at = paged_offset(p, page, pos) + h * p.head_stride + c * 8;
-    if constexpr (CODE == kCodeF16) {
-      xk = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.k) + at);
-      xv = *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.v) + at);
-    } else {
-      const int64_t so = paged_scale_offset(p, page, h, pos);
-      xk = dequantise<CODE>(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.k) + at),
-                            p.k_scale[so]);
-      xv = dequantise<CODE>(*reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.v) + at),
-                            p.v_scale[so]);
+  constexpr int CH = HD / 8, U = 2;
+  __shared__ Places places;
+  const int t0 = blockIdx.x * cta_tokens, tokens = min(cta_tokens, p.num_tokens - t0);
+  look_up(p, t0, tokens, places);
+  const int pieces = tokens * p.kv_heads * CH;
+  const int64_t head_scale = static_cast<int64_t>(1) << p.page_shift;
+  for (int i0 = threadIdx.x; i0 < pieces; i0 += U * kThreads) {
+    Piece pc[U];
+    int64_t at[U];
+    uint4 xk[U], xv[U];  // 8 bit: codes in the first half
+    float sk[U], sv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      pc[u] = piece_of<CH>(min(i, pieces - 1), p.kv_heads, div);
+      at[u] = i < pieces ? places.at[pc[u].token] : -2;
+      xk[u] = xv[u] = make_uint4(0, 0, 0, 0);
+      sk[u] = sv[u] = 0.f;
+      if (at[u] >= 0) {
+        const int64_t from = at[u] + pc[u].head * p.head_stride + pc[u].chunk * 8;
+        if constexpr (CODE == kCodeF16) {
+          xk[u] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.k) + from));
+          xv[u] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const __half*>(p.v) + from));
+        } else {
+          const uint2 ck = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.k) + from));
+          const uint2 cv = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.v) + from));
+          const int64_t so = places.scale[pc[u].token] + pc[u].head * head_scale;
+          xk[u] = make_uint4(ck.x, ck.y, 0, 0);
+          xv[u] = make_uint4(cv.x, cv.y, 0, 0);
+          sk[u] = p.k_scale[so];
+          sv[u] = p.v_scale[so];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at[u] == -2) continue;
+      if constexpr (CODE != kCodeF16) {
+        xk[u] = dequantise<CODE>(make_uint2(xk[u].x, xk[u].y), sk[u]);
+        xv[u] = dequantise<CODE>(make_uint2(xv[u].x, xv[u].y), sv[u]);
+      }
+      const int64_t t = t0 + pc[u].token;
+      __stcs(reinterpret_cast<uint4*>(k + t * ld_k + pc[u].head * HD) + pc[u].chunk, xk[u]);
+      __stcs(reinterpret_cast<uint4*>(v + t * ld_v + pc[u].head * HD) + pc[u].chunk, xv[u]);
     }
   }
-  __stcs(reinterpret_cast<uint4*>(k + t * ld_k + h * HD + c * 8), xk);
-  __stcs(reinterpret_cast<uint4*>(v + t * ld_v + h * HD + c * 8), xv);
 }
 
 template <int CODE, int HD>
 int launch_copy(bool append, __half* k, int64_t ld_k, __half* v, int64_t ld_v, const Paged& p,
                 cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_heads;
-  constexpr int per_block = kThreads / (HD / 8);
-  const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block));
+  // Tokens of a CTA: about 8192 elements of K, fewer where that leaves SMs idle.
+  const int width = p.kv_heads * HD;
+  int tokens = width < 8192 ? 8192 / width : 1;
+  const int spread = (p.num_tokens + 4 * num_sms() - 1) / (4 * num_sms());
+  if (tokens > spread) tokens = spread;
+  if (tokens > kMostTokens) tokens = kMostTokens;
+  const dim3 grid(static_cast<unsigned>((p.num_tokens + tokens - 1) / tokens));
+  const uint32_t div =
+      p.kv_heads == 1 ? 0u : static_cast<uint32_t>((1ull << 32) / static_cast<uint32_t>(p.kv_heads)) + 1u;
   if (append) {
     launch_pdl(paged_append_kernel<CODE, HD>, grid, dim3(kThreads), 0, stream,
-               static_cast<const __half*>(k), ld_k, static_cast<const __half*>(v), ld_v, p);
+               static_cast<const __half*>(k), ld_k, static_cast<const __half*>(v), ld_v, p, tokens,
+               div);
     return check_launch("paged_append_kernel");
   }
-  launch_pdl(paged_read_kernel<CODE, HD>, grid, dim3(kThreads), 0, stream, k, ld_k, v, ld_v, p);
+  launch_pdl(paged_read_kernel<CODE, HD>, grid, dim3(kThreads), 0, stream, k, ld_k, v, ld_v, p,
+             tokens, div);
   return check_launch("paged_read_kernel");
 }
 

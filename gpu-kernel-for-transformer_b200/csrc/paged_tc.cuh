@@ -43,6 +43,8 @@
 // end to the rows that see them. Rows whose scores hold a NaN or +inf are NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace tfx {
@@ -126,6 +128,25 @@ struct PtExpand {
     }
   }
 };
+
+// Adds the non-finite values of keys [lo, hi) to a finished row (rare; out of
+// the kernel's registers): exactly what its weights, all above 0, make of them.
+template <int CODE, int HD>
+__device__ __noinline__ void pt_add_cleared(const Paged& p, int b, int hk, int lo, int hi,
+                                            float* part, __half* out) {
+  for (int key = lo; key < hi; ++key) {
+    const int page = paged_page(p, b, key);
+    if (page < 0) continue;
+    const int64_t at = paged_offset(p, page, key) + hk * p.head_stride;
+    const float vs = CODE != kCodeF16 ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
+    for (int d = 0; d < HD; ++d) {
+      const float y = paged_value<CODE>(p.v, at + d, vs);
+      if (isfinite(y)) continue;
+      if (part != nullptr) part[d] += y;
+      else out[d] = __float2half_rn(__half2float(out[d]) + y);
+    }
+  }
+}
 
 template <int CODE, int HD>
 __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
@@ -546,6 +567,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     float m_ref = -INFINITY;  // -inf: no key seen yet
     uint64_t lsum0 = 0, lsum1 = 0;
     bool ok = true;
+    auto softmax = [&](auto with_holes) {
     for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
       const int j = u / N, h = u % N;
       if (!__all_sync(0xffffffffu,
@@ -572,7 +594,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         for (int c = 0; c < KC; ++c)
           if (c >= c0) s[c] = 0xff800000u;  // -inf
       }
-      if (holes) {
+      if constexpr (decltype(with_holes)::value) {
         uint32_t there = 0;  // bit i: keys 16 i .. 16 i + 15 exist
 #pragma unroll 1
         for (int i = 0; i < KC / 16; ++i)
@@ -668,6 +690,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[x * N + h]);
     }
+    };
+    if (holes) softmax(std::true_type{}); else softmax(std::false_type{});
     if (ok && nx > 0)
       ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x * N + N - 1], (nx - 1) & 1, err,
                                              kDevTimeoutAccum));
@@ -697,19 +721,6 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         }
         float* of = reinterpret_cast<float*>(o);
         if (owned) {
-          if (fix) {
-            for (int key = max(k_begin, lim_first - kPtTile); key < min(lim_row, k_stop); ++key) {
-              const int page = paged_page(p, b, key);
-              if (page < 0) continue;
-              const int64_t va = paged_offset(p, page, key) + hk * p.head_stride + c;
-              const float vs = kQuant ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float y = paged_value<CODE>(p.v, va + i, vs);
-                if (!isfinite(y)) of[i] += y;
-              }
-            }
-          }
           if (is_split) {
             float4* d4 = reinterpret_cast<float4*>(a.part_o + at * HD + c);
 #pragma unroll
@@ -729,6 +740,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         }
         __syncwarp();  // the next tmem_ld is warp-collective
       }
+      if (fix && owned)
+        pt_add_cleared<CODE, HD>(p, b, hk, max(k_begin, lim_first - kPtTile), min(lim_row, k_stop),
+                                 is_split ? a.part_o + at * HD : nullptr, dst);
     }
   }
 

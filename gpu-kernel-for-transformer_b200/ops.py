@@ -308,8 +308,7 @@ def paged_read(
     index = _paged_device(cache, batch)
     n, heads, hd, dev = batch.num_tokens, cache.kv_heads, cache.head_dim, cache.device
     if out is None:
-        k = torch.empty((n, heads, hd), dtype=torch.float16, device=dev)
-        v = torch.empty_like(k)
+        k, v = cache._half.new_empty(n, heads, hd), cache._half.new_empty(n, heads, hd)
         ld_k = ld_v = heads * hd
     else:
         k, v = out
@@ -352,7 +351,7 @@ def paged_attention(
         raise ValueError(f"q_heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
     ld_out = heads * hd
     if out is None:
-        out = torch.empty((n, ld_out), dtype=torch.float16, device=dev)
+        out = q.new_empty(n, ld_out)
     elif out.shape != (n, ld_out) or out.dtype != torch.float16 or out.device != dev or \
             (n > 0 and out.stride(1) != 1):
         raise ValueError("out must be float16 [num_tokens, q_heads * head_dim] with contiguous rows")
@@ -366,7 +365,7 @@ def paged_attention(
     if need > 0:
         # A workspace of its own for each call, from the stream's allocator: calls
         # on different streams, and graphs captured apart, never share one.
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        ws = cache._half.new_empty(need // 2)
     _call_on(index, "tfx_paged_attention", lib.tfx_paged_attention, q.data_ptr(), ld_q, cache._ref,
              batch._ref, out.data_ptr(), ld_out, heads, hd ** -0.5 if scale is None else float(scale),
              int(is_causal), None if ws is None else ws.data_ptr(), max(need, 0))

@@ -93,6 +93,7 @@ class PagedKVCache:
             v_scale.data_ptr() if quant else None, _CODES[k.dtype], pages, page_size, heads, hd,
             *strides[:3])
         self._ref = ctypes.byref(self._struct)
+        self._half = k.new_empty(0, dtype=torch.float16)  # outputs are allocated from it
 
 
 def _strides(t: torch.Tensor):
