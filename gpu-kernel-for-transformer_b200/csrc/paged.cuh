@@ -83,10 +83,17 @@ __device__ __forceinline__ int64_t paged_scale_offset(const Paged& p, int page, 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// Two e4m3 codes (low 16 bits) -> two fp16, exact.
+// Two e4m3 codes (low or high 16 bits) -> two fp16, exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t x) {
   uint32_t r;
   asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}"
+      : "=r"(r) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t e4m3x2_hi_to_h2(uint32_t x) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}"
       : "=r"(r) : "r"(x));
   return r;
 }
@@ -100,6 +107,8 @@ __device__ __forceinline__ uint32_t codes_to_h2(uint32_t x) {
     const uint32_t u = __byte_perm(x ^ 0x80808080u, 0x64646464u, 0x4040 | (J << 8) | I);
     return h2_bits(__hsub2(bits_h2(u), bits_h2(0x64806480u)));
   } else {
+    if constexpr (I == 0 && J == 1) return e4m3x2_to_h2(x);
+    if constexpr (I == 2 && J == 3) return e4m3x2_hi_to_h2(x);
     return e4m3x2_to_h2(__byte_perm(x, 0u, 0x4400 | (J << 4) | I));
   }
 }

@@ -7,9 +7,9 @@ namespace {
 
 // Keys of a split: a multiple of every kernel's round of tiles over its warps.
 constexpr int kSplitKeys = 256;
-// Sequences with more rows (new tokens x query heads per key/value head) go to
-// the tcgen05 kernel, whose tiles have 128.
-constexpr int kTcRows = 64;
+// Sequences with more rows (new tokens x query heads per key/value head) may go
+// to the tcgen05 kernel, whose tiles have 128.
+constexpr int kTcRows = 32;
 
 // out[row] = sum over splits of partial O scaled to the common maximum, over
 // the sum of their sums. `wpr` warps of the CTA per (token, head) row: one when
@@ -111,16 +111,17 @@ struct Plan {
 // CTAs at a time, each of which costs `start` keys besides its own; `most`
 // ranges at most, of `least` keys at least. Sequences are taken to have any
 // length up to kv: the work per slot, and behind it the longest range (alone,
-// where all CTAs run at once).
-int64_t cut(int64_t blocks, int64_t slots, int64_t kv, int64_t start, int64_t least, int64_t most,
-            double* cost) {
+// where all CTAs run at once). More than one range costs `join` keys.
+int64_t cut(int64_t blocks, int64_t slots, int64_t kv, int64_t start, int64_t join, int64_t least,
+            int64_t most, double* cost) {
   int64_t best = 1;
   *cost = 0.;
   for (int64_t n = 1; n <= most; n += n < 8 ? 1 : n / 4) {
     const int64_t keys = (kv + n - 1) / n;
     if (n > 1 && keys < least) break;
     const double waves = static_cast<double>(blocks) * n / slots;
-    const double c = waves <= 1. ? keys + start : 0.55 * waves * keys + waves * start + keys;
+    const double c = (waves <= 1. ? keys + start : waves * (0.55 * keys + start) + keys) +
+                     (n > 1 ? join : 0);
     if (n == 1 || c < *cost) {
       best = n;
       *cost = c;
@@ -141,43 +142,20 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   const int group = q_heads / c->kv_heads, hd = c->head_dim;
   pl.q = b->max_query_len < b->num_tokens ? b->max_query_len : b->num_tokens;
   pl.rows = pl.q * group;
-  pl.tc_rows = 0x7fffffff;
-  if ((hd == 64 || hd == 128) && group <= 128) pl.tc_rows = kTcRows;
-  pl.tc = pl.rows > pl.tc_rows;
-  pl.small = !pl.tc || b->batch > 1;  // a single sequence has all the rows
-  if (!pl.tc) pl.tc_rows = 0x7fffffff;
-  if (!pl.small) pl.tc_rows = 0;
-  const int64_t small_rows = pl.rows < pl.tc_rows ? pl.rows : pl.tc_rows;
-  pl.block_rows = paged_rows_block(hd, small_rows);
+  const bool quant = c->dtype != TFX_CACHE_F16;
   const int64_t pairs = static_cast<int64_t>(b->batch) * c->kv_heads;
   int64_t kv = static_cast<int64_t>(b->max_pages) * c->page_size;
   if (b->max_kv_len < kv) kv = b->max_kv_len;
   if (kv < 1) kv = 1;
-  // mma.sync: CTAs to an SM by registers and shared memory; a start costs about
-  // as much as 400 keys, a second launch to join as much as 512.
-  const int row_bytes = hd * (c->dtype == TFX_CACHE_F16 ? 2 : 1);
-  const int64_t slots = num_sms() * (row_bytes >= 512 ? 1 : pl.block_rows >= 32 ? 2 :
-                                     pl.block_rows == 16 || row_bytes == 256 ? 3 : 4);
-  const int64_t blocks = pairs * ((small_rows + pl.block_rows - 1) / pl.block_rows);
-  double alone = 0., joined = 0.;
-  const int64_t share = cut(blocks, slots, kv, 400, 128, 8, &alone);
-  // (beside the tcgen05 kernel few splits: its many rows are joined by the same kernel)
-  const int64_t parts = cut(blocks, slots, kv, 400, kSplitKeys, pl.tc ? 8 : 1024, &joined);
-  // (CTAs of a cluster wait for one another at its end: for one wave only)
-  if (!pl.tc && alone <= joined + 512. && (share == 1 || 4 * blocks * share <= 5 * slots)) {
-    pl.cluster = share > 1 ? static_cast<int>(share) : 0;
-    pl.kps = round_keys(kv, 1);
-  } else {
-    pl.kps = round_keys(kv, parts);
-  }
+
   // tcgen05: one CTA to an SM, whose start costs about as much as 768 keys.
   // Whole waves of equal CTAs, and what the partial results of every row cost
-  // (written and read once, in units of a key tile's time): cutting pays where
-  // there are few row blocks.
+  // (written and read once, in units of a key's time): cutting pays where there
+  // are few row blocks.
   const int tokens = group <= 128 ? 2 * (128 / group) : 1;
   const int64_t tc_blocks = pairs * ((pl.q + tokens - 1) / tokens);
   int64_t tc_parts = 1;
-  double tc_cost = 0.;
+  double tc_cost = 0., tc_keys = 0.;
   for (int64_t n = 1; n <= 16 && (n == 1 || (kv + n - 1) / n >= 1024); ++n) {
     const double waves = static_cast<double>((tc_blocks * n + num_sms() - 1) / num_sms());
     const double join = n > 1 ? 500. + 1e-5 * 8. * b->num_tokens * q_heads * n * hd : 0.;
@@ -185,9 +163,45 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
     if (n == 1 || cost < tc_cost) {
       tc_parts = n;
       tc_cost = cost;
+      tc_keys = waves * ((kv + n - 1) / n + 300);
     }
   }
   pl.kps_tc = round_keys(kv, tc_parts);
+
+  // Which kernel: more than 32 rows, and enough work. Times in ns, fitted to
+  // both kernels at 1 to 64 sequences of 2 000 to 30 000 tokens, 8 heads, 16 to 128
+  // rows; e.g. 128 rows, head_dim 64, fp16: 1 x 2 000 26 us tcgen05, 13 mma.sync;
+  // 1 x 30 000 40 and 56; 16 x 3 000 47 and 108; 64 x 4 000 210 and 382.
+  pl.tc = (hd == 64 || hd == 128) && group <= 128 && pl.rows > kTcRows;
+  if (pl.tc) {
+    const double tc_ns = 10e3 + tc_keys * (hd == 64 ? (quant ? 12.5 : 11.) : (quant ? 22. : 13.));
+    const double rows_ns = 6e3 + static_cast<double>(pairs) * ((pl.rows + 31) / 32) * kv *
+                                     (hd == 64 ? (quant ? .06 : .05) : (quant ? .09 : .08));
+    pl.tc = tc_ns < rows_ns;
+  }
+  pl.small = !pl.tc || b->batch > 1;  // a single sequence has all the rows
+  pl.tc_rows = !pl.tc ? 0x7fffffff : pl.small ? kTcRows : 0;
+
+  // mma.sync: CTAs to an SM by registers and shared memory; a start costs about
+  // as much as 400 keys, a second launch to join as much as 512 (beside the
+  // tcgen05 kernel 3000: its many rows are looked at by the same launch).
+  const int64_t small_rows = pl.rows < pl.tc_rows ? pl.rows : pl.tc_rows;
+  pl.block_rows = paged_rows_block(hd, small_rows);
+  const int row_bytes = hd * (quant ? 1 : 2);
+  const int64_t slots = num_sms() * (row_bytes >= 512 ? 1 : pl.block_rows >= 32 ? 2 :
+                                     pl.block_rows == 16 || row_bytes == 256 ? 3 : 4);
+  const int64_t blocks = pairs * ((small_rows + pl.block_rows - 1) / pl.block_rows);
+  double alone = 0., joined = 0.;
+  const int64_t share = cut(blocks, slots, kv, 400, 0, 128, 8, &alone);
+  const int64_t parts =
+      cut(blocks, slots, kv, 400, pl.tc ? 3000 : 512, kSplitKeys, pl.tc ? 8 : 1024, &joined);
+  // (CTAs of a cluster wait for one another at its end: for one wave only)
+  if (!pl.tc && alone <= joined && (share == 1 || 4 * blocks * share <= 5 * slots)) {
+    pl.cluster = share > 1 ? static_cast<int>(share) : 0;
+    pl.kps = round_keys(kv, 1);
+  } else {
+    pl.kps = round_keys(kv, parts);
+  }
   int64_t least = pl.tc ? pl.kps_tc : pl.kps;
   if (pl.small && pl.kps < least) least = pl.kps;
   pl.splits = static_cast<int>((kv + least - 1) / least);
@@ -223,9 +237,11 @@ int check_heads(const char* fn, const tfx_paged_cache* c, const tfx_paged_batch*
 }  // namespace
 
 int paged_rows_block(int head_dim, int64_t rows) {
-  // Registers hold 64 rows up to head_dim 64, 32 at 128, 16 at 256.
-  const int most = head_dim <= 64 ? 64 : (head_dim == 128 ? 32 : 16);
-  const int need = rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 64));
+  // Registers hold 32 rows, 16 at head_dim 256. (64 rows up to head_dim 64 halve
+  // the reads of K and V from L2 but leave two CTAs to an SM: 48.9 against 33.1 us
+  // for 40 sequences of up to 200 new tokens, 4 heads of 32.)
+  const int most = head_dim <= 128 ? 32 : 16;
+  const int need = rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
   return need < most ? need : most;
 }
 

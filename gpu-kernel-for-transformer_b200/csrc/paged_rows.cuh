@@ -252,31 +252,49 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
     }
   };
   // 16 keys lie in one page. Lane = (row of it, 16-byte chunk); a pass covers
-  // 32 / U rows.
-  constexpr int RP = 32 / U;  // rows of a pass
+  // RP rows, a group of passes 16 keys (32 where a pass does).
+  constexpr int RP = 32 / U, GK = RP > 16 ? RP : 16;
   const int64_t row_step = p.token_stride * code_bytes(CODE);
   const int64_t lane_off = (lane / U) % 16 * row_step + (lane % U) * 16;
+  const uint8_t* klane = kb + lane_off;
+  const uint8_t* vlane = vb + lane_off;
   const uint32_t lane_dst = smem_u32(ring) + (lane / U) * C::kPitch + (lane % U) * 16;
   auto load = [&](int i) {
     const uint32_t st = (i % NS) * C::kStageBytes;
     const int k0 = tile_key(i);
-    // Byte offset of this lane's group of 16 keys, negative without a page.
-    int64_t base[KW];
+    uint32_t there[KW];  // keys that exist
 #pragma unroll
-    for (int u = 0; u < KW; ++u)
-      base[u] = pg[u] < 0 ? -1
-                          : paged_offset(p, pg[u], (k0 + 32 * u + lane) & ~15) * code_bytes(CODE);
+    for (int u = 0; u < KW; ++u) there[u] = __ballot_sync(0xffffffffu, pg[u] >= 0);
 #pragma unroll
-    for (int it = 0; it < KT / RP + (KT % RP != 0); ++it) {
-      const int first = it * RP;  // row of lane 0
-      // (a pass of 32 rows holds two groups)
-      const int src = RP == 32 ? lane & 16 : (first & 16);
-      const int64_t from = __shfl_sync(0xffffffffu, base[first / 32], src);
-      const bool ok = from >= 0 && k0 + first + lane / U < k_end;
-      const int64_t off = (ok ? from + (first % 16) * row_step : 0) + lane_off;
-      if (KT % RP == 0 || lane / U < KT) {
-        rows_cp16(lane_dst + st + first * C::kPitch, kb + off, ok);
-        rows_cp16(lane_dst + st + C::kTileBytes + first * C::kPitch, vb + off, ok);
+    for (int g0 = 0; g0 < KT; g0 += GK) {
+      // Byte offset of the group's first key (of each half's, where a pass is two).
+      const int page = __shfl_sync(0xffffffffu, pg[g0 / 32], GK == 32 ? lane & 16 : g0 & 16);
+      const int first = k0 + g0 + (GK == 32 ? lane & 16 : 0);
+      const int64_t from = page >= 0 ? paged_offset(p, page, first & ~15) * code_bytes(CODE) : 0;
+      const uint8_t* kp = klane + from;
+      const uint8_t* vp = vlane + from;
+      const uint32_t dst = lane_dst + st + g0 * C::kPitch;
+      constexpr uint32_t kAll = GK >= 32 ? 0xffffffffu : 0xffffu;
+      const bool mine = KT % RP == 0 || lane / U < KT;
+      if (((there[g0 / 32] >> (g0 & 31)) & kAll) == kAll) {
+#pragma unroll
+        for (int it = 0; it < GK / RP; ++it) {
+          rows_cp16(dst + it * RP * C::kPitch, kp, true);
+          rows_cp16(dst + C::kTileBytes + it * RP * C::kPitch, vp, true);
+          kp += RP * row_step;
+          vp += RP * row_step;
+        }
+      } else {  // zeros where there is no key
+#pragma unroll 1
+        for (int it = 0; it < GK / RP; ++it) {
+          const int r = g0 + it * RP + lane / U;
+          const bool ok = mine && ((there[g0 / 32] >> (r & 31)) & 1u);
+          const int64_t off = static_cast<int64_t>(it) * RP * row_step;
+          if (mine) {
+            rows_cp16(dst + it * RP * C::kPitch, ok ? kp + off : kb, ok);
+            rows_cp16(dst + C::kTileBytes + it * RP * C::kPitch, ok ? vp + off : vb, ok);
+          }
+        }
       }
     }
     uint8_t* at = ring + st + 2 * C::kTileBytes;
@@ -292,10 +310,8 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
       }
     }
 #pragma unroll
-    for (int u = 0; u < KW; ++u) {
-      const uint32_t m = __ballot_sync(0xffffffffu, pg[u] >= 0);
-      if (lane == 0) reinterpret_cast<uint32_t*>(at + C::kScaleBytes)[u] = m;
-    }
+    for (int u = 0; u < KW; ++u)
+      if (lane == 0) reinterpret_cast<uint32_t*>(at + C::kScaleBytes)[u] = there[u];
   };
   look_up(0);
 #pragma unroll
@@ -767,9 +783,6 @@ int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t s
 template <int CODE, int HD>
 int launch_rows_hd(const Paged& p, const PagedAttn& a, int block_rows, int64_t rows,
                    cudaStream_t stream) {
-  if constexpr (HD <= 64) {
-    if (block_rows == 64) return launch_rows<CODE, HD, 8>(p, a, rows, stream);
-  }
   if constexpr (HD <= 128) {
     if (block_rows == 32) return launch_rows<CODE, HD, 4>(p, a, rows, stream);
   }

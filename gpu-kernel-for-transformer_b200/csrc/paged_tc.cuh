@@ -124,7 +124,7 @@ struct PtExpand {
       hi = h2_bits(__hmul2(__hsub2(bits_h2(__byte_perm(u, a, 0x4342)), bits_h2(c)), bits_h2(m)));
     } else {
       lo = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_to_h2(x)), bits_h2(m)), bits_h2(c)));
-      hi = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_to_h2(x >> 16)), bits_h2(m)), bits_h2(c)));
+      hi = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_hi_to_h2(x)), bits_h2(m)), bits_h2(c)));
     }
   }
 };
