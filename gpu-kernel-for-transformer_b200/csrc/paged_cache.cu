@@ -392,8 +392,8 @@ int check_paged(const char* fn, const tfx_paged_cache* c, const tfx_paged_batch*
     return fail(TFX_ERR_MISALIGNED, "%s: k and v 16-byte aligned, strides multiples of 16 bytes",
                 fn);
   if (!aligned(b->page_table, 4) || !aligned(b->query_start, 4) || !aligned(b->kv_len, 4) ||
-      (quant && (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))))
-    return fail(TFX_ERR_MISALIGNED, "%s: int32 and scale arrays must be 4-byte aligned", fn);
+      (quant && (!aligned(c->k_scale, 16) || !aligned(c->v_scale, 16))))
+    return fail(TFX_ERR_MISALIGNED, "%s: int32 arrays 4-byte, scales 16-byte aligned", fn);
   p->k = c->k;
   p->v = c->v;
   p->k_scale = quant ? c->k_scale : nullptr;

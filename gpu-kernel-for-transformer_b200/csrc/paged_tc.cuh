@@ -7,14 +7,14 @@
 // the last 128 % group rows stay unused). CTA = two such tiles A and B of one
 // (sequence, key/value head) that share every 128-key tile, and one range of
 // the keys; 12 warps (8 bit: 16), one CTA per SM:
-//   warps 2..5, 6..9  softmax of A and of B; thread = row = TMEM lane
-//   warps 1, 10       MMA issuers of A and of B (one lane)
+//   warps 4..7, 8..11  softmax of A and of B; thread = row = TMEM lane
+//   warps 1, 2         MMA issuers of A and of B (one lane)
 //   fp16:  warp 0 loads K and V, a TMA box per page and 64 columns (lane =
-//          box); warp 11 looks after V tiles that hold keys which not every
+//          box); warp 3 looks after V tiles that hold keys which not every
 //          row sees
-//   8 bit: warp 0 loads raw tiles (a box per page), warps 11..14 expand 32 rows
+//   8 bit: warp 0 loads raw tiles (a box per page), warps 12..15 expand 32 rows
 //          each of every K and V tile to fp16, a lane per row (both tiles are
-//          swizzled: no bank conflicts)
+//          swizzled: no bank conflicts), warp 3 brings the scales
 // A key tile is 128 consecutive positions, 128 / page_size pages or half of
 // one; pages outside the pool are boxes outside the tensor map and read as
 // zeros.
@@ -30,12 +30,12 @@
 // computed as soon as this one is in registers; head_dim 128: O fills half of
 // TMEM and P lies over S.
 //
-// 8-bit values are expanded as code * scale in fp16. The scale s is used as
-// m * 2^k with an fp16 m: int8 codes are placed behind the exponent of
-// 2^(10+k) (as 1024 + u in units of 2^k), so that subtracting 1152 * 2^k gives
-// code * 2^k exactly, and one multiplication by m follows; e4m3 codes convert
-// exactly and are multiplied by m and by 2^k. m's rounding and the product's
-// are each half an fp16 step, small scales lose nothing more.
+// 8-bit codes are expanded to fp16 exactly, without the scales: a key's scale
+// multiplies its column of scores, a value's its column of weights, in fp32 (as
+// fp16 factors of the tiles they cost as much, in the warps that expand, and
+// five times the error: a key's rounded scale multiplies its whole score).
+// Weights are divided by a unit U, the largest scale so far or at least 1/16 of
+// it, before they are rounded to fp16; U is put back at the end.
 //
 // What a row does not see must not reach it, and 0 * inf does: V rows behind
 // the sequence are cleared; in tiles that some rows of the CTA see and others
@@ -53,7 +53,9 @@ namespace {
 constexpr int kPtConvert = 4;  // 8 bit: warps that expand
 constexpr int kPtTile = 128;
 constexpr float kPtRescale = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8
-constexpr int kPtPoly = 2;          // of 8 pairs of exponentials, on the FMA pipe
+// Of 8 pairs of exponentials, so many on the FMA pipe (8 bit: it has the scales
+// to multiply as well).
+constexpr int kPtPoly = 2, kPtPolyQuant = 1;
 constexpr uint32_t kPtCols = 512;
 
 template <int CODE, int HD>
@@ -70,8 +72,12 @@ struct PtCfg {
   static constexpr int kK = 2 * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kR = kV + kStages * kTileBytes;
-  static constexpr int kBar = kR + kRaws * kRawBytes;
-  static constexpr int kSmem = kBar + 512 + 1024;  // barriers + alignment slack
+  // 8 bit: scales of kSlots parts of tiles, K's times the softmax scale, V's over U
+  static constexpr int kSlots = 3;
+  static constexpr int kSc = kR + kRaws * kRawBytes;
+  static constexpr int kBar = kSc + (kQuant ? kSlots * 2 * 64 * 4 : 0);
+  static constexpr int kBarBytes = HD == 64 ? 1024 : 512;
+  static constexpr int kSmem = kBar + kBarBytes + 1024;  // barriers + alignment slack
   static constexpr bool kSepP = HD == 64 && !kQuant;  // P has its own TMEM columns
   static constexpr int kParts = kSepP ? 1 : 2;        // a tile's S in so many parts
   static constexpr int kKeys = kPtTile / kParts;   // keys of one
@@ -92,42 +98,14 @@ __device__ __forceinline__ void pt_load_4d(uint32_t dst, const CUtensorMap* map,
       : "memory");
 }
 
-// A row's scale as the expansion uses it: fp16 bits of m (low half), k + 64 (high).
+// Four codes to two fp16 pairs, exact.
 template <int CODE>
-__device__ __forceinline__ uint32_t pt_scale(float s) {
-  const int e = static_cast<int>((__float_as_uint(s) >> 23) & 0xff) - 127;
-  const int k = min(max(e, CODE == kCodeI8 ? -24 : -14), CODE == kCodeI8 ? 5 : 8);
-  const float m = s * __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
-  return static_cast<uint32_t>(__half_as_ushort(__float2half_rn(m))) |
-         (static_cast<uint32_t>(k + 64) << 16);
+__device__ __forceinline__ void pt_expand(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  lo = codes_to_h2<CODE, 0, 1>(x);
+  hi = codes_to_h2<CODE, 2, 3>(x);
 }
 
-// Four codes to two fp16 pairs, times the row's scale.
-template <int CODE>
-struct PtExpand {
-  uint32_t m, a, c;  // m twice; int8: high byte x 4, 1152 * 2^k; e4m3: 2^k
-  __device__ __forceinline__ explicit PtExpand(uint32_t packed) {
-    const int k = static_cast<int>(packed >> 16) - 64;
-    m = __byte_perm(packed, 0u, 0x1010);
-    if constexpr (CODE == kCodeI8) {
-      a = (0x64u + 4u * static_cast<uint32_t>(k)) * 0x01010101u;
-      c = (0x6480u + (static_cast<uint32_t>(k) << 10)) * 0x00010001u;
-    } else {
-      a = 0u;
-      c = (static_cast<uint32_t>(k + 15) << 10) * 0x00010001u;
-    }
-  }
-  __device__ __forceinline__ void operator()(uint32_t x, uint32_t& lo, uint32_t& hi) const {
-    if constexpr (CODE == kCodeI8) {
-      const uint32_t u = x ^ 0x80808080u;
-      lo = h2_bits(__hmul2(__hsub2(bits_h2(__byte_perm(u, a, 0x4140)), bits_h2(c)), bits_h2(m)));
-      hi = h2_bits(__hmul2(__hsub2(bits_h2(__byte_perm(u, a, 0x4342)), bits_h2(c)), bits_h2(m)));
-    } else {
-      lo = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_to_h2(x)), bits_h2(m)), bits_h2(c)));
-      hi = h2_bits(__hmul2(__hmul2(bits_h2(e4m3x2_hi_to_h2(x)), bits_h2(m)), bits_h2(c)));
-    }
-  }
-};
+constexpr float kPtUnit = 16.0f;  // U grows when a scale is more than so many times it
 
 // Adds the non-finite values of keys [lo, hi) to a finished row (rare; out of
 // the kernel's registers): exactly what its weights, all above 0, make of them.
@@ -207,9 +185,14 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   uint64_t* drain = o_done + 2 * N;     // [2]
   uint64_t* r_full = drain + 2;         // [R] raw tile loaded
   uint64_t* r_empty = r_full + R;       // [R] raw tile expanded by all its warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + R);
+  constexpr int SC = L::kSlots;
+  uint64_t* c_full = r_empty + R;       // [SC] scales of a part
+  uint64_t* c_empty = c_full + SC;      // [2][SC]
+  float2* units = reinterpret_cast<float2*>(c_empty + 2 * SC);  // [SC] (old U / U, U)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + SC);
   volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
-  static_assert((1 + 7 * S + 2 + 8 * N + 2 * R) * 8 + 8 <= 512, "barrier space");
+  float* scales = reinterpret_cast<float*>(smem + L::kSc);  // [SC][K 64, V 64]
+  static_assert((1 + 7 * S + 2 + 8 * N + 2 * R + 4 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q);
@@ -237,6 +220,11 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     for (int r = 0; r < R; ++r) {
       mbar_init(&r_full[r], 1);
       mbar_init(&r_empty[r], kPtConvert);
+    }
+    for (int c = 0; c < SC; ++c) {
+      mbar_init(&c_full[c], 1);
+      mbar_init(&c_empty[c], 4);
+      mbar_init(&c_empty[SC + c], 4);
     }
     *cleared = 0;
     fence_mbar_init();
@@ -291,7 +279,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     }
   };
 
-  if (warp == 0 || warp >= 11) {
+  if (warp == 0 || warp == 3 || warp >= 12) {
     if constexpr (!kQuant) {
       if (warp == 0) {
         // -------------------------------------------------- TMA of K and V
@@ -326,7 +314,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           mbar_wait(&k_full[j % S], (j / S) & 1, nullptr, 0);
         for (int j = max(0, issued - S); j < issued; ++j)
           mbar_wait(&v_full[j % S], (j / S) & 1, nullptr, 0);
-      } else if (warp == 11) {
+      } else {
         // ---------------------------------------------- V tiles not all see
         for (int j = 0; j < n_iter; ++j) {
           const int st = j % S, key0 = k_begin + j * kPtTile;
@@ -385,33 +373,23 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         mbar_wait(q_full, 0, nullptr, 0);
         for (int e = max(0, issued - R); e < issued; ++e)
           mbar_wait(&r_full[e % R], (e / R) & 1, nullptr, 0);
-      } else if (warp < 11 + kPtConvert) {
+      } else if (warp >= 12) {
         // ------------------------------------------------- expansion to fp16
-        const int r = (warp - 11) * 32 + lane;  // this lane's row of every tile
-        float sc[2];                            // its scales in K and V, a tile ahead
-        auto load_scales = [&](int j) {
-          const int key = k_begin + j * kPtTile + r;
-          const int page = j < n_iter && key < seq.len ? paged_page(p, b, key) : -1;
-          const int64_t so = page >= 0 ? paged_scale_offset(p, page, hk, key) : 0;
-          sc[0] = page >= 0 ? p.k_scale[so] : 0.f;
-          sc[1] = page >= 0 ? p.v_scale[so] : 0.f;
-        };
-        load_scales(0);
+        const int r = (warp - 12) * 32 + lane;  // this lane's row of every tile
         // Raw rows of 128 bytes: 16-byte chunk c at c ^ (r & 7); of 64 bytes: at
         // c ^ (r >> 1 & 3). fp16 rows: chunk c of a 64-column block at c ^ (r & 7).
         const uint32_t rx = HD == 128 ? (r & 7) << 4 : ((r >> 1) & 3) << 4;
         const uint32_t dx = (r & 7) << 4;
         for (int e = 0; e < total; ++e) {
           const int j = e >> 1, kv = e & 1, st = j % S, key0 = k_begin + j * kPtTile;
-          const PtExpand<CODE> expand(pt_scale<CODE>(kv ? sc[1] : sc[0]));
-          if (kv) load_scales(j + 1);
           if (!__all_sync(0xffffffffu,
                           mbar_wait_sleep(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) ||
               !stage_free(kv ? v_empty : k_empty, j))
             break;
           const uint8_t* src = smem + L::kR + (e % R) * L::kRawBytes + r * HD;
           uint8_t* dst = smem + (kv ? L::kV : L::kK) + st * L::kTileBytes + r * 128;
-          const bool partly = kv && key0 + kPtTile > lim_first;  // not every row sees all
+          // Not every row sees all of it: NaN codes must not leak (int8 has none).
+          const bool partly = CODE == kCodeE4M3 && kv && key0 + kPtTile > lim_first;
           const bool behind = partly && key0 + r >= seq.len;
           bool found = false;
 #pragma unroll
@@ -423,10 +401,10 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               uint32_t w[8];
-              expand(x[c].x, w[0], w[1]);
-              expand(x[c].y, w[2], w[3]);
-              expand(x[c].z, w[4], w[5]);
-              expand(x[c].w, w[6], w[7]);
+              pt_expand<CODE>(x[c].x, w[0], w[1]);
+              pt_expand<CODE>(x[c].y, w[2], w[3]);
+              pt_expand<CODE>(x[c].z, w[4], w[5]);
+              pt_expand<CODE>(x[c].w, w[6], w[7]);
               if (partly) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -450,9 +428,60 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
             mbar_arrive(&r_empty[e % R]);
           }
         }
+      } else {
+        // ------------------------------------------------------ the scales
+        float unit = 1e-37f;  // U (its reciprocal stays finite)
+        // Lane = two consecutive keys of the part, one part ahead.
+        float2 ks, vs;
+        auto load_scales = [&](int u) {
+          const int key = k_begin + u * L::kKeys + 2 * lane;
+          const int page = u < n_iter * N && key < seq.len ? paged_page(p, b, key) : -1;
+          const int64_t so = page >= 0 ? paged_scale_offset(p, page, hk, key) : 0;
+          ks = vs = make_float2(0.f, 0.f);
+          if (page >= 0) {
+            ks = *reinterpret_cast<const float2*>(p.k_scale + so);
+            vs = *reinterpret_cast<const float2*>(p.v_scale + so);
+            if (key + 1 >= seq.len) ks.y = vs.y = 0.f;
+          }
+        };
+        load_scales(0);
+        for (int u = 0; u < n_iter * N; ++u) {
+          const int slot = u % SC;
+          const uint32_t par = ((u / SC) - 1) & 1;
+          bool ok = true;
+          if (u >= SC) {
+            if (u - SC < nA * N) ok = mbar_wait_sleep(&c_empty[slot], par, err, kDevTimeoutEmpty);
+            if (ok && u - SC < nB * N)
+              ok = mbar_wait_sleep(&c_empty[SC + slot], par, err, kDevTimeoutEmpty);
+          }
+          if (!__all_sync(0xffffffffu, ok)) break;
+          if (k_begin + (u + 1) * L::kKeys > lim_first) {
+            // A scale that is not finite must not leak to rows that do not see it.
+            const bool x = !isfinite(vs.x), y = !isfinite(vs.y);
+            if (x) vs.x = 0.f;
+            if (y) vs.y = 0.f;
+            if (x || y) *cleared = 1;
+          }
+          const uint32_t vx = __float_as_uint(vs.x) & 0x7fffffffu, vy = __float_as_uint(vs.y) & 0x7fffffffu;
+          const float top = __uint_as_float(__reduce_max_sync(
+              0xffffffffu, max(vx < 0x7f800000u ? vx : 0u, vy < 0x7f800000u ? vy : 0u)));
+          float ratio = 1.f;
+          if (top > unit * kPtUnit) {
+            ratio = unit / top;
+            unit = top;
+          }
+          const float inv = 1.f / unit;
+          float2* dst = reinterpret_cast<float2*>(scales + slot * 128) + lane;
+          dst[0] = make_float2(ks.x * a.scale_log2, ks.y * a.scale_log2);
+          dst[32] = make_float2(vs.x * inv, vs.y * inv);
+          if (lane == 0) units[slot] = make_float2(ratio, unit);
+          load_scales(u + 1);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&c_full[slot]);
+        }
       }
     }
-  } else if (warp == 1 || warp == 10) {
+  } else if (warp == 1 || warp == 2) {
     // ------------------------------------------------ MMA issuer of tile x
     if (lane == 0) {
       const int x = warp == 1 ? 0 : 1;
@@ -551,7 +580,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     }
   } else {
     // ------------------------------------------------------------ softmax
-    const int x = (warp - 2) >> 2;
+    const int x = (warp - 4) >> 2;
     const int quarter = warp & 3;  // this warp's TMEM lanes [32*quarter, +32)
     const int row = quarter * 32 + lane;
     const int first = i0 + x * tile_tokens;
@@ -566,6 +595,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     const int lim_tile = lim_of(min(first, seq.n - 1));  // smallest of the tile
     float m_ref = -INFINITY;  // -inf: no key seen yet
     uint64_t lsum0 = 0, lsum1 = 0;
+    float unit = 1.f;  // 8 bit: U
     bool ok = true;
     auto softmax = [&](auto with_holes) {
     for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
@@ -587,6 +617,30 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x * N + h]);
+      }
+      // 8 bit: scores in the log2 domain from here on.
+      [[maybe_unused]] const float* sc = scales + (u % SC) * 128;
+      float ratio = 1.f;
+      if constexpr (kQuant) {
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(&c_full[u % SC], (u / SC) & 1, err, kDevTimeoutOther))) {
+          ok = false;
+          break;
+        }
+        const float2 un = units[u % SC];
+        ratio = un.x;
+        unit = un.y;
+#pragma unroll
+        for (int c = 0; c < KC; c += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(sc + c);
+          float y[4];
+          f2_unpack(f2_mul(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
+                           f2_pack(f.x, f.y)), y[0], y[1]);
+          f2_unpack(f2_mul(f2_pack(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])),
+                           f2_pack(f.z, f.w)), y[2], y[3]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[c + i] = __float_as_uint(y[i]);
+        }
       }
       if (key0 + KC > lim_tile) {  // warp-uniform
         const int c0 = lim_row - key0;
@@ -617,7 +671,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           mm[i] = fmax3(mm[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
       const float mx = fmaxf(fmax3(mm[0], mm[1], mm[2]),
                              fmax3(fmax3(mm[3], mm[4], mm[5]), mm[6], mm[7]));
-      const float m_new = mx * a.scale_log2;
+      const float m_new = kQuant ? mx : mx * a.scale_log2;
       bool rescale = false;
       float f = 1.f;
       if (u == 0) {
@@ -631,31 +685,40 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         lsum1 = f2_fma(lsum1, f2v, 0);
         rescale = true;
       }
+      if (kQuant && u > 0 && ratio != 1.f) rescale = true;  // the same for every row
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
       const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2);
       const uint64_t negm2 = f2_pack(-m_use, -m_use);
+      // P goes to TMEM 64 keys at a time; 8 bit: 32 (registers).
+      constexpr int PC = kQuant ? 32 : 64;
 #pragma unroll
-      for (int q = 0; q < KC / 64; ++q) {
-        uint32_t pr[32];
+      for (int q = 0; q < KC / PC; ++q) {
+        uint32_t pr[PC / 2];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int c = 64 * q + 2 * i;
-          const uint64_t arg =
-              f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, negm2);
-          uint64_t e;
-          if ((i & 7) < kPtPoly) {
-            uint64_t mant;
-            e = exp2_poly_nan_f2(arg, &mant);
-            lsum0 = f2_fma(mant, 0, lsum0);  // a NaN score makes the sum NaN
-          } else {
-            float a0, a1;
-            f2_unpack(arg, a0, a1);
-            e = f2_pack(fast_exp2(a0), fast_exp2(a1));
+        for (int i2 = 0; i2 < PC / 2; i2 += 2) {
+          [[maybe_unused]] float4 w;  // 8 bit: the values' scales
+          if constexpr (kQuant) w = *reinterpret_cast<const float4*>(sc + 64 + PC * q + 2 * i2);
+#pragma unroll
+          for (int i = i2; i < i2 + 2; ++i) {
+            const int c = PC * q + 2 * i;
+            const uint64_t x = f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            const uint64_t arg = kQuant ? f2_add(x, negm2) : f2_fma(x, c2, negm2);
+            uint64_t e;
+            if ((i & 7) < (kQuant ? kPtPolyQuant : kPtPoly)) {
+              uint64_t mant;
+              e = exp2_poly_nan_f2(arg, &mant);
+              lsum0 = f2_fma(mant, 0, lsum0);  // a NaN score makes the sum NaN
+            } else {
+              float a0, a1;
+              f2_unpack(arg, a0, a1);
+              e = f2_pack(fast_exp2(a0), fast_exp2(a1));
+            }
+            if (i & 1) lsum1 = f2_add(lsum1, e); else lsum0 = f2_add(lsum0, e);
+            if constexpr (kQuant) e = f2_mul(e, i == i2 ? f2_pack(w.x, w.y) : f2_pack(w.z, w.w));
+            float e0, e1;
+            f2_unpack(e, e0, e1);
+            pr[i] = pack_half2(e0, e1);
           }
-          if (i & 1) lsum1 = f2_add(lsum1, e); else lsum0 = f2_add(lsum0, e);
-          float e0, e1;
-          f2_unpack(e, e0, e1);
-          pr[i] = pack_half2(e0, e1);
         }
         if (q == 0) {
           // P's columns are free once the product of this part of the last tile
@@ -677,18 +740,23 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
               tmem_ld16(t_o + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              for (int i = 0; i < 16; ++i)
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * (f * ratio));
               tmem_st16(t_o + c, o);
             }
           }
         }
-        tmem_st32(t_p + h * L::kPPart + 32 * q, pr);
+        if constexpr (kQuant) tmem_st16(t_p + h * L::kPPart + 16 * q, pr);
+        else tmem_st32(t_p + h * L::kPPart + 32 * q, pr);
       }
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x * N + h]);
+      if (lane == 0) {
+        mbar_arrive(&p_full[x * N + h]);
+        if (kQuant) mbar_arrive(&c_empty[x * SC + u % SC]);
+      }
     }
     };
     if (holes) softmax(std::true_type{}); else softmax(std::false_type{});
@@ -704,7 +772,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     if (ok) {
       const bool fix = *cleared != 0;  // the writer arrived before the last product
       const int head = hk * group + row % group;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = l == 0.f ? 0.f : unit / l;
       const int64_t at = (static_cast<int64_t>(seq.row0 + tok) * (p.kv_heads * group) + head) *
                              a.splits + split;
       __half* dst = a.out + static_cast<int64_t>(seq.row0 + tok) * a.ld_out + head * HD;
@@ -725,7 +793,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
             float4* d4 = reinterpret_cast<float4*>(a.part_o + at * HD + c);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              d4[i] = make_float4(of[4 * i], of[4 * i + 1], of[4 * i + 2], of[4 * i + 3]);
+              d4[i] = make_float4(of[4 * i] * unit, of[4 * i + 1] * unit, of[4 * i + 2] * unit,
+                                  of[4 * i + 3] * unit);
             if (c == 0) a.part_ml[at] = make_float2(m_ref, l);
           } else {
             uint4* d4 = reinterpret_cast<uint4*>(dst + c);

@@ -293,7 +293,7 @@ typedef enum tfx_cache_dtype {
  * k[p*page_stride + t*token_stride + h*head_stride + e] (in elements of the
  * dtype; the same strides for v), so a page may hold its tokens head by head
  * or its heads token by token. Scales (8-bit types; NULL for fp16):
- * k_scale[(p*kv_heads + h)*page_size + t].
+ * k_scale[(p*kv_heads + h)*page_size + t], 16-byte aligned.
  * page_size: 16, 32, 64, 128 or 256; head_dim: 8, 16, 32, 64, 128 or 256 (8-bit
  * types: 16 and up); k and v 16-byte aligned, each stride a multiple of 16
  * bytes and at least head_dim.

@@ -170,7 +170,7 @@ def attention(pool, q, group, causal=True, scale=None, absent=()):
     return out.flatten(1), mag.flatten(1), expo.expand(-1, -1, hd).flatten(1)
 
 
-def tolerance(pool, ref, mag, expo, rounded_keys=False):
+def tolerance(pool, ref, mag, expo):
     """How far fp16 results may be off the 64-bit ones, element by element.
 
     Half a step of the result (2^-11 of it; 2^-25 where it is subnormal), and of
@@ -179,17 +179,12 @@ def tolerance(pool, ref, mag, expo, rounded_keys=False):
     within 2^-13 of themselves (7.5e-5, the polynomial's). Sums over hd
     products and over the keys in fp32 whose steps may truncate (2^-23 each): on
     the exponent hd + 8 steps of its largest sum, on the result one step for each
-    16 keys and 8 more. rounded_keys: cached values expanded to fp16 before the
-    products with a scale in fp16 (two half steps, 2^-10, of the exponent's sum and
-    of each value)."""
+    16 keys and 8 more."""
     n = max([kv for _, kv in pool.lens] + [1])
     most = max([float(torch.nan_to_num(pool.values(b, 1), 0, 0, 0).abs().max()) if kv else 0.0
                 for b, (_, kv) in enumerate(pool.lens)] + [0.0])
     on_exp = (pool.hd + 8) * 2.0 ** -23 * expo + 2.0 ** -21
     per = 2.0 ** -11 + 2.0 ** -13 + (n / 16 + 8) * 2.0 ** -23
-    if rounded_keys:
-        on_exp = on_exp + 2.0 ** -10 * expo
-        per += 2.0 ** -10
     # an error d of the exponents moves weights by at most exp(2d) - 1 of themselves
     return 2.0 ** -11 * ref.abs() + 2.0 ** -25 + (per + torch.expm1(2 * on_exp)) * mag + \
         n * 2.0 ** -25 * most
