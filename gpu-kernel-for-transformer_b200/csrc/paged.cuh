@@ -35,6 +35,11 @@ struct Paged {
 int check_paged(const char* fn, const tfx_paged_cache* cache, const tfx_paged_batch* batch,
                 Paged* p);
 
+// Whether `rows` fp16 rows of `width` elements at a (row pitch ld_a) and at b share
+// an element.
+bool rows_overlap(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int64_t rows,
+                  int64_t width);
+
 // One sequence of the batch, clamped: rows [row0, row0 + n) of the packed
 // tensors at positions pos0 + i; len: keys that may be looked up.
 struct PagedSeq {
@@ -177,6 +182,13 @@ __device__ __forceinline__ int paged_split_keys(const PagedAttn& a, const PagedS
 // otherwise split 0 holds all of them and writes the rows itself.
 __device__ __forceinline__ bool paged_is_split(const PagedAttn& a, const PagedSeq& s) {
   return a.splits > 1 && s.len > paged_split_keys(a, s);
+}
+
+// End of the keys of a split (the last one takes whatever is left: max_kv_len may
+// have been less than a sequence's length).
+__device__ __forceinline__ int paged_split_end(const PagedAttn& a, const PagedSeq& s, int split,
+                                               int k_begin) {
+  return split == a.splits - 1 ? s.len : min(s.len, k_begin + paged_split_keys(a, s));
 }
 
 // Rows of a CTA of the mma.sync kernel for rows = max_query_len * group.

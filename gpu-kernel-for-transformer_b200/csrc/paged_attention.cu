@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(128)
       const PagedSeq s = paged_seq(p, b);
       if (paged_is_split(a, s) && tok >= s.row0 && tok < s.row0 + s.n) {
         const int lim = a.causal ? min(s.len, max(0, s.pos0 + (tok - s.row0) + 1)) : s.len;
-        n = (lim + paged_split_keys(a, s) - 1) / paged_split_keys(a, s);
+        n = min(a.splits, (lim + paged_split_keys(a, s) - 1) / paged_split_keys(a, s));
         if (n == 0) n = -1;  // a split sequence's row that sees no key
       }
     }
@@ -284,6 +284,8 @@ int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* 
       ld_q % 8 != 0 || ld_out % 8 != 0)
     return fail(TFX_ERR_MISALIGNED,
                 "%s: pointers 16-byte aligned and leading dims multiples of 8 needed", fn);
+  if (rows_overlap(q, ld_q, out, ld_out, batch->num_tokens, width))
+    return fail(TFX_ERR_INVALID_ARGUMENT, "%s: out must not overlap q", fn);
   const Plan pl = make_plan(cache, batch, q_heads);
   if (pl.bytes > 0) {
     if (workspace == nullptr) return fail(TFX_ERR_INVALID_ARGUMENT, "%s: null workspace", fn);

@@ -353,6 +353,17 @@ int check_copy(const char* fn, const void* k, int64_t ld_k, const void* v, int64
 
 }  // namespace
 
+bool rows_overlap(const void* a, int64_t ld_a, const void* b, int64_t ld_b, int64_t rows,
+                  int64_t width) {
+  if (rows <= 0) return false;
+  const int64_t a0 = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a)) / 2;
+  const int64_t b0 = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b)) / 2;
+  if (a0 + (rows - 1) * ld_a + width <= b0 || b0 + (rows - 1) * ld_b + width <= a0) return false;
+  if (ld_a != ld_b) return true;
+  const int64_t d = (a0 < b0 ? b0 - a0 : a0 - b0) % ld_a;  // columns apart in a common row
+  return d < width || ld_a - d < width;
+}
+
 int check_paged(const char* fn, const tfx_paged_cache* c, const tfx_paged_batch* b, Paged* p) {
   if (c == nullptr || b == nullptr)
     return fail(TFX_ERR_INVALID_ARGUMENT, "%s: null cache or batch", fn);
@@ -438,6 +449,9 @@ int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* batch, t
   Paged p;
   const int st = check_copy("tfx_paged_read", k_out, ld_k, v_out, ld_v, cache, batch, &p);
   if (st != TFX_OK || p.num_tokens == 0) return st;
+  if (rows_overlap(k_out, ld_k, v_out, ld_v, p.num_tokens,
+                   static_cast<int64_t>(cache->kv_heads) * cache->head_dim))
+    return fail(TFX_ERR_INVALID_ARGUMENT, "tfx_paged_read: k_out and v_out overlap");
   return launch_copy_code(false, cache, reinterpret_cast<__half*>(k_out), ld_k,
                           reinterpret_cast<__half*>(v_out), ld_v, p,
                           reinterpret_cast<cudaStream_t>(stream));

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
     if (is_split ? static_cast<int64_t>(split) * a.kps >= lim_last : split > 0) return;
     if (is_split) {
       k_begin = split * a.kps;
-      k_end = min(lim_last, k_begin + a.kps);
+      k_end = min(lim_last, paged_split_end(a, seq, split, k_begin));
     }
   }
 

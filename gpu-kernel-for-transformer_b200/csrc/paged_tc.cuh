@@ -155,7 +155,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   // Splits behind the sequence (64 bits: splits is the larger kernel's number).
   if (is_split ? static_cast<int64_t>(split) * a.kps_tc >= seq.len : split > 0) return;
   const int k_begin = is_split ? split * a.kps_tc : 0;
-  const int k_stop = is_split ? k_begin + a.kps_tc : seq.len;  // of the split
+  const int k_stop = is_split ? paged_split_end(a, seq, split, k_begin) : seq.len;  // of the split
   auto tiles_of = [&](int x) {
     const int first = i0 + x * tile_tokens;
     if (first >= seq.n) return 0;

@@ -354,7 +354,8 @@ TFX_API int tfx_paged_append(const tfx_half* k, int64_t ld_k, const tfx_half* v,
 /*
  * Reads k and v of the same tokens (the last n of each sequence: the whole
  * sequence where n = kv_len) into fp16 rows laid out as tfx_paged_append's.
- * Tokens without a page, and positions before 0, read as zeros.
+ * Tokens without a page, and positions before 0, read as zeros. k_out and
+ * v_out must not overlap (slices of one row are fine).
  */
 TFX_API int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* batch,
                            tfx_half* k_out, int64_t ld_k, tfx_half* v_out, int64_t ld_v,
@@ -368,8 +369,8 @@ TFX_API int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* 
  * has no part in its row, whatever its cached values are (NaN included); a
  * row that sees no key is zero.
  * q, out: fp16, element (row, h, e) at q[row*ld_q + h*head_dim + e], 16-byte
- * aligned, ld a multiple of 8; scale > 0 and finite. q_heads is a multiple of
- * cache->kv_heads. The new tokens' keys and values must be in the cache
+ * aligned, ld a multiple of 8, not overlapping (slices of one row are fine);
+ * scale > 0 and finite. q_heads is a multiple of cache->kv_heads. The new tokens' keys and values must be in the cache
  * (tfx_paged_append before, on the same stream).
  * workspace: tfx_paged_attention_workspace_bytes() of the same arguments (0:
  * may be NULL), 256-byte aligned, for partial results of keys split over

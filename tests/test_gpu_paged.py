@@ -335,6 +335,61 @@ def test_no_new_tokens(pkg, dev):
     assert q.shape[0] == 0
 
 
+@pytest.mark.parametrize("dtype", [F16, I8], ids=["fp16", "int8"])
+@pytest.mark.parametrize("lens,hint", [([(1, 5000), (1, 300)], 700), ([(1, 9000)], 2000),
+                                       ([(90, 9000), (1, 4000)], 4096), ([(200, 7000)], 1)])
+def test_sequences_longer_than_the_hint(pkg, dev, dtype, lens, hint):
+    """max_kv_len only sizes the split over keys: longer sequences are attended whole."""
+    pool = pr.Pool(lens, 64, 1, 64, dtype, 13)
+    cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled()))
+    batch = _batch(pkg, dev, pool, max_query_len=max(n for n, _ in lens), max_kv_len=hint)
+    q = torch.randn(pool.tokens, 2, 64, generator=pool.q_gen).half()
+    got = pkg.ops.paged_attention(q.to(dev), cache, batch).double().cpu()
+    _check(pool, got, q, 2)
+
+
+@pytest.mark.parametrize("dtype", [F16, E4], ids=["fp16", "e4m3"])
+def test_shared_pages_and_packed_slices(pkg, dev, dtype):
+    """Two sequences share the pages of a common prefix; q, k, v are slices of one
+    packed projection and the results slices of one packed buffer."""
+    hd, heads, page = 64, 2, 16
+    pool = pr.Pool([(3, 67), (3, 70)], page, heads, hd, dtype, 3)
+    for which in (0, 1):  # the first 48 tokens are the same
+        pool.data[1][which][:48] = pool.data[0][which][:48]
+    pool.table[1, :3] = pool.table[0, :3]
+    cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled(upto=[64, 67])))
+    batch = _batch(pkg, dev, pool)
+    q = torch.randn(pool.tokens, heads, hd, generator=pool.q_gen).half()
+    packed = torch.stack((q, pool.rows(0), pool.rows(1)), 1).to(dev)  # [T, 3, heads, hd]
+    pkg.ops.paged_append(packed[:, 1], packed[:, 2], cache, batch)
+    both = torch.zeros(pool.tokens, 2, heads, hd, dtype=F16, device=dev)
+    pkg.ops.paged_read(cache, batch, out=(both[:, 0], both[:, 1]))
+    for which in (0, 1):
+        want = torch.cat([pool.values(b, which)[kv - 3:] for b, (_, kv) in enumerate(pool.lens)])
+        assert torch.equal(both[:, which].cpu(), want.float().half())
+    out = torch.zeros(pool.tokens, 3 * heads * hd, dtype=F16, device=dev)[:, heads * hd:2 * heads * hd]
+    got = pkg.ops.paged_attention(packed[:, 0], cache, batch, out=out)
+    _check(pool, got.double().cpu(), q, 1)
+
+
+def test_two_streams_at_once(pkg, dev):
+    """Split decodes on two streams of one cache at the same time, many times over."""
+    pool = pr.Pool([(1, 6000), (1, 5000)], 64, 1, 128, I8, 5)
+    cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled()))
+    batch = _batch(pkg, dev, pool, **_hints(pool))
+    qs = [torch.randn(2, 8, 128, generator=pool.q_gen).half().to(dev) for _ in range(2)]
+    alone = [pkg.ops.paged_attention(q, cache, batch) for q in qs]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in qs], [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(pkg.ops.paged_attention(qs[i], cache, batch))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
 @pytest.mark.parametrize("dtype", [F16, I8, E4], ids=["fp16", "int8", "e4m3"])
 def test_running_sequences(pkg, dev, dtype):
     """Prompts written whole, then single tokens and drafts, as a server runs:

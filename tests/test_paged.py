@@ -90,6 +90,12 @@ def test_bad_calls(lib):
                      ({"scale": 3e38}, inv), ({"q": 4100}, mis), ({"out": 8200}, mis),
                      ({"ld_q": 260}, mis), ({"ld_out": 260}, mis)):
         assert attend(**kw) == want, kw
+    # outputs over inputs, K over V; slices of one packed row are fine
+    assert attend(out=4096) == inv and b"overlap" in lib.tfx_last_error_message()
+    assert attend(out=4096 + 512 * 3) == inv  # 7 rows of 512 bytes
+    assert attend(out=4096 + 128, ld_q=264) == inv
+    assert lib.tfx_paged_read(c, b, 4096, 128, 4096 + 256, 128, None) == inv
+    assert lib.tfx_paged_read(c, b, 4096, 256, 4096 + 128, 256, None) == inv
     # keys long enough to be split: the workspace is checked
     c, b = _structs(L, max_pages=4096, table_stride=4096, max_kv_len=65536)
     need = lib.tfx_paged_attention_workspace_bytes(c, b, 4)
