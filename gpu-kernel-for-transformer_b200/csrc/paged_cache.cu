@@ -15,7 +15,7 @@
 //        near a border ulp(s) <= ulp(x), so e has at most 24), and |e| against
 //        s/2 tells which.
 //  e4m3: the quotient's bits behind the 3 of the code decide unless they are
-//        within 4 ulp of a half (or the code is subnormal); then the quotient
+//        within 8 ulp of a half (or the code is subnormal); then the quotient
 //        is divided out and rounded to odd, which rounds on correctly.
 // Eight elements are quantised without a branch, and again with these
 // corrections where one of them needs it (a few in 10^5 for int8).
@@ -58,6 +58,15 @@ __device__ __forceinline__ uint32_t row_absmax(const uint4& x) {
   return m;
 }
 
+// x / 127 or x / 448, correctly rounded: a product with the rounded reciprocal and
+// one correction by the exact remainder (equal to the division for every fp16).
+template <int CODE>
+__device__ __forceinline__ float scale_of(float top) {
+  constexpr float kTop = CODE == kCodeI8 ? 127.0f : 448.0f, kInv = 1.0f / kTop;
+  const float q = top * kInv;
+  return fmaf(fmaf(-q, kTop, top), kInv, q);
+}
+
 // Eight codes of a row whose max|x| has the fp16 bits `top`; *scale gets s.
 template <int CODE>
 __device__ __forceinline__ uint2 quantise(const uint4& x, uint32_t top, float* scale) {
@@ -65,11 +74,12 @@ __device__ __forceinline__ uint2 quantise(const uint4& x, uint32_t top, float* s
     *scale = __uint_as_float(0x7fc00000u);
     return make_uint2(0u, 0u);
   }
-  const float s = __fdiv_rn(__half2float(__ushort_as_half(static_cast<unsigned short>(top))),
-                            CODE == kCodeI8 ? 127.0f : 448.0f);
+  const float s = scale_of<CODE>(__half2float(__ushort_as_half(static_cast<unsigned short>(top))));
   *scale = s;
   if (top == 0u) return make_uint2(0u, 0u);
-  const float inv = __frcp_rn(s), half_s = 0.5f * s;
+  float inv;  // within an ulp: the checks below allow for it
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float half_s = 0.5f * s;
   float f[8];
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -105,9 +115,9 @@ __device__ __forceinline__ uint2 quantise(const uint4& x, uint32_t top, float* s
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       y[i] = f[i] * inv;
-      const uint32_t bits = __float_as_uint(y[i]);
-      border |= ((bits & 0xfffffu) - 0x7fffcu) <= 8u;
-      border |= (bits & 0x7fffffffu) - 1u < 0x3c800000u - 1u;  // below 2^-6, not 0
+      // The low 20 bits within 8 of a half, tested at the top of the word; below 2^-6.
+      border |= __float_as_uint(y[i]) * 4096u - (0x7fff8u << 12) <= (16u << 12);
+      border |= fabsf(y[i]) < 0.015625f;
     }
     if (border) {
 #pragma unroll

@@ -360,7 +360,7 @@ def paged_attention(
     if n == 0:
         return out
     lib = _lib.load()
-    need = lib.tfx_paged_attention_workspace_bytes(cache._ref, batch._ref, heads)
+    need = batch._workspace_bytes(lib, cache, heads)
     ws = None
     if need > 0:
         # A workspace of its own for each call, from the stream's allocator: calls

@@ -94,6 +94,7 @@ class PagedKVCache:
             *strides[:3])
         self._ref = ctypes.byref(self._struct)
         self._half = k.new_empty(0, dtype=torch.float16)  # outputs are allocated from it
+        self._geometry = (heads, hd, page_size, k.dtype)
 
 
 def _strides(t: torch.Tensor):
@@ -153,3 +154,13 @@ class PagedBatch:
             query_start.data_ptr(), kv_len.data_ptr(), b, num_tokens, self.max_query_len,
             min(self.max_kv_len, 1 << 30))
         self._ref = ctypes.byref(self._struct)
+        self._workspaces = {}
+
+    def _workspace_bytes(self, lib, cache: PagedKVCache, q_heads: int) -> int:
+        """Workspace of an attention call (a function of sizes only, looked up once)."""
+        key = (q_heads, cache._geometry)
+        need = self._workspaces.get(key)
+        if need is None:
+            need = lib.tfx_paged_attention_workspace_bytes(cache._ref, self._ref, q_heads)
+            self._workspaces[key] = need
+        return need
