@@ -8,8 +8,12 @@ namespace {
 // Keys of a split: a multiple of every kernel's round of tiles over its warps.
 constexpr int kSplitKeys = 256;
 // Sequences with more rows (new tokens x query heads per key/value head) may go
-// to the tcgen05 kernel, whose tiles have 128.
-constexpr int kTcRows = 32;
+// to the tcgen05 kernel, whose tiles have 128. (From 33 to 64 rows it is up to 1.4
+// times faster at head_dim 128 in fp16 and hardly elsewhere, but drafts of 2 to 6
+// tokens in groups of 8 then fall to both kernels, one behind the other.)
+constexpr int kTcRows = 64;
+// Partial results kept for a call at most, where few splits would do as well.
+constexpr int64_t kPartBytes = 128 << 20;
 
 // out[row] = sum over splits of partial O scaled to the common maximum, over
 // the sum of their sums. `wpr` warps of the CTA per (token, head) row: one when
@@ -168,7 +172,7 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   }
   pl.kps_tc = round_keys(kv, tc_parts);
 
-  // Which kernel: more than 32 rows, and enough work. Times in ns, fitted to
+  // Which kernel: more than kTcRows rows, and enough work. Times in ns, fitted to
   // both kernels at 1 to 64 sequences of 2 000 to 30 000 tokens, 8 heads, 16 to 128
   // rows; e.g. 128 rows, head_dim 64, fp16: 1 x 2 000 26 us tcgen05, 13 mma.sync;
   // 1 x 30 000 40 and 56; 16 x 3 000 47 and 108; 64 x 4 000 210 and 382.
@@ -183,8 +187,8 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   pl.tc_rows = !pl.tc ? 0x7fffffff : pl.small ? kTcRows : 0;
 
   // mma.sync: CTAs to an SM by registers and shared memory; a start costs about
-  // as much as 400 keys, a second launch to join as much as 512 (beside the
-  // tcgen05 kernel 3000: its many rows are looked at by the same launch).
+  // as much as 400 keys, a second launch to join as much as 512 and one for every
+  // 100 rows that it looks at (beside the tcgen05 kernel: all of its rows).
   const int64_t small_rows = pl.rows < pl.tc_rows ? pl.rows : pl.tc_rows;
   pl.block_rows = paged_rows_block(hd, small_rows);
   const int row_bytes = hd * (quant ? 1 : 2);
@@ -193,8 +197,10 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   const int64_t blocks = pairs * ((small_rows + pl.block_rows - 1) / pl.block_rows);
   double alone = 0., joined = 0.;
   const int64_t share = cut(blocks, slots, kv, 400, 0, 128, 8, &alone);
-  const int64_t parts =
-      cut(blocks, slots, kv, 400, pl.tc ? 3000 : 512, kSplitKeys, pl.tc ? 8 : 1024, &joined);
+  const int64_t all_rows = static_cast<int64_t>(b->num_tokens) * q_heads;
+  int64_t most = kPartBytes / ((all_rows + 1) * (hd + 2) * 4);
+  most = most < 1 ? 1 : most > 1024 ? 1024 : most;
+  const int64_t parts = cut(blocks, slots, kv, 400, 512 + all_rows / 100, kSplitKeys, most, &joined);
   // (CTAs of a cluster wait for one another at its end: for one wave only)
   if (!pl.tc && alone <= joined && (share == 1 || 4 * blocks * share <= 5 * slots)) {
     pl.cluster = share > 1 ? static_cast<int>(share) : 0;

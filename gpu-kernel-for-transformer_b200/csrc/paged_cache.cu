@@ -294,9 +294,9 @@ __global__ void __launch_bounds__(kThreads)
 template <int CODE, int HD>
 int launch_copy(bool append, __half* k, int64_t ld_k, __half* v, int64_t ld_v, const Paged& p,
                 cudaStream_t stream) {
-  // Tokens of a CTA: about 8192 elements of K, fewer where that leaves SMs idle.
+  // Tokens of a CTA: about 16384 elements of K, fewer where that leaves SMs idle.
   const int width = p.kv_heads * HD;
-  int tokens = width < 8192 ? 8192 / width : 1;
+  int tokens = width < 16384 ? 16384 / width : 1;
   const int spread = (p.num_tokens + 4 * num_sms() - 1) / (4 * num_sms());
   if (tokens > spread) tokens = spread;
   if (tokens > kMostTokens) tokens = kMostTokens;
