@@ -156,7 +156,7 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   // Whole waves of equal CTAs, and what the partial results of every row cost
   // (written and read once, in units of a key's time): cutting pays where there
   // are few row blocks.
-  const int tokens = group <= 128 ? 2 * (128 / group) : 1;
+  const int tokens = group <= 128 ? (hd == 256 ? 1 : 2) * (128 / group) : 1;
   const int64_t tc_blocks = pairs * ((pl.q + tokens - 1) / tokens);
   int64_t tc_parts = 1;
   double tc_cost = 0., tc_keys = 0.;
@@ -176,11 +176,14 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   // both kernels at 1 to 64 sequences of 2 000 to 30 000 tokens, 8 heads, 16 to 128
   // rows; e.g. 128 rows, head_dim 64, fp16: 1 x 2 000 26 us tcgen05, 13 mma.sync;
   // 1 x 30 000 40 and 56; 16 x 3 000 47 and 108; 64 x 4 000 210 and 382.
-  pl.tc = (hd == 64 || hd == 128) && group <= 128 && pl.rows > kTcRows;
+  pl.tc = hd >= 64 && group <= 128 && pl.rows > kTcRows;
   if (pl.tc) {
-    const double tc_ns = 10e3 + tc_keys * (hd == 64 ? (quant ? 12.5 : 11.) : (quant ? 22. : 13.));
-    const double rows_ns = 6e3 + static_cast<double>(pairs) * ((pl.rows + 31) / 32) * kv *
-                                     (hd == 64 ? (quant ? .06 : .05) : (quant ? .09 : .08));
+    const int i = hd == 64 ? 0 : hd == 128 ? 1 : 2;
+    constexpr double kTcKey[2][3] = {{11., 13., 16.}, {12.5, 22., 25.}};
+    constexpr double kRowsKey[2][3] = {{.05, .08, .16}, {.06, .09, .18}};  // of 32 rows
+    const double tc_ns = 10e3 + tc_keys * kTcKey[quant][i];
+    const double rows_ns =
+        6e3 + static_cast<double>(pairs) * ((pl.rows + 31) / 32) * kv * kRowsKey[quant][i];
     pl.tc = tc_ns < rows_ns;
   }
   pl.small = !pl.tc || b->batch > 1;  // a single sequence has all the rows

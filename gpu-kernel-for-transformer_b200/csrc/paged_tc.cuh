@@ -1,5 +1,5 @@
 // Attention of many query rows (chunks of prompts) over a paged cache on the
-// 5th-generation tensor cores, head_dim 64 and 128. Included by one
+// 5th-generation tensor cores, head_dim 64, 128 and 256. Included by one
 // translation unit per cache type.
 //
 // The `group` query heads that read one key/value head are rows of the same
@@ -15,7 +15,7 @@
 //   8 bit: warp 0 loads raw tiles (a box per page), warps 12..15 expand 32 rows
 //          each of every K and V tile to fp16, a lane per row (both tiles are
 //          swizzled: no bank conflicts), warp 3 brings the scales
-// A key tile is 128 consecutive positions, 128 / page_size pages or half of
+// A key tile is 128 consecutive positions, 128 / page_size pages or a part of
 // one; pages outside the pool are boxes outside the tensor map and read as
 // zeros.
 //
@@ -28,7 +28,8 @@
 // 1029 TFLOP/s, one fp16 head_dim 128 sequence of 16k, not causal). head_dim 64:
 // P has columns of its own (S 2 x 128, P 2 x 64, O 2 x 64), so the next S is
 // computed as soon as this one is in registers; head_dim 128: O fills half of
-// TMEM and P lies over S.
+// TMEM and P lies over S. head_dim 256: one query tile to a CTA and tiles of 64
+// keys (O alone is 256 columns, Q 64 KB), two of them in S.
 //
 // 8-bit codes are expanded to fp16 exactly, without the scales: a key's scale
 // multiplies its column of scores, a value's its column of weights, in fp32 (as
@@ -62,14 +63,17 @@ template <int CODE, int HD>
 struct PtCfg {
   static constexpr bool kQuant = CODE != kCodeF16;
   static constexpr int kThreads = kQuant ? 512 : 384;
+  static constexpr int kNT = HD == 256 ? 1 : 2;            // query tiles (TMEM, shared memory)
+  static constexpr int kKT = HD == 256 ? 64 : kPtTile;     // keys of a K or V tile
   static constexpr int kStages = HD == 64 ? 4 : 2;
-  static constexpr int kBlocks = HD / 64;
-  static constexpr int kBlockBytes = kPtTile * 128;
-  static constexpr int kTileBytes = kPtTile * HD * 2;
+  static constexpr int kBlocks = HD / 64;                  // 64-column blocks, 128-byte rows
+  static constexpr int kQBlock = kPtTile * 128, kQBytes = kPtTile * HD * 2;
+  static constexpr int kBlockBytes = kKT * 128, kTileBytes = kKT * HD * 2;
   static constexpr int kRaws = kQuant ? (HD == 64 ? 4 : 2) : 0;  // raw tiles: K and V in turn
-  static constexpr int kRawBytes = kPtTile * HD;
+  static constexpr int kRawRow = HD < 128 ? HD : 128;            // bytes: blocks of 128 columns
+  static constexpr int kRawBytes = kKT * HD;
   static constexpr int kQ = 0;
-  static constexpr int kK = 2 * kTileBytes;
+  static constexpr int kK = kNT * kQBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kR = kV + kStages * kTileBytes;
   // 8 bit: scales of kSlots parts of tiles, K's times the softmax scale, V's over U
@@ -79,13 +83,13 @@ struct PtCfg {
   static constexpr int kBarBytes = HD == 64 ? 1024 : 512;
   static constexpr int kSmem = kBar + kBarBytes + 1024;  // barriers + alignment slack
   static constexpr bool kSepP = HD == 64 && !kQuant;  // P has its own TMEM columns
-  static constexpr int kParts = kSepP ? 1 : 2;        // a tile's S in so many parts
-  static constexpr int kKeys = kPtTile / kParts;   // keys of one
+  static constexpr int kParts = kSepP || kKT == 64 ? 1 : 2;  // a tile's S in so many parts
+  static constexpr int kKeys = kKT / kParts;                 // keys of one
+  static constexpr int kBufs = kSepP ? 1 : 2;                // parts of S in TMEM at a time
   static constexpr uint32_t kColP = kSepP ? 2 * kPtTile : 0;
-  static constexpr uint32_t kPStride = kSepP ? kPtTile / 2 : kPtTile;  // of a tile
-  static constexpr uint32_t kPPart = kSepP ? kKeys / 2 : kKeys;        // of a part
-  static constexpr uint32_t kColO = kSepP ? 3 * kPtTile : 2 * kPtTile;
-  static_assert(kColO + 2 * HD <= kPtCols, "TMEM budget");
+  static constexpr uint32_t kPStride = kSepP ? kPtTile / 2 : kPtTile;  // of a query tile
+  static constexpr uint32_t kColO = kNT == 1 ? kPtTile : kSepP ? 3 * kPtTile : 2 * kPtTile;
+  static_assert(kColO + kNT * HD <= kPtCols, "TMEM budget");
   static_assert(kSmem <= 227 * 1024, "shared-memory budget");
 };
 
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   const int rb = row_blocks - 1 - static_cast<int>(blockIdx.z) / a.splits;
   const int group = a.group, tile_tokens = kPtTile / group;
   const PagedSeq seq = paged_seq(p, b);
-  const int i0 = rb * 2 * tile_tokens;  // first token
+  const int i0 = rb * L::kNT * tile_tokens;  // first token
   if (i0 >= seq.n || !paged_is_tc(a, seq)) return;
   auto lim_of = [&](int i) {  // token i sees keys [0, lim)
     return a.causal ? min(seq.len, max(0, seq.pos0 + i + 1)) : seq.len;
@@ -160,13 +164,13 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     const int first = i0 + x * tile_tokens;
     if (first >= seq.n) return 0;
     const int lim = min(lim_of(min(first + tile_tokens, seq.n) - 1), k_stop);
-    return lim > k_begin ? (lim - k_begin + kPtTile - 1) / kPtTile : 0;
+    return lim > k_begin ? (lim - k_begin + L::kKT - 1) / L::kKT : 0;
   };
-  const int nA = tiles_of(0), nB = tiles_of(1), n_iter = max(nA, nB);
+  const int nA = tiles_of(0), nB = L::kNT == 2 ? tiles_of(1) : 0, n_iter = max(nA, nB);
   if (is_split && n_iter == 0) return;  // not looked at when the splits are joined
   // Keys from here on are not seen by every row; the first tile that holds one.
   const int lim_first = lim_of(i0);
-  const int j_partly = max(0, lim_first - k_begin) / kPtTile;
+  const int j_partly = max(0, lim_first - k_begin) / L::kKT;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -177,12 +181,12 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   uint64_t* v_ready = v_full + S;       // V may be multiplied
   uint64_t* k_empty = v_ready + S;      // [2][S]
   uint64_t* v_empty = k_empty + 2 * S;  // [2][S]
-  constexpr int N = L::kParts;
-  uint64_t* s_full = v_empty + 2 * S;   // [2][N]
-  uint64_t* s_free = s_full + 2 * N;    // [2][N], separate P only
-  uint64_t* p_full = s_free + 2 * N;    // [2][N]
-  uint64_t* o_done = p_full + 2 * N;    // [2][N]
-  uint64_t* drain = o_done + 2 * N;     // [2]
+  constexpr int N = L::kParts, SB = L::kBufs;
+  uint64_t* s_full = v_empty + 2 * S;   // [2][SB] S of a part computed
+  uint64_t* s_free = s_full + 2 * SB;   // [2][SB] in registers (separate P only)
+  uint64_t* p_full = s_free + 2 * SB;   // [2][SB] its P written
+  uint64_t* o_done = p_full + 2 * SB;   // [2][SB] and multiplied
+  uint64_t* drain = o_done + 2 * SB;    // [2]
   uint64_t* r_full = drain + 2;         // [R] raw tile loaded
   uint64_t* r_empty = r_full + R;       // [R] raw tile expanded by all its warps
   constexpr int SC = L::kSlots;
@@ -192,7 +196,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + SC);
   volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
   float* scales = reinterpret_cast<float*>(smem + L::kSc);  // [SC][K 64, V 64]
-  static_assert((1 + 7 * S + 2 + 8 * N + 2 * R + 4 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
+  static_assert((1 + 7 * S + 2 + 8 * SB + 2 * R + 4 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q);
@@ -210,11 +214,11 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&drain[x], 1);
-      for (int h = 0; h < N; ++h) {
-        mbar_init(&s_free[x * N + h], 4);
-        mbar_init(&s_full[x * N + h], 1);
-        mbar_init(&p_full[x * N + h], 4);
-        mbar_init(&o_done[x * N + h], 1);
+      for (int h = 0; h < SB; ++h) {
+        mbar_init(&s_free[x * SB + h], 4);
+        mbar_init(&s_full[x * SB + h], 1);
+        mbar_init(&p_full[x * SB + h], 4);
+        mbar_init(&o_done[x * SB + h], 1);
       }
     }
     for (int r = 0; r < R; ++r) {
@@ -236,7 +240,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   // Pages of the range that are outside the pool: rare, so looked for once.
   int hole = 0;
   {
-    const int last = min(k_stop, min(seq.len, lim_of(min(i0 + 2 * tile_tokens, seq.n) - 1)));
+    const int last = min(k_stop, min(seq.len, lim_of(min(i0 + L::kNT * tile_tokens, seq.n) - 1)));
     for (int pos = k_begin + (static_cast<int>(threadIdx.x) << p.page_shift); pos < last;
          pos += L::kThreads << p.page_shift)
       hole |= paged_page(p, b, pos) < 0;
@@ -245,17 +249,17 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   const bool holes = __syncthreads_or(hole);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int page_rows = min(1 << p.page_shift, kPtTile);  // of a tile in one page
-  const int tile_pages = kPtTile / page_rows;
+  const int page_rows = min(1 << p.page_shift, L::kKT);  // of a tile in one page
+  const int tile_pages = L::kKT / page_rows;
 
   // Page of a tile's part, as a coordinate (outside the map: zeros).
   auto page_coord = [&](int j, int part) {
-    const int pos = k_begin + j * kPtTile + part * page_rows;
+    const int pos = k_begin + j * L::kKT + part * page_rows;
     const int page = j < n_iter && pos < seq.len ? paged_page(p, b, pos) : -1;
     return page < 0 ? p.num_pages : page;
   };
   auto slot_coord = [&](int j, int part) {
-    return (k_begin + j * kPtTile + part * page_rows) & ((1 << p.page_shift) - 1);
+    return (k_begin + j * L::kKT + part * page_rows) & ((1 << p.page_shift) - 1);
   };
   auto stage_free = [&](uint64_t* empty, int j) {  // stage of tile j, which held tile j - S
     const uint32_t par = ((j / S) - 1) & 1;
@@ -269,12 +273,12 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   auto load_q = [&]() {
     if (lane == 0) {
       const int rows = tile_tokens * group;
-      mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(2 * L::kBlocks * rows * 128));
+      mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(L::kNT * L::kBlocks * rows * 128));
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < L::kNT; ++x)
 #pragma unroll
         for (int cb = 0; cb < L::kBlocks; ++cb)
-          tma_load_3d(smem + L::kQ + x * L::kTileBytes + cb * L::kBlockBytes, &tm_q, q_full,
+          tma_load_3d(smem + L::kQ + x * L::kQBytes + cb * L::kQBlock, &tm_q, q_full,
                       64 * cb, hk * group, seq.row0 + i0 + x * tile_tokens);
     }
   };
@@ -317,7 +321,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       } else {
         // ---------------------------------------------- V tiles not all see
         for (int j = 0; j < n_iter; ++j) {
-          const int st = j % S, key0 = k_begin + j * kPtTile;
+          const int st = j % S, key0 = k_begin + j * L::kKT;
           // (every phase is waited for: a parity tells only neighbours apart)
           if (!__all_sync(0xffffffffu,
                           mbar_wait_sleep(&v_full[st], (j / S) & 1, err, kDevTimeoutFull)))
@@ -327,9 +331,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           bool found = false;
 #pragma unroll 4
           for (int c = lane; c < L::kTileBytes / 16; c += 32) {
-            // 16-byte chunk c lies in row (c / 8) % 128 of its 64-column block
+            // 16-byte chunk c lies in row (c / 8) % kKT of its 64-column block
             uint4* at = reinterpret_cast<uint4*>(tile) + c;
-            const bool behind = key0 + ((c >> 3) & (kPtTile - 1)) >= seq.len;
+            const bool behind = key0 + ((c >> 3) & (L::kKT - 1)) >= seq.len;
             uint4 x = *at;
             bool hit = h2_clear(x.x);
             hit |= h2_clear(x.y);
@@ -350,8 +354,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       if (warp == 0) {
         // ------------------------------------------------ TMA of raw tiles
         load_q();
-        const int part = lane % tile_pages;
-        const uint32_t dst = smem_u32(smem + L::kR) + part * page_rows * HD;
+        // Lane = (part of the tile, block of 128 columns).
+        const int part = lane % tile_pages, cb = lane / tile_pages;
+        const uint32_t dst = smem_u32(smem + L::kR) + cb * L::kKT * 128 + part * page_rows * L::kRawRow;
         int page = page_coord(0, part), next = page_coord(1, part), issued = 0;
         for (int e = 0; e < total; ++e) {
           const int j = e >> 1;
@@ -360,9 +365,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
             break;
           if (lane == 0) mbar_arrive_expect_tx(&r_full[e % R], L::kRawBytes);
           __syncwarp();
-          if (lane < tile_pages)
-            pt_load_4d(dst + (e % R) * L::kRawBytes, (e & 1) ? &tm_v : &tm_k, &r_full[e % R], 0,
-                       slot_coord(j, part), hk, page);
+          if (cb < HD / L::kRawRow)
+            pt_load_4d(dst + (e % R) * L::kRawBytes, (e & 1) ? &tm_v : &tm_k, &r_full[e % R],
+                       128 * cb, slot_coord(j, part), hk, page);
           issued = e + 1;
           if (e & 1) {
             page = next;
@@ -375,25 +380,26 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           mbar_wait(&r_full[e % R], (e / R) & 1, nullptr, 0);
       } else if (warp >= 12) {
         // ------------------------------------------------- expansion to fp16
-        const int r = (warp - 12) * 32 + lane;  // this lane's row of every tile
+        // This lane's row of every tile (of 64 keys: two lanes, 128 columns each).
+        const int r = ((warp - 12) * 32 + lane) % L::kKT, cb = ((warp - 12) * 32 + lane) / L::kKT;
         // Raw rows of 128 bytes: 16-byte chunk c at c ^ (r & 7); of 64 bytes: at
         // c ^ (r >> 1 & 3). fp16 rows: chunk c of a 64-column block at c ^ (r & 7).
-        const uint32_t rx = HD == 128 ? (r & 7) << 4 : ((r >> 1) & 3) << 4;
+        const uint32_t rx = HD >= 128 ? (r & 7) << 4 : ((r >> 1) & 3) << 4;
         const uint32_t dx = (r & 7) << 4;
         for (int e = 0; e < total; ++e) {
-          const int j = e >> 1, kv = e & 1, st = j % S, key0 = k_begin + j * kPtTile;
+          const int j = e >> 1, kv = e & 1, st = j % S, key0 = k_begin + j * L::kKT;
           if (!__all_sync(0xffffffffu,
                           mbar_wait_sleep(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) ||
               !stage_free(kv ? v_empty : k_empty, j))
             break;
-          const uint8_t* src = smem + L::kR + (e % R) * L::kRawBytes + r * HD;
-          uint8_t* dst = smem + (kv ? L::kV : L::kK) + st * L::kTileBytes + r * 128;
+          const uint8_t* src = smem + L::kR + (e % R) * L::kRawBytes + cb * L::kKT * 128 + r * L::kRawRow;
+          uint8_t* dst = smem + (kv ? L::kV : L::kK) + st * L::kTileBytes + 2 * cb * L::kBlockBytes + r * 128;
           // Not every row sees all of it: NaN codes must not leak (int8 has none).
-          const bool partly = CODE == kCodeE4M3 && kv && key0 + kPtTile > lim_first;
+          const bool partly = CODE == kCodeE4M3 && kv && key0 + L::kKT > lim_first;
           const bool behind = partly && key0 + r >= seq.len;
           bool found = false;
 #pragma unroll
-          for (int c0 = 0; c0 < HD / 16; c0 += 4) {
+          for (int c0 = 0; c0 < L::kRawRow / 16; c0 += 4) {
             uint4 x[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -483,8 +489,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     }
   } else if (warp == 1 || warp == 2) {
     // ------------------------------------------------ MMA issuer of tile x
-    if (lane == 0) {
-      const int x = warp == 1 ? 0 : 1;
+    const int x = warp == 1 ? 0 : 1;
+    if (lane == 0 && x < L::kNT) {
       const int nx = x == 0 ? nA : nB;
       uint64_t* k_free = k_empty + x * S;
       uint64_t* v_free = v_empty + x * S;
@@ -493,85 +499,75 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       const uint64_t dq0 = sdesc_k_sw128(smem_u32(smem + L::kQ));
       const uint64_t dk0 = sdesc_k_sw128(smem_u32(smem + L::kK));
       const uint64_t dv0 = sdesc_mn_sw128(smem_u32(smem + L::kV), L::kBlockBytes);
-      // Part h of a tile: rows 64 h .. of K and of V, columns 64 h .. of S.
-      auto issue_qk = [&](int st, int h) {
-        const uint64_t da = dq0 + static_cast<uint64_t>(x * (L::kTileBytes >> 4));
-        const uint64_t db =
-            dk0 + static_cast<uint64_t>((st * L::kTileBytes + h * L::kKeys * 128) >> 4);
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint64_t off = static_cast<uint64_t>(((k >> 2) * L::kBlockBytes + (k & 3) * 32) >> 4);
-          mma_f16_ss(tmem + x * kPtTile + h * L::kKeys, da + off, db + off, id_qk, k > 0 ? 1u : 0u);
-        }
-        mma_commit(&s_full[x * N + h]);
+      // Part u: rows (u % N) * kKeys .. of K and V of tile u / N, buffer u % SB of S.
+      auto rows_of = [&](int u) {
+        return static_cast<uint64_t>((u / N % S * L::kTileBytes + u % N * L::kKeys * 128) >> 4);
       };
-      auto issue_pv = [&](int st, int h, bool accumulate) {
-        const uint64_t db =
-            dv0 + static_cast<uint64_t>((st * L::kTileBytes + h * L::kKeys * 128) >> 4);
+      auto issue_qk = [&](int u) {
+        const uint64_t da = dq0 + static_cast<uint64_t>(x * (L::kQBytes >> 4));
+        const uint64_t db = dk0 + rows_of(u);
+        const uint32_t d = tmem + x * kPtTile + u % SB * L::kKeys;
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+          mma_f16_ss(d, da + static_cast<uint64_t>(((k >> 2) * L::kQBlock + (k & 3) * 32) >> 4),
+                     db + static_cast<uint64_t>(((k >> 2) * L::kBlockBytes + (k & 3) * 32) >> 4),
+                     id_qk, k > 0 ? 1u : 0u);
+        mma_commit(&s_full[x * SB + u % SB]);
+        if (u % N == N - 1) mma_commit(&k_free[u / N % S]);
+      };
+      auto issue_pv = [&](int u) {
+        const uint64_t db = dv0 + rows_of(u);
+        const uint32_t p = tmem + L::kColP + x * L::kPStride + u % SB * L::kKeys;
 #pragma unroll
         for (int k = 0; k < L::kKeys / 16; ++k)
-          mma_f16_ts(tmem + L::kColO + x * HD,
-                     tmem + L::kColP + x * L::kPStride + h * L::kPPart + 8 * k,
-                     db + static_cast<uint64_t>((k * 2048) >> 4), id_pv,
-                     (accumulate || k > 0) ? 1u : 0u);
-        mma_commit(&o_done[x * N + h]);
+          mma_f16_ts(tmem + L::kColO + x * HD, p + 8 * k, db + static_cast<uint64_t>((k * 2048) >> 4),
+                     id_pv, (u > 0 || k > 0) ? 1u : 0u);
+        mma_commit(&o_done[x * SB + u % SB]);
+        if (u % N == N - 1) mma_commit(&v_free[u / N % S]);
+      };
+      auto wait_k = [&](int u) {  // for the first part of a tile
+        const int j = u / N;
+        return u % N != 0 || mbar_wait(&k_full[j % S], (j / S) & 1, err, kDevTimeoutFull);
       };
       // fp16: V as loaded, where every row sees all of the tile.
-      auto wait_v = [&](int j) {
+      auto wait_v = [&](int u) {
+        const int j = u / N;
+        if (u % N != 0) return true;
         if (!kQuant && j < j_partly)
           return mbar_wait(&v_full[j % S], (j / S) & 1, err, kDevTimeoutFull);
         const int uses = kQuant ? j / S : (j - j_partly) / S;  // of v_ready's stage before
         return mbar_wait(&v_ready[j % S], uses & 1, err, kDevTimeoutFull);
       };
+      const int parts = nx * N;
       bool ok = mbar_wait(q_full, 0, err, kDevTimeoutFull);
-      if (ok && nx > 0) {
-        ok = mbar_wait(&k_full[0], 0, err, kDevTimeoutFull);
-        if (ok) {
-          tc_fence_after();
-#pragma unroll
-          for (int h = 0; h < N; ++h) issue_qk(0, h);
-          mma_commit(&k_free[0]);
-        }
+      for (int u = 0; ok && u < min(SB, parts); ++u) {
+        ok = wait_k(u);
+        if (!ok) break;
+        tc_fence_after();
+        issue_qk(u);
       }
-      for (int j = 0; ok && j < nx; ++j) {
-        const int st = j % S, st1 = (j + 1) % S;
-        const uint32_t par1 = ((j + 1) / S) & 1, jp = j & 1;
+      for (int u = 0; ok && u < parts; ++u) {
+        const int h = u % SB;
+        const uint32_t ph = (u / SB) & 1;
         if constexpr (L::kSepP) {
-#pragma unroll
-          for (int h = 0; h < N; ++h) {
-            if (j + 1 < nx) {  // the next S, as soon as this one is in registers
-              ok = (h > 0 || mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) &&
-                   mbar_wait(&s_free[x * N + h], jp, err, kDevTimeoutOther);
-              if (!ok) break;
-              tc_fence_after();
-              issue_qk(st1, h);
-              if (h == N - 1) mma_commit(&k_free[st1]);
-            }
-            ok = (h > 0 || wait_v(j)) &&
-                 mbar_wait(&p_full[x * N + h], jp, err, kDevTimeoutOther);
+          if (u + SB < parts) {  // the next S, as soon as this one is in registers
+            ok = wait_k(u + SB) && mbar_wait(&s_free[x * SB + h], ph, err, kDevTimeoutOther);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(st, h, j > 0 || h > 0);
-            if (h == N - 1) mma_commit(&v_free[st]);
+            issue_qk(u + SB);
           }
-        } else {
-          if (!wait_v(j)) break;
-#pragma unroll
-          for (int h = 0; h < N; ++h) {
-            ok = mbar_wait(&p_full[x * N + h], jp, err, kDevTimeoutOther);
+        }
+        ok = wait_v(u) && mbar_wait(&p_full[x * SB + h], ph, err, kDevTimeoutOther);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(u);
+        if constexpr (!L::kSepP) {
+          if (u + SB < parts) {
+            // The next S overwrites this part's P: after the product that reads it.
+            ok = wait_k(u + SB) && mbar_wait(&o_done[x * SB + h], ph, err, kDevTimeoutAccum);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(st, h, j > 0 || h > 0);
-            if (h == N - 1) mma_commit(&v_free[st]);
-            if (j + 1 < nx) {
-              // The next S overwrites this part's P: after the product that reads it.
-              ok = (h > 0 || mbar_wait(&k_full[st1], par1, err, kDevTimeoutFull)) &&
-                   mbar_wait(&o_done[x * N + h], jp, err, kDevTimeoutAccum);
-              if (!ok) break;
-              tc_fence_after();
-              issue_qk(st1, h);
-              if (h == N - 1) mma_commit(&k_free[st1]);
-            }
+            issue_qk(u + SB);
           }
         }
       }
@@ -581,6 +577,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   } else {
     // ------------------------------------------------------------ softmax
     const int x = (warp - 4) >> 2;
+    if (x < L::kNT) {
     const int quarter = warp & 3;  // this warp's TMEM lanes [32*quarter, +32)
     const int row = quarter * 32 + lane;
     const int first = i0 + x * tile_tokens;
@@ -599,9 +596,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     bool ok = true;
     auto softmax = [&](auto with_holes) {
     for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
-      const int j = u / N, h = u % N;
+      const int h = u % SB;
       if (!__all_sync(0xffffffffu,
-                      mbar_wait(&s_full[x * N + h], j & 1, err, kDevTimeoutAccum))) {
+                      mbar_wait(&s_full[x * SB + h], (u / SB) & 1, err, kDevTimeoutAccum))) {
         ok = false;
         break;
       }
@@ -616,7 +613,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       if constexpr (L::kSepP) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[x * N + h]);
+        if (lane == 0) mbar_arrive(&s_free[x * SB + h]);
       }
       // 8 bit: scores in the log2 domain from here on.
       [[maybe_unused]] const float* sc = scales + (u % SC) * 128;
@@ -721,13 +718,14 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           }
         }
         if (q == 0) {
-          // P's columns are free once the product of this part of the last tile
-          // is through (P over S: it was before this S was computed); O may be
-          // rescaled once the previous part's is.
-          if (L::kSepP && j > 0)
-            ok = mbar_wait(&o_done[x * N + h], (j - 1) & 1, err, kDevTimeoutAccum);
+          // P's columns are free once the last product that read them is through
+          // (P over S: it was before this S was computed); O may be rescaled once
+          // the previous part's is.
+          if (L::kSepP && u >= SB)
+            ok = mbar_wait(&o_done[x * SB + h], (u / SB - 1) & 1, err, kDevTimeoutAccum);
           if (rescale && u > 0 && ok)
-            ok = mbar_wait(&o_done[x * N + (u - 1) % N], ((u - 1) / N) & 1, err, kDevTimeoutAccum);
+            ok = mbar_wait(&o_done[x * SB + (u - 1) % SB], ((u - 1) / SB) & 1, err,
+                           kDevTimeoutAccum);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
@@ -746,23 +744,23 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
             }
           }
         }
-        if constexpr (kQuant) tmem_st16(t_p + h * L::kPPart + 16 * q, pr);
-        else tmem_st32(t_p + h * L::kPPart + 32 * q, pr);
+        if constexpr (kQuant) tmem_st16(t_p + h * KC + 16 * q, pr);
+        else tmem_st32(t_p + h * KC + 32 * q, pr);
       }
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&p_full[x * N + h]);
+        mbar_arrive(&p_full[x * SB + h]);
         if (kQuant) mbar_arrive(&c_empty[x * SC + u % SC]);
       }
     }
     };
     if (holes) softmax(std::true_type{}); else softmax(std::false_type{});
     if (ok && nx > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x * N + N - 1], (nx - 1) & 1, err,
-                                             kDevTimeoutAccum));
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x * SB + (nx * N - 1) % SB],
+                                             ((nx * N - 1) / SB) & 1, err, kDevTimeoutAccum));
     float la, lb, lc, ld;
     f2_unpack(lsum0, la, lb);
     f2_unpack(lsum1, lc, ld);
@@ -810,9 +808,10 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         __syncwarp();  // the next tmem_ld is warp-collective
       }
       if (fix && owned)
-        pt_add_cleared<CODE, HD>(p, b, hk, max(k_begin, lim_first - kPtTile), min(lim_row, k_stop),
+        pt_add_cleared<CODE, HD>(p, b, hk, max(k_begin, lim_first - L::kKT), min(lim_row, k_stop),
                                  is_split ? a.part_o + at * HD : nullptr, dst);
     }
+    }  // x < kNT
   }
 
   tc_fence_before();
@@ -832,7 +831,7 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   auto kern = paged_tc_kernel<CODE, HD>;
   int st = ensure_smem(reinterpret_cast<const void*>(kern), L::kSmem, done);
   if (st != TFX_OK) return st;
-  const int eb = code_bytes(CODE), page_rows = c->page_size < kPtTile ? c->page_size : kPtTile;
+  const int eb = code_bytes(CODE), page_rows = c->page_size < L::kKT ? c->page_size : L::kKT;
   const uint32_t tile_tokens = static_cast<uint32_t>(kPtTile / a.group);
   CUtensorMap tq, tk, tv;
   const uint64_t qd[3] = {HD, static_cast<uint64_t>(p.kv_heads) * a.group,
@@ -847,7 +846,7 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   const uint64_t ks[3] = {static_cast<uint64_t>(p.token_stride) * eb,
                           static_cast<uint64_t>(p.head_stride) * eb,
                           static_cast<uint64_t>(p.page_stride) * eb};
-  const uint32_t kb[4] = {L::kQuant ? HD : 64, static_cast<uint32_t>(page_rows), 1, 1};
+  const uint32_t kb[4] = {L::kQuant ? L::kRawRow : 64, static_cast<uint32_t>(page_rows), 1, 1};
   const CUtensorMapDataType dt =
       L::kQuant ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUtensorMapSwizzle sw =
@@ -855,7 +854,7 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   if (st == TFX_OK) st = make_tmap(&tk, p.k, dt, 4, kd, ks, kb, sw);
   if (st == TFX_OK) st = make_tmap(&tv, p.v, dt, 4, kd, ks, kb, sw);
   if (st != TFX_OK) return st;
-  const int64_t blocks = (tokens + 2 * tile_tokens - 1) / (2 * tile_tokens);
+  const int64_t blocks = (tokens + L::kNT * tile_tokens - 1) / (L::kNT * tile_tokens);
   if (blocks * a.splits > 65535)
     return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: max_query_len is too long for the grid");
   launch_pdl(kern, dim3(p.kv_heads, p.batch, static_cast<unsigned>(blocks * a.splits)),
@@ -869,8 +868,11 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
 template <int CODE>
 int launch_paged_tc(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, int64_t tokens,
                     cudaStream_t stream) {
-  return c->head_dim == 64 ? launch_tc_hd<CODE, 64>(c, p, a, tokens, stream)
-                           : launch_tc_hd<CODE, 128>(c, p, a, tokens, stream);
+  switch (c->head_dim) {
+    case 64: return launch_tc_hd<CODE, 64>(c, p, a, tokens, stream);
+    case 128: return launch_tc_hd<CODE, 128>(c, p, a, tokens, stream);
+    default: return launch_tc_hd<CODE, 256>(c, p, a, tokens, stream);
+  }
 }
 
 }  // namespace tfx

@@ -193,34 +193,41 @@ def _check(pool, got, q, group, causal=True, scale=None, absent=()):
 DECODE = [(1, 1), (1, 700), (1, 16), (0, 40), (1, 257), (1, 513), (1, 1300)]
 DRAFT = [(4, 300), (1, 64), (7, 7), (3, 1025), (0, 0), (2, 31)]
 CHUNK = [(130, 400), (1, 77), (64, 64), (257, 300), (31, 1000)]
+# (10 heads of CHUNK are enough work for the tcgen05 kernel, 2 are not)
 
 
 @pytest.mark.parametrize("dtype,hd", [(F16, hd) for hd in (8, 16, 32, 64, 128, 256)] +
                          [(t, hd) for t in (I8, E4) for hd in (16, 32, 64, 128, 256)],
                          ids=lambda v: NAMES.get(v, str(v)) if not isinstance(v, int) else str(v))
-@pytest.mark.parametrize("what", ["decode", "draft", "chunk"])
+@pytest.mark.parametrize("what", ["decode", "draft", "chunk", "prompt"])
 def test_attention(pkg, dev, dtype, hd, what):
-    lens = {"decode": DECODE, "draft": DRAFT, "chunk": CHUNK}[what]
+    lens = {"decode": DECODE, "draft": DRAFT, "chunk": CHUNK, "prompt": CHUNK}[what]
     heads, group, page, order = {"decode": (3, 1, 16, "head"), "draft": (2, 4, 64, "token"),
-                                 "chunk": (2, 2, 128, "head")}[what]
+                                 "chunk": (2, 2, 128, "head"), "prompt": (10, 2, 32, "token")}[what]
     pool = pr.Pool(lens, page, heads, hd, dtype, hd, order)
     q, got = _attend(pkg, dev, pool, group)
     _check(pool, got, q, group)
 
 
 @pytest.mark.parametrize("dtype", [F16, I8, E4], ids=["fp16", "int8", "e4m3"])
-@pytest.mark.parametrize("hd,group,page,order,lens", [
-    (64, 3, 32, "gap", [(43, 43), (1, 90), (50, 177)]),       # groups that do not divide a tile
-    (64, 5, 16, "head", [(7, 400), (3, 3)]),
-    (128, 7, 256, "head", [(40, 300), (1, 256), (2, 257)]),
-    (64, 16, 64, "head", [(1, 2000)]),
-    (128, 33, 64, "head", [(5, 70)]),                          # more heads in a group than rows of a block
-    (64, 130, 64, "head", [(2, 70), (1, 5)]),
-    (128, 1, 128, "token", [(300, 1111)]),
-    (256, 2, 16, "head", [(33, 333)]),
+@pytest.mark.parametrize("hd,heads,group,page,order,lens", [
+    (64, 2, 3, 32, "gap", [(43, 43), (1, 90), (50, 177)]),     # groups that do not divide a tile
+    (64, 2, 5, 16, "head", [(7, 400), (3, 3)]),
+    (64, 2, 16, 64, "head", [(1, 2000)]),
+    (128, 2, 33, 64, "head", [(5, 70)]),                        # more heads in a group than rows of a block
+    (64, 1, 130, 64, "head", [(2, 70), (1, 5)]),
+    # the tcgen05 kernel
+    (64, 16, 3, 32, "gap", [(43, 1043), (1, 90), (50, 1177), (90, 90)]),
+    (64, 20, 5, 16, "head", [(37, 1400), (3, 3)]),
+    (128, 12, 7, 256, "head", [(40, 1300), (1, 256), (22, 1257)]),
+    (128, 24, 33, 64, "gap", [(9, 1070)]),
+    (128, 32, 1, 128, "token", [(300, 1111)]),
+    (256, 12, 2, 16, "head", [(133, 1333), (65, 65)]),
+    (256, 10, 128, 64, "gap", [(2, 900), (1, 300)]),
+    (256, 12, 3, 128, "token", [(90, 700), (30, 500)]),
 ])
-def test_attention_heads_and_orders(pkg, dev, dtype, hd, group, page, order, lens):
-    pool = pr.Pool(lens, page, 2, hd, dtype, group, order)
+def test_attention_heads_and_orders(pkg, dev, dtype, hd, heads, group, page, order, lens):
+    pool = pr.Pool(lens, page, heads, hd, dtype, group, order)
     q, got = _attend(pkg, dev, pool, group)
     _check(pool, got, q, group)
     # without the optional bounds: more splits and blocks than needed
@@ -229,9 +236,9 @@ def test_attention_heads_and_orders(pkg, dev, dtype, hd, group, page, order, len
 
 
 @pytest.mark.parametrize("dtype", [F16, I8], ids=["fp16", "int8"])
-@pytest.mark.parametrize("hd", [32, 64, 128])
-def test_attention_not_causal_and_scaled(pkg, dev, dtype, hd):
-    pool = pr.Pool(CHUNK, 32, 2, hd, dtype, 3)
+@pytest.mark.parametrize("hd,heads", [(32, 2), (64, 2), (64, 10), (128, 10), (256, 10)])
+def test_attention_not_causal_and_scaled(pkg, dev, dtype, hd, heads):
+    pool = pr.Pool(CHUNK, 32, heads, hd, dtype, 3)
     q, got = _attend(pkg, dev, pool, 1, causal=False)
     _check(pool, got, q, 1, causal=False)
     q, got = _attend(pkg, dev, pool, 1, scale=0.3)
@@ -239,13 +246,14 @@ def test_attention_not_causal_and_scaled(pkg, dev, dtype, hd):
 
 
 @pytest.mark.parametrize("dtype", [F16, I8, E4], ids=["fp16", "int8", "e4m3"])
-@pytest.mark.parametrize("hd", [32, 64, 128])
-@pytest.mark.parametrize("lens", [DRAFT, CHUNK], ids=["draft", "chunk"])
-def test_attention_hides_what_a_row_does_not_see(pkg, dev, dtype, hd, lens):
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("lens,heads", [(DRAFT, 2), (CHUNK, 2), (CHUNK, 10)],
+                         ids=["draft", "chunk", "prompt"])
+def test_attention_hides_what_a_row_does_not_see(pkg, dev, dtype, hd, lens, heads):
     """NaN, infinities and huge values at positions that a row does not see (later
     tokens; slots behind the sequence are NaN in every test here) leave it as
     it is; the rows that see them get them."""
-    pool = pr.Pool(lens, 16, 2, hd, dtype, 11)
+    pool = pr.Pool(lens, 16, heads, hd, dtype, 11)
     n, kv = lens[0]
     pool.data[0][1][kv - 2, 0, 1] = float("inf")     # value
     pool.data[0][1][kv - 1, 1, 5] = float("nan")
@@ -260,20 +268,25 @@ def test_attention_hides_what_a_row_does_not_see(pkg, dev, dtype, hd, lens):
     err = (got - ref).abs()
     assert bool((err <= tol)[rows].all()), float((err / tol)[rows].max())
     # row n - 2 sees the infinity of head 0 (8 bits: its whole scale is NaN), not the last token
-    assert not torch.isfinite(got[n - 2].view(4, hd)[:2, 1]).any()
+    row = got[n - 2].view(2 * heads, hd)
+    assert not torch.isfinite(row[:2, 1]).any() and torch.isfinite(row[2:]).all()
     if dtype == F16:
-        bad = ~torch.isfinite(got[n - 2].view(4, hd))
-        assert int(bad.sum()) == 2 and bool((got[n - 2].view(4, hd)[:2, 1] == float("inf")).all())
-    assert torch.isfinite(got[n - 2].view(4, hd)[2:]).all()
+        assert int((~torch.isfinite(row)).sum()) == 2 and bool((row[:2, 1] == float("inf")).all())
+    last = got[n - 1].view(2 * heads, hd)  # a NaN key of head 0, a NaN value of head 1
+    assert not torch.isfinite(last[:2]).any() and not torch.isfinite(last[2:4, 5]).any()
+    assert torch.isfinite(last[4:]).all()
 
 
 @pytest.mark.parametrize("dtype", [F16, I8, E4], ids=["fp16", "int8", "e4m3"])
-@pytest.mark.parametrize("hd", [32, 64, 128])
-def test_attention_pages_outside_the_pool(pkg, dev, dtype, hd):
+@pytest.mark.parametrize("hd,heads,lens", [
+    (32, 2, [(20, 300), (3, 40), (2, 10), (90, 200)]), (64, 2, [(20, 300), (3, 40), (2, 10), (90, 200)]),
+    (64, 12, [(20, 3000), (3, 40), (2, 10), (200, 2000)]),
+    (128, 12, [(20, 2000), (3, 40), (2, 10), (200, 1500)]),
+    (256, 8, [(20, 2000), (3, 40), (2, 10), (100, 1500)])])
+def test_attention_pages_outside_the_pool(pkg, dev, dtype, hd, heads, lens):
     """Their keys are masked; a row that sees no key at all is zero; rows behind the
     last sequence are left as they were."""
-    lens = [(20, 300), (3, 40), (2, 10), (90, 200)]
-    pool = pr.Pool(lens, 16, 2, hd, dtype, 4)
+    pool = pr.Pool(lens, 16, heads, hd, dtype, 4)
     cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled()))
     table = pool.table.clone()
     absent = [(0, 0), (0, 7), (0, 18), (2, 0), (3, 9), (3, 8)]
@@ -281,8 +294,8 @@ def test_attention_pages_outside_the_pool(pkg, dev, dtype, hd):
         table[b, page] = [-1, pool.pages, 2 ** 31 - 1, -2 ** 31][i % 4]
     rows = pool.tokens + 3
     batch = pkg.PagedBatch(table.to(dev), pool.start.to(dev), pool.kv.to(dev), rows, **_hints(pool))
-    q = torch.randn(rows, 4, hd, generator=pool.q_gen).half()
-    out = torch.full((rows, 4 * hd), -3.0, dtype=F16, device=dev)
+    q = torch.randn(rows, 2 * heads, hd, generator=pool.q_gen).half()
+    out = torch.full((rows, 2 * heads * hd), -3.0, dtype=F16, device=dev)
     got = pkg.ops.paged_attention(q.to(dev), cache, batch, out=out)
     assert got is out
     got = got.double().cpu()
