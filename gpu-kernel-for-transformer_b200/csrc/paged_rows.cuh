@@ -131,9 +131,12 @@ struct RowsCfg {
   static constexpr int kPitch = ((kHDP * code_bytes(CODE) / 16) | 1) * 16;
   static constexpr int kQPitch = (kHDP + 8) * 2;
   // Keys of a warp's tile: about 2 KB of K (small tiles keep more warps on an
-  // SM), at most 64, and 128 scores to a column of lanes (registers).
+  // SM), 4 KB with more than 8 rows (registers bound the warps there, and a tile's
+  // fixed cost is larger: 46 against 40 us for drafts of 2 to 8 tokens in groups of
+  // 4, int8, 128); at most 64, and 128 scores to a column of lanes.
   static constexpr int kMost = 128 / NT < 64 ? 128 / NT : 64;
-  static constexpr int kWant = 2048 / kRowBytes < 16 ? 16 : 2048 / kRowBytes;
+  static constexpr int kWantBytes = NT >= 2 ? 4096 : 2048;
+  static constexpr int kWant = kWantBytes / kRowBytes < 16 ? 16 : kWantBytes / kRowBytes;
   static constexpr int kKT = kWant < kMost ? kWant : kMost;
   static constexpr int NS = 2;
   static constexpr int kTileBytes = kKT * kPitch;

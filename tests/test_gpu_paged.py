@@ -218,13 +218,13 @@ def test_attention(pkg, dev, dtype, hd, what):
     (64, 1, 130, 64, "head", [(2, 70), (1, 5)]),
     # the tcgen05 kernel
     (64, 16, 3, 32, "gap", [(43, 1043), (1, 90), (50, 1177), (90, 90)]),
-    (64, 20, 5, 16, "head", [(37, 1400), (3, 3)]),
-    (128, 12, 7, 256, "head", [(40, 1300), (1, 256), (22, 1257)]),
-    (128, 24, 33, 64, "gap", [(9, 1070)]),
-    (128, 32, 1, 128, "token", [(300, 1111)]),
+    (64, 32, 5, 16, "head", [(37, 1400), (3, 3)]),
+    (128, 16, 7, 256, "head", [(40, 1300), (1, 256), (22, 1257)]),
+    (128, 40, 33, 64, "gap", [(9, 1070)]),
+    (128, 48, 1, 128, "token", [(300, 1111)]),
     (256, 12, 2, 16, "head", [(133, 1333), (65, 65)]),
-    (256, 10, 128, 64, "gap", [(2, 900), (1, 300)]),
-    (256, 12, 3, 128, "token", [(90, 700), (30, 500)]),
+    (256, 16, 128, 64, "gap", [(2, 900), (1, 300)]),
+    (256, 16, 3, 128, "token", [(90, 700), (30, 500)]),
 ])
 def test_attention_heads_and_orders(pkg, dev, dtype, hd, heads, group, page, order, lens):
     pool = pr.Pool(lens, page, heads, hd, dtype, group, order)
