@@ -350,28 +350,35 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         }
       }
     } else {
-      const int total = 2 * n_iter;  // raw tiles: K and V in turn
+      // Raw tiles: K and V in turn, K one tile ahead (K0 K1 V0 K2 V1 .. V), so that
+      // the next scores do not wait behind a V that waits for its stage.
+      const int total = 2 * n_iter;
+      auto is_v = [&](int e) { return e == total - 1 || (e > 0 && !(e & 1)); };
+      auto tile_of = [&](int e) { return is_v(e) ? (e - 1) / 2 : (e + 1) / 2; };
       if (warp == 0) {
         // ------------------------------------------------ TMA of raw tiles
         load_q();
         // Lane = (part of the tile, block of 128 columns).
         const int part = lane % tile_pages, cb = lane / tile_pages;
         const uint32_t dst = smem_u32(smem + L::kR) + cb * L::kKT * 128 + part * page_rows * L::kRawRow;
-        int page = page_coord(0, part), next = page_coord(1, part), issued = 0;
+        int v_page = page_coord(0, part), k_page = page_coord(1, part), issued = 0;
+        int next = page_coord(2, part);
         for (int e = 0; e < total; ++e) {
-          const int j = e >> 1;
+          const int j = tile_of(e);
+          const bool v = is_v(e);
           if (e >= R && !__all_sync(0xffffffffu, mbar_wait_sleep(&r_empty[e % R], ((e / R) - 1) & 1, err,
                                                            kDevTimeoutEmpty)))
             break;
           if (lane == 0) mbar_arrive_expect_tx(&r_full[e % R], L::kRawBytes);
           __syncwarp();
           if (cb < HD / L::kRawRow)
-            pt_load_4d(dst + (e % R) * L::kRawBytes, (e & 1) ? &tm_v : &tm_k, &r_full[e % R],
-                       128 * cb, slot_coord(j, part), hk, page);
+            pt_load_4d(dst + (e % R) * L::kRawBytes, v ? &tm_v : &tm_k, &r_full[e % R],
+                       128 * cb, slot_coord(j, part), hk, v || e == 0 ? v_page : k_page);
           issued = e + 1;
-          if (e & 1) {
-            page = next;
-            next = page_coord(j + 2, part);
+          if (v) {
+            v_page = k_page;
+            k_page = next;
+            next = page_coord(j + 3, part);
           }
         }
         // Our own copies land before the CTA may exit.
@@ -387,7 +394,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         const uint32_t rx = HD >= 128 ? (r & 7) << 4 : ((r >> 1) & 3) << 4;
         const uint32_t dx = (r & 7) << 4;
         for (int e = 0; e < total; ++e) {
-          const int j = e >> 1, kv = e & 1, st = j % S, key0 = k_begin + j * L::kKT;
+          const int j = tile_of(e), st = j % S, key0 = k_begin + j * L::kKT;
+          const bool kv = is_v(e);
           if (!__all_sync(0xffffffffu,
                           mbar_wait_sleep(&r_full[e % R], (e / R) & 1, err, kDevTimeoutFull)) ||
               !stage_free(kv ? v_empty : k_empty, j))
