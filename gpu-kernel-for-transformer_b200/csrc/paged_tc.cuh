@@ -599,10 +599,35 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     const int lim_row = lim_of(min(tok, seq.n - 1));
     const int lim_tile = lim_of(min(first, seq.n - 1));  // smallest of the tile
     float m_ref = -INFINITY;  // -inf: no key seen yet
-    uint64_t lsum0 = 0, lsum1 = 0;
+    float l = 0.f;
     float unit = 1.f;  // 8 bit: U
     bool ok = true;
+    auto wait_o = [&](int u) {  // the product of part u is through
+      return mbar_wait(&o_done[x * SB + u % SB], (u / SB) & 1, err, kDevTimeoutAccum);
+    };
+    auto rescale_o = [&](float f) {  // this lane's row of O
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(t_o + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st16(t_o + c, o);
+      }
+    };
+    constexpr int KC = L::kKeys;
+    // Which groups of 16 keys of a part exist (page in the pool): bit i.
+    auto there_of = [&](int key0) {
+      uint32_t there = 0;
+#pragma unroll 1
+      for (int i = 0; i < KC / 16; ++i)
+        there |= static_cast<uint32_t>(key0 + 16 * i < seq.len &&
+                                       paged_page(p, b, key0 + 16 * i) >= 0) << i;
+      return there;
+    };
     auto softmax = [&](auto with_holes) {
+    uint64_t lsum0 = 0, lsum1 = 0;
     for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
       const int h = u % SB;
       if (!__all_sync(0xffffffffu,
@@ -611,7 +636,6 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         break;
       }
       tc_fence_after();
-      constexpr int KC = L::kKeys;
       const int key0 = k_begin + u * KC;
       uint32_t s[KC];
 #pragma unroll
@@ -623,30 +647,6 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x * SB + h]);
       }
-      // 8 bit: scores in the log2 domain from here on.
-      [[maybe_unused]] const float* sc = scales + (u % SC) * 128;
-      float ratio = 1.f;
-      if constexpr (kQuant) {
-        if (!__all_sync(0xffffffffu,
-                        mbar_wait(&c_full[u % SC], (u / SC) & 1, err, kDevTimeoutOther))) {
-          ok = false;
-          break;
-        }
-        const float2 un = units[u % SC];
-        ratio = un.x;
-        unit = un.y;
-#pragma unroll
-        for (int c = 0; c < KC; c += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(sc + c);
-          float y[4];
-          f2_unpack(f2_mul(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])),
-                           f2_pack(f.x, f.y)), y[0], y[1]);
-          f2_unpack(f2_mul(f2_pack(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])),
-                           f2_pack(f.z, f.w)), y[2], y[3]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[c + i] = __float_as_uint(y[i]);
-        }
-      }
       if (key0 + KC > lim_tile) {  // warp-uniform
         const int c0 = lim_row - key0;
 #pragma unroll
@@ -654,11 +654,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           if (c >= c0) s[c] = 0xff800000u;  // -inf
       }
       if constexpr (decltype(with_holes)::value) {
-        uint32_t there = 0;  // bit i: keys 16 i .. 16 i + 15 exist
-#pragma unroll 1
-        for (int i = 0; i < KC / 16; ++i)
-          there |= static_cast<uint32_t>(key0 + 16 * i < seq.len &&
-                                         paged_page(p, b, key0 + 16 * i) >= 0) << i;
+        const uint32_t there = there_of(key0);
         if (there != (1u << (KC / 16)) - 1u) {
 #pragma unroll
           for (int c = 0; c < KC; ++c)
@@ -674,9 +670,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           mm[i] = fmax3(mm[i], __uint_as_float(s[c + i]), __uint_as_float(s[c + 8 + i]));
-      const float mx = fmaxf(fmax3(mm[0], mm[1], mm[2]),
-                             fmax3(fmax3(mm[3], mm[4], mm[5]), mm[6], mm[7]));
-      const float m_new = kQuant ? mx : mx * a.scale_log2;
+      const float m_new = fmaxf(fmax3(mm[0], mm[1], mm[2]),
+                                fmax3(fmax3(mm[3], mm[4], mm[5]), mm[6], mm[7])) * a.scale_log2;
       bool rescale = false;
       float f = 1.f;
       if (u == 0) {
@@ -690,89 +685,230 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         lsum1 = f2_fma(lsum1, f2v, 0);
         rescale = true;
       }
-      if (kQuant && u > 0 && ratio != 1.f) rescale = true;  // the same for every row
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
       const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2);
       const uint64_t negm2 = f2_pack(-m_use, -m_use);
-      // P goes to TMEM 64 keys at a time; 8 bit: 32 (registers).
-      constexpr int PC = kQuant ? 32 : 64;
 #pragma unroll
-      for (int q = 0; q < KC / PC; ++q) {
-        uint32_t pr[PC / 2];
+      for (int q = 0; q < KC / 64; ++q) {  // P goes to TMEM 64 keys at a time
+        uint32_t pr[32];
 #pragma unroll
-        for (int i2 = 0; i2 < PC / 2; i2 += 2) {
-          [[maybe_unused]] float4 w;  // 8 bit: the values' scales
-          if constexpr (kQuant) w = *reinterpret_cast<const float4*>(sc + 64 + PC * q + 2 * i2);
-#pragma unroll
-          for (int i = i2; i < i2 + 2; ++i) {
-            const int c = PC * q + 2 * i;
-            const uint64_t x = f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-            const uint64_t arg = kQuant ? f2_add(x, negm2) : f2_fma(x, c2, negm2);
-            uint64_t e;
-            if ((i & 7) < (kQuant ? kPtPolyQuant : kPtPoly)) {
-              uint64_t mant;
-              e = exp2_poly_nan_f2(arg, &mant);
-              lsum0 = f2_fma(mant, 0, lsum0);  // a NaN score makes the sum NaN
-            } else {
-              float a0, a1;
-              f2_unpack(arg, a0, a1);
-              e = f2_pack(fast_exp2(a0), fast_exp2(a1));
-            }
-            if (i & 1) lsum1 = f2_add(lsum1, e); else lsum0 = f2_add(lsum0, e);
-            if constexpr (kQuant) e = f2_mul(e, i == i2 ? f2_pack(w.x, w.y) : f2_pack(w.z, w.w));
-            float e0, e1;
-            f2_unpack(e, e0, e1);
-            pr[i] = pack_half2(e0, e1);
+        for (int i = 0; i < 32; ++i) {
+          const int c = 64 * q + 2 * i;
+          const uint64_t arg =
+              f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), c2, negm2);
+          uint64_t e;
+          if ((i & 7) < kPtPoly) {
+            uint64_t mant;
+            e = exp2_poly_nan_f2(arg, &mant);
+            lsum0 = f2_fma(mant, 0, lsum0);  // a NaN score makes the sum NaN
+          } else {
+            float a0, a1;
+            f2_unpack(arg, a0, a1);
+            e = f2_pack(fast_exp2(a0), fast_exp2(a1));
           }
+          if (i & 1) lsum1 = f2_add(lsum1, e); else lsum0 = f2_add(lsum0, e);
+          float e0, e1;
+          f2_unpack(e, e0, e1);
+          pr[i] = pack_half2(e0, e1);
         }
         if (q == 0) {
           // P's columns are free once the last product that read them is through
           // (P over S: it was before this S was computed); O may be rescaled once
           // the previous part's is.
-          if (L::kSepP && u >= SB)
-            ok = mbar_wait(&o_done[x * SB + h], (u / SB - 1) & 1, err, kDevTimeoutAccum);
-          if (rescale && u > 0 && ok)
-            ok = mbar_wait(&o_done[x * SB + (u - 1) % SB], ((u - 1) / SB) & 1, err,
-                           kDevTimeoutAccum);
+          if (L::kSepP && u >= SB) ok = wait_o(u - SB);
+          if (rescale && ok) ok = wait_o(u - 1);
           if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          if (rescale) {
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-              uint32_t o[16];
-              tmem_ld16(t_o + c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                o[i] = __float_as_uint(__uint_as_float(o[i]) * (f * ratio));
-              tmem_st16(t_o + c, o);
-            }
-          }
+          if (rescale) rescale_o(f);
         }
-        if constexpr (kQuant) tmem_st16(t_p + h * KC + 16 * q, pr);
-        else tmem_st32(t_p + h * KC + 32 * q, pr);
+        tmem_st32(t_p + h * KC + 32 * q, pr);
       }
       if (!ok) break;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&p_full[x * SB + h]);
-        if (kQuant) mbar_arrive(&c_empty[x * SC + u % SC]);
-      }
+      if (lane == 0) mbar_arrive(&p_full[x * SB + h]);
     }
-    };
-    if (holes) softmax(std::true_type{}); else softmax(std::false_type{});
-    if (ok && nx > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x * SB + (nx * N - 1) % SB],
-                                             ((nx * N - 1) / SB) & 1, err, kDevTimeoutAccum));
     float la, lb, lc, ld;
     f2_unpack(lsum0, la, lb);
     f2_unpack(lsum1, lc, ld);
-    float l = (la + lb) + (lc + ld);
+    l = (la + lb) + (lc + ld);
+    };
+    // 8 bit: every score and weight meets a scale from shared memory. A lane holds
+    // 16 keys of 4 rows (lane / 4 + 8 k: the layout of matrix fragments) and so reads
+    // 16 + 16 scales a part; with 64 keys of one row it read 64 + 64, and that was
+    // what bounded the kernel (128 bytes a clock: 1024 of a part's 3100 clocks).
+    auto softmax_quant = [&](auto with_holes) {
+    static_assert(!kQuant || KC == 64, "one fragment load per 16 rows");
+    const int quad = lane & 3, sub = lane >> 2;
+    float mr[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    uint64_t ls[4] = {0, 0, 0, 0};
+    auto of_row = [&](const float (&v)[4]) {  // from this layout to a lane per row
+      float y = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float z = __shfl_sync(0xffffffffu, v[k], (lane & 7) * 4);
+        if (lane >> 3 == k) y = z;
+      }
+      return y;
+    };
+    for (int u = 0; u < nx * N; ++u) {  // parts of the tiles
+      const int h = u % SB, slot = u % SC;
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(&s_full[x * SB + h], (u / SB) & 1, err, kDevTimeoutAccum) &&
+                          mbar_wait(&c_full[slot], (u / SC) & 1, err, kDevTimeoutOther))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int key0 = k_begin + u * KC;
+      uint32_t s[2][32];  // [k / 2][4 c + 2 (k % 2)]: keys 8 c + 2 quad, + 1 of row k
+      tmem_ld_16x64(t_s + h * KC, s[0]);
+      tmem_ld_16x64(t_s + (16u << 16) + h * KC, s[1]);
+      tmem_ld_wait();
+      const float2 un = units[slot];
+      const float ratio = un.x;
+      unit = un.y;
+      const float2* sk = reinterpret_cast<const float2*>(scales + slot * 128) + quad;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {  // scores in the log2 domain from here on
+        const float2 f = sk[4 * c];
+        const uint64_t f2 = f2_pack(f.x, f.y);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t* at = &s[k >> 1][4 * c + 2 * (k & 1)];
+          float y0, y1;
+          f2_unpack(f2_mul(f2_pack(__uint_as_float(at[0]), __uint_as_float(at[1])), f2), y0, y1);
+          at[0] = __float_as_uint(y0);
+          at[1] = __float_as_uint(y1);
+        }
+      }
+      if (key0 + KC > lim_tile) {  // warp-uniform
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = first + (quarter * 32 + sub + 8 * k) / group;
+          const int c0 = lim_of(min(i, seq.n - 1)) - key0 - 2 * quad;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            if (8 * c >= c0) s[k >> 1][4 * c + 2 * (k & 1)] = 0xff800000u;  // -inf
+            if (8 * c + 1 >= c0) s[k >> 1][4 * c + 2 * (k & 1) + 1] = 0xff800000u;
+          }
+        }
+      }
+      if constexpr (decltype(with_holes)::value) {
+        const uint32_t there = there_of(key0);
+        if (there != (1u << (KC / 16)) - 1u) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((there >> (i >> 3)) & 1u)) s[0][i] = s[1][i] = 0xff800000u;
+        }
+      }
+      float mn[4];
+      bool more = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t* at = &s[k >> 1][2 * (k & 1)];
+        float z = fmaxf(__uint_as_float(at[0]), __uint_as_float(at[1]));
+#pragma unroll
+        for (int c = 1; c < 8; ++c)
+          z = fmax3(z, __uint_as_float(at[4 * c]), __uint_as_float(at[4 * c + 1]));
+        mn[k] = z;
+      }
+#pragma unroll
+      for (int m = 1; m <= 2; m *= 2)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mn[k] = fmaxf(mn[k], __shfl_xor_sync(0xffffffffu, mn[k], m));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) more |= mn[k] > mr[k] + kPtRescale;
+      bool rescale = u > 0 && ratio != 1.f;  // the same for every row
+      float f = 1.f;                         // of this lane's row of O
+      if (u == 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mr[k] = mn[k];
+      } else if (__any_sync(0xffffffffu, more)) {
+        float fk[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float up = fmaxf(mr[k], mn[k]);
+          fk[k] = mr[k] == up ? 1.f : fast_exp2(mr[k] - up);  // mr -inf: 0
+          mr[k] = up;
+          ls[k] = f2_fma(ls[k], f2_pack(fk[k], fk[k]), 0);
+        }
+        f = of_row(fk);
+        rescale = true;
+      }
+      uint64_t neg[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float z = mr[k] == -INFINITY ? 0.f : -mr[k];
+        neg[k] = f2_pack(z, z);
+      }
+      uint32_t pr[2][16];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float2 w = sk[32 + 4 * c];  // the values' scales over U
+        const uint64_t w2 = f2_pack(w.x, w.y);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t* at = &s[k >> 1][4 * c + 2 * (k & 1)];
+          const uint64_t arg =
+              f2_add(f2_pack(__uint_as_float(at[0]), __uint_as_float(at[1])), neg[k]);
+          uint64_t e;
+          if (((4 * c + k) & 7) < kPtPolyQuant) {
+            uint64_t mant;
+            e = exp2_poly_nan_f2(arg, &mant);
+            ls[k] = f2_fma(mant, 0, ls[k]);  // a NaN score makes the sum NaN
+          } else {
+            float a0, a1;
+            f2_unpack(arg, a0, a1);
+            e = f2_pack(fast_exp2(a0), fast_exp2(a1));
+          }
+          ls[k] = f2_add(ls[k], e);
+          float e0, e1;
+          f2_unpack(f2_mul(e, w2), e0, e1);
+          pr[k >> 1][2 * c + (k & 1)] = pack_half2(e0, e1);
+        }
+      }
+      // (P lies over S: the product that read these columns was before this S.)
+      if (rescale) {
+        ok = wait_o(u - 1);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        rescale_o(f * ratio);
+      }
+      tmem_st_16x32(t_p + h * KC, pr[0]);
+      tmem_st_16x32(t_p + (16u << 16) + h * KC, pr[1]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&p_full[x * SB + h]);
+        mbar_arrive(&c_empty[x * SC + slot]);
+      }
+    }
+    float lk[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float y0, y1;
+      f2_unpack(ls[k], y0, y1);
+      lk[k] = y0 + y1;
+      lk[k] += __shfl_xor_sync(0xffffffffu, lk[k], 1);
+      lk[k] += __shfl_xor_sync(0xffffffffu, lk[k], 2);
+    }
+    l = of_row(lk);
+    m_ref = of_row(mr);
+    };
+    auto run = [&](auto with_holes) {
+      if constexpr (kQuant) softmax_quant(with_holes); else softmax(with_holes);
+    };
+    if (holes) run(std::true_type{}); else run(std::false_type{});
+    if (ok && nx > 0) ok = __all_sync(0xffffffffu, wait_o(nx * N - 1));
     if (m_ref == -INFINITY && l == l) l = 0.f;                  // no key seen
     if (m_ref == INFINITY) l = __uint_as_float(0x7fc00000u);  // a score of +inf
     if (ok) {
