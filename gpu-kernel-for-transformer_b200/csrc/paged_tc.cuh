@@ -54,9 +54,11 @@ namespace {
 constexpr int kPtConvert = 4;  // 8 bit: warps that expand
 constexpr int kPtTile = 128;
 constexpr float kPtRescale = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8
-// Of 8 pairs of exponentials, so many on the FMA pipe (8 bit: it has the scales
-// to multiply as well).
-constexpr int kPtPoly = 2, kPtPolyQuant = 1;
+// fp16: of 8 pairs of exponentials, so many on the FMA pipe. 8 bit: none; its warps
+// have the scales to multiply as well, and are bound by the instructions that they
+// issue (16k int8 sequence, head_dim 64, not causal: 2318, 2447 and 2436 us with 0, 1
+// and 2 of 8).
+constexpr int kPtPoly = 2;
 constexpr uint32_t kPtCols = 512;
 
 template <int CODE, int HD>
@@ -856,18 +858,10 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           const uint32_t* at = &s[k >> 1][4 * c + 2 * (k & 1)];
           const uint64_t arg =
               f2_add(f2_pack(__uint_as_float(at[0]), __uint_as_float(at[1])), neg[k]);
-          uint64_t e;
-          if (((4 * c + k) & 7) < kPtPolyQuant) {
-            uint64_t mant;
-            e = exp2_poly_nan_f2(arg, &mant);
-            ls[k] = f2_fma(mant, 0, ls[k]);  // a NaN score makes the sum NaN
-          } else {
-            float a0, a1;
-            f2_unpack(arg, a0, a1);
-            e = f2_pack(fast_exp2(a0), fast_exp2(a1));
-          }
+          float a0, a1, e0, e1;
+          f2_unpack(arg, a0, a1);
+          const uint64_t e = f2_pack(fast_exp2(a0), fast_exp2(a1));
           ls[k] = f2_add(ls[k], e);
-          float e0, e1;
           f2_unpack(f2_mul(e, w2), e0, e1);
           pr[k >> 1][2 * c + (k & 1)] = pack_half2(e0, e1);
         }
