@@ -195,7 +195,7 @@ __device__ __forceinline__ int paged_split_end(const PagedAttn& a, const PagedSe
 int paged_rows_block(int head_dim, int64_t rows);
 template <int CODE>
 int launch_paged_rows(const Paged& p, const PagedAttn& a, int head_dim, int block_rows,
-                      int64_t rows, cudaStream_t stream);
+                      bool mixed, int64_t rows, cudaStream_t stream);
 // tokens: max_query_len.
 template <int CODE>
 int launch_paged_tc(const tfx_paged_cache* cache, const Paged& p, const PagedAttn& a,

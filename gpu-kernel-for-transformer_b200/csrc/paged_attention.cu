@@ -229,7 +229,7 @@ int launch_attention_code(const tfx_paged_cache* c, const Paged& p, const PagedA
   int st = TFX_OK;
   if (pl.tc) st = launch_paged_tc<CODE>(c, p, a, pl.q, stream);
   if (st == TFX_OK && pl.small)
-    st = launch_paged_rows<CODE>(p, a, c->head_dim, pl.block_rows,
+    st = launch_paged_rows<CODE>(p, a, c->head_dim, pl.block_rows, pl.tc,
                                  pl.rows < pl.tc_rows ? pl.rows : pl.tc_rows, stream);
   return st;
 }

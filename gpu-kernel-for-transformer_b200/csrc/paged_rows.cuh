@@ -157,13 +157,11 @@ struct RowsCfg {
   static_assert(kKT >= 16 && kKT % 16 == 0, "tile of 16 to 64 keys");
 };
 
-template <int CODE, int HD, int NT>
-__global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
-    paged_rows_kernel(const __grid_constant__ Paged p, const __grid_constant__ PagedAttn a,
-                      int row_blocks) {
-  grid_dep_wait();
-  grid_dep_launch();
-  using C = RowsCfg<CODE, HD, NT>;
+// A CTA's work, in the layout C of NTC blocks of 8 rows; NT of them hold rows.
+template <int CODE, int HD, int NTC, int NT>
+__device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, const PagedSeq& seq,
+                                         int rb, int split) {
+  using C = RowsCfg<CODE, HD, NTC>;
   constexpr int KT = C::kKT, NS = C::NS, HDP = C::kHDP, U = C::kU, W = C::kWarps;
   constexpr int KB = KT / 16;                // 16-key blocks of a tile
   constexpr int KS = HDP / 16;               // 16-wide steps of the first product
@@ -182,13 +180,8 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
   const int g = lane >> 2, t = lane & 3;
   const int b = blockIdx.z, hk = blockIdx.y;
   const int parts = a.cluster > 0 ? a.cluster : a.splits;
-  const int split = static_cast<int>(blockIdx.x) % parts;  // cluster: also the CTA's rank
-  // The last rows see the most keys: they go first.
-  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.x) / parts;
-  const PagedSeq seq = paged_seq(p, b);
   const int rows = seq.n * a.group;  // below 2^31: checked on the host
   const int r0 = rb * C::kRows;
-  if (r0 >= rows || paged_is_tc(a, seq)) return;  // the same for a whole cluster
   // Keys that row r sees: [0, lim(r)).
   auto lim_of = [&](int r) {
     return a.causal ? min(seq.len, max(0, seq.pos0 + r / a.group + 1)) : seq.len;
@@ -211,7 +204,7 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
 
   // ---- queries as the product's B operand, zero rows behind the last one.
   // 8 bits: dims in the order of the codes' k pairs (see the file's comment).
-  for (int i = threadIdx.x; i < C::kRows * (HD / 8); i += C::kThreads) {
+  for (int i = threadIdx.x; i < 8 * NT * (HD / 8); i += C::kThreads) {
     const int r = i / (HD / 8), c = i % (HD / 8), row = r0 + r;
     uint4 x = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows)
@@ -750,11 +743,48 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
   cluster_sync_all();  // no CTA leaves while another reads its results
 }
 
-template <int CODE, int HD, int NT>
+// MIXED: launched behind the tcgen05 kernel of the same call, which waited for what
+// came before both. This one writes other rows, so it need not wait for that kernel;
+// it only ends after it (one CTA stays), so that what follows finds both done. Most
+// of its sequences are running ones, with few rows in a batch that has many: they
+// take only the blocks of 8 that hold rows. (36 sequences with 1 new token and 4 with
+// 200, 8 heads in groups of 4, head_dim 128, 800 to 8000 keys: one behind the other
+// and with all blocks 282 us, so 193; int8 309 and 216. In kernels that run alone the
+// three bodies cost more, in instructions fetched, than they save: drafts of 2 to 8
+// tokens, 55 against 43 us.)
+template <int CODE, int HD, int NT, bool MIXED>
+__global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
+    paged_rows_kernel(const __grid_constant__ Paged p, const __grid_constant__ PagedAttn a,
+                      int row_blocks) {
+  if constexpr (!MIXED) grid_dep_wait();
+  grid_dep_launch();
+  const int parts = a.cluster > 0 ? a.cluster : a.splits;
+  const int split = static_cast<int>(blockIdx.x) % parts;  // cluster: also the CTA's rank
+  // The last rows see the most keys: they go first.
+  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.x) / parts;
+  const PagedSeq seq = paged_seq(p, blockIdx.z);
+  const int left = seq.n * a.group - rb * 8 * NT;
+  const bool mine = left > 0 && !paged_is_tc(a, seq);  // the same for a whole cluster
+  if constexpr (!MIXED) {
+    if (mine) rows_cta<CODE, HD, NT, NT>(p, a, seq, rb, split);
+  } else {
+    if (!mine) {
+    } else if (left <= 8) {
+      rows_cta<CODE, HD, NT, 1>(p, a, seq, rb, split);
+    } else if (NT >= 4 && left <= 16) {
+      rows_cta<CODE, HD, NT, NT >= 4 ? 2 : NT>(p, a, seq, rb, split);
+    } else {
+      rows_cta<CODE, HD, NT, NT>(p, a, seq, rb, split);
+    }
+    if ((blockIdx.x | blockIdx.y | blockIdx.z) == 0) grid_dep_wait();
+  }
+}
+
+template <int CODE, int HD, int NT, bool MIXED>
 int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t stream) {
   using C = RowsCfg<CODE, HD, NT>;
   static int done[kMaxDevices] = {0};
-  auto kern = paged_rows_kernel<CODE, HD, NT>;
+  auto kern = paged_rows_kernel<CODE, HD, NT, MIXED>;
   int st = ensure_smem(reinterpret_cast<const void*>(kern), C::kSmem, done);
   if (st != TFX_OK) return st;
   const int64_t blocks = (rows + C::kRows - 1) / C::kRows;
@@ -784,29 +814,33 @@ int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t s
 }
 
 template <int CODE, int HD>
-int launch_rows_hd(const Paged& p, const PagedAttn& a, int block_rows, int64_t rows,
+int launch_rows_hd(const Paged& p, const PagedAttn& a, int block_rows, bool mixed, int64_t rows,
                    cudaStream_t stream) {
-  if constexpr (HD <= 128) {
-    if (block_rows == 32) return launch_rows<CODE, HD, 4>(p, a, rows, stream);
+  // (beside the tcgen05 kernel: it has head_dim 64 and more, and leaves up to 64 rows)
+  if constexpr (HD >= 64) {
+    if (mixed) return launch_rows<CODE, HD, HD <= 128 ? 4 : 2, true>(p, a, rows, stream);
   }
-  if (block_rows == 16) return launch_rows<CODE, HD, 2>(p, a, rows, stream);
-  return launch_rows<CODE, HD, 1>(p, a, rows, stream);
+  if constexpr (HD <= 128) {
+    if (block_rows == 32) return launch_rows<CODE, HD, 4, false>(p, a, rows, stream);
+  }
+  if (block_rows == 16) return launch_rows<CODE, HD, 2, false>(p, a, rows, stream);
+  return launch_rows<CODE, HD, 1, false>(p, a, rows, stream);
 }
 
 }  // namespace
 
 template <int CODE>
 int launch_paged_rows(const Paged& p, const PagedAttn& a, int head_dim, int block_rows,
-                      int64_t rows, cudaStream_t stream) {
+                      bool mixed, int64_t rows, cudaStream_t stream) {
   switch (head_dim) {
     case 8:
-      if constexpr (CODE == kCodeF16) return launch_rows_hd<CODE, 8>(p, a, block_rows, rows, stream);
+      if constexpr (CODE == kCodeF16) return launch_rows_hd<CODE, 8>(p, a, block_rows, mixed, rows, stream);
       break;
-    case 16: return launch_rows_hd<CODE, 16>(p, a, block_rows, rows, stream);
-    case 32: return launch_rows_hd<CODE, 32>(p, a, block_rows, rows, stream);
-    case 64: return launch_rows_hd<CODE, 64>(p, a, block_rows, rows, stream);
-    case 128: return launch_rows_hd<CODE, 128>(p, a, block_rows, rows, stream);
-    case 256: return launch_rows_hd<CODE, 256>(p, a, block_rows, rows, stream);
+    case 16: return launch_rows_hd<CODE, 16>(p, a, block_rows, mixed, rows, stream);
+    case 32: return launch_rows_hd<CODE, 32>(p, a, block_rows, mixed, rows, stream);
+    case 64: return launch_rows_hd<CODE, 64>(p, a, block_rows, mixed, rows, stream);
+    case 128: return launch_rows_hd<CODE, 128>(p, a, block_rows, mixed, rows, stream);
+    case 256: return launch_rows_hd<CODE, 256>(p, a, block_rows, mixed, rows, stream);
   }
   return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: head_dim %d", head_dim);
 }

@@ -2,5 +2,6 @@
 #include "paged_rows.cuh"
 
 namespace tfx {
-template int launch_paged_rows<kCodeE4M3>(const Paged&, const PagedAttn&, int, int, int64_t, cudaStream_t);
+template int launch_paged_rows<kCodeE4M3>(const Paged&, const PagedAttn&, int, int, bool, int64_t,
+                                         cudaStream_t);
 }  // namespace tfx

@@ -465,6 +465,51 @@ def test_captured_steps_follow_the_tensors(pkg, dev):
     assert warm.shape == (3, heads * hd)
 
 
+@pytest.mark.parametrize("dtype,hd,heads", [(F16, 64, 16), (F16, 128, 10), (I8, 128, 10),
+                                            (E4, 256, 8)],
+                         ids=lambda v: NAMES.get(v, str(v)) if not isinstance(v, int) else str(v))
+def test_chained_steps_of_prompts_and_single_tokens(pkg, dev, dtype, hd, heads):
+    """Both attention kernels of a mixed batch run at the same time; what follows
+    finds both done: each step writes its tokens from the step before and attends,
+    with nothing between the calls, against the same steps one at a time."""
+    lens, group = [(1, 900), (190, 1100), (1, 3000), (17, 30), (140, 140), (1, 1), (6, 2000)], 2
+    pool = pr.Pool(lens, 64, heads, hd, dtype, 31)
+    batch = _batch(pkg, dev, pool, **_hints(pool))
+    q = torch.randn(pool.tokens, heads * group, hd, generator=pool.q_gen).half().to(dev)
+    filled = pool.on(dev, pool.filled())
+
+    def steps(cache, pause):
+        outs, x = [], q
+        for _ in range(6):
+            pkg.ops.paged_append(x[:, :heads], x[:, heads:], cache, batch)
+            pause()
+            out = pkg.ops.paged_attention(x, cache, batch)
+            pause()
+            outs.append(out)
+            x = out.view(pool.tokens, heads * group, hd)
+        return outs
+
+    def fresh():
+        return pkg.PagedKVCache.from_tensors(*[None if t is None else t.clone() for t in filled])
+
+    alone = steps(fresh(), torch.cuda.synchronize)
+    for _ in range(5):
+        got = steps(fresh(), lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+    cache = fresh()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = steps(cache, lambda: None)
+    for _ in range(3):
+        for new, old in zip((cache.k, cache.v, cache.k_scale, cache.v_scale), filled):
+            if old is not None:
+                new.copy_(old)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+
+
 def test_offsets_past_32_bits(pkg, dev):
     """Pages whose offset passes 2^32 elements (8-bit codes: 4.3 GB of K and of V)."""
     heads, hd, page = 16, 128, 256
