@@ -8,10 +8,12 @@ namespace {
 // Keys of a split: a multiple of every kernel's round of tiles over its warps.
 constexpr int kSplitKeys = 256;
 // Sequences with more rows (new tokens x query heads per key/value head) may go
-// to the tcgen05 kernel, whose tiles have 128. (From 33 to 64 rows it is up to 1.4
-// times faster at head_dim 128 in fp16 and hardly elsewhere, but drafts of 2 to 6
-// tokens in groups of 8 then fall to both kernels, one behind the other.)
-constexpr int kTcRows = 64;
+// to the tcgen05 kernel, whose tiles have 128: the wider the head, the more the
+// mma.sync kernel's registers cost it. us with 64 and with this many: 64 sequences
+// with 1 to 8 new tokens and up to 6000 keys, 8 heads in groups of 8, head_dim 64
+// fp16 127 and (32) 136, 128 215 and 191, 256 504 and 308; 32 with 3 at head_dim 256
+// (32 rows) 314 and 239.
+constexpr int tc_rows(int head_dim) { return 4096 / head_dim; }  // from head_dim 64
 // Partial results kept for a call at most, where few splits would do as well.
 constexpr int64_t kPartBytes = 128 << 20;
 
@@ -172,14 +174,14 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   }
   pl.kps_tc = round_keys(kv, tc_parts);
 
-  // Which kernel: more than kTcRows rows, and enough work. Times in ns, fitted to
+  // Which kernel: more than tc_rows rows, and enough work. Times in ns, fitted to
   // both kernels at 1 to 64 sequences of 2 000 to 30 000 tokens, 8 heads, 16 to 128
   // rows; e.g. 128 rows, head_dim 64, fp16: 1 x 2 000 26 us tcgen05, 13 mma.sync;
   // 1 x 30 000 40 and 56; 16 x 3 000 47 and 108; 64 x 4 000 210 and 382.
-  pl.tc = hd >= 64 && group <= 128 && pl.rows > kTcRows;
+  pl.tc = hd >= 64 && group <= 128 && pl.rows > tc_rows(hd);
   if (pl.tc) {
     const int i = hd == 64 ? 0 : hd == 128 ? 1 : 2;
-    constexpr double kTcKey[2][3] = {{11., 13., 16.}, {12.5, 22., 25.}};
+    constexpr double kTcKey[2][3] = {{11., 13., 16.}, {12.5, 13., 16.}};
     constexpr double kRowsKey[2][3] = {{.05, .08, .16}, {.06, .09, .18}};  // of 32 rows
     const double tc_ns = 10e3 + tc_keys * kTcKey[quant][i];
     const double rows_ns =
@@ -187,7 +189,7 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
     pl.tc = tc_ns < rows_ns;
   }
   pl.small = !pl.tc || b->batch > 1;  // a single sequence has all the rows
-  pl.tc_rows = !pl.tc ? 0x7fffffff : pl.small ? kTcRows : 0;
+  pl.tc_rows = !pl.tc ? 0x7fffffff : pl.small ? tc_rows(hd) : 0;
 
   // mma.sync: CTAs to an SM by registers and shared memory; a start costs about
   // as much as 400 keys, a second launch to join as much as 512 and one for every

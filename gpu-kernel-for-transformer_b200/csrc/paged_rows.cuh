@@ -816,7 +816,7 @@ int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t s
 template <int CODE, int HD>
 int launch_rows_hd(const Paged& p, const PagedAttn& a, int block_rows, bool mixed, int64_t rows,
                    cudaStream_t stream) {
-  // (beside the tcgen05 kernel: it has head_dim 64 and more, and leaves up to 64 rows)
+  // (beside the tcgen05 kernel: it has head_dim 64 and more, and leaves this one 64 rows at most, 16 at 256)
   if constexpr (HD >= 64) {
     if (mixed) return launch_rows<CODE, HD, HD <= 128 ? 4 : 2, true>(p, a, rows, stream);
   }
