@@ -151,10 +151,11 @@ __device__ __forceinline__ float paged_value(const void* base, int64_t at, float
 // ------------------------------------------------------------- attention
 // One attention call as its kernels take it. Sequences with more than
 // tc_rows rows (new tokens x group) belong to the tcgen05 kernel, the others to
-// the mma.sync kernel. `splits` CTAs share the keys of a row block, kps (or
-// kps_tc) keys each, a multiple of 256; with splits > 1 their unnormalised
-// results go to part_o [token][q_head][split][head_dim] with the (max, sum) in
-// part_ml, and a third kernel joins them.
+// the mma.sync kernel. splits_rows (or splits_tc) CTAs share the keys of a row
+// block, kps (kps_tc) keys each, a multiple of 256; if more than one, their
+// unnormalised results go to part_o [token][q_head][split][head_dim] with the (max,
+// sum) in part_ml (room for `splits`, the larger number), and a third kernel joins
+// them.
 struct PagedAttn {
   const __half* q;
   int64_t ld_q;
@@ -164,7 +165,7 @@ struct PagedAttn {
   float scale_log2;
   int causal;
   int tc_rows;
-  int splits, kps, kps_tc;
+  int splits, splits_rows, splits_tc, kps, kps_tc;
   int cluster;  // mma.sync kernel: CTAs of a cluster that share a row block's keys; 0: splits
   float* part_o;
   float2* part_ml;
@@ -178,17 +179,22 @@ __device__ __forceinline__ int paged_split_keys(const PagedAttn& a, const PagedS
   return paged_is_tc(a, s) ? a.kps_tc : a.kps;
 }
 
+__device__ __forceinline__ int paged_split_count(const PagedAttn& a, const PagedSeq& s) {
+  return paged_is_tc(a, s) ? a.splits_tc : a.splits_rows;
+}
+
 // Keys are split for this sequence (its partial results are joined later);
 // otherwise split 0 holds all of them and writes the rows itself.
 __device__ __forceinline__ bool paged_is_split(const PagedAttn& a, const PagedSeq& s) {
-  return a.splits > 1 && s.len > paged_split_keys(a, s);
+  return paged_split_count(a, s) > 1 && s.len > paged_split_keys(a, s);
 }
 
 // End of the keys of a split (the last one takes whatever is left: max_kv_len may
 // have been less than a sequence's length).
 __device__ __forceinline__ int paged_split_end(const PagedAttn& a, const PagedSeq& s, int split,
                                                int k_begin) {
-  return split == a.splits - 1 ? s.len : min(s.len, k_begin + paged_split_keys(a, s));
+  return split == paged_split_count(a, s) - 1 ? s.len
+                                              : min(s.len, k_begin + paged_split_keys(a, s));
 }
 
 // Rows of a CTA of the mma.sync kernel for rows = max_query_len * group.

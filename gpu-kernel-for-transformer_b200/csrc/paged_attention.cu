@@ -17,90 +17,139 @@ constexpr int tc_rows(int head_dim) { return 4096 / head_dim; }  // from head_di
 // Partial results kept for a call at most, where few splits would do as well.
 constexpr int64_t kPartBytes = 128 << 20;
 
-// out[row] = sum over splits of partial O scaled to the common maximum, over
-// the sum of their sums. `wpr` warps of the CTA per (token, head) row: one when
-// there are few splits (more rows per CTA), four when there are many.
+// N consecutive floats of a lane, aligned to as many.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* src, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(src + i);
+      v[i] = x.x;
+      v[i + 1] = x.y;
+      v[i + 2] = x.z;
+      v[i + 3] = x.w;
+    }
+  } else if constexpr (N == 2) {
+    const float2 x = *reinterpret_cast<const float2*>(src);
+    v[0] = x.x;
+    v[1] = x.y;
+  } else {
+    v[0] = *src;
+  }
+}
+
+// out[row] = sum over splits of partial O scaled to the common maximum, over the
+// sum of their sums, for the rows of sequences whose keys are split. blockIdx.y:
+// sequence, whose first CTA-many rows (token, head) go to its CTAs in turn, so that
+// sequences without splits cost next to nothing (a search for every row's sequence
+// took 33 us behind a batch of prompts that had no splits). `wpr` warps of the CTA
+// per row: one when there are few splits (more rows per CTA), four when there are
+// many. Bound by latency: lanes hold a split's factor each, the loads of partial O
+// do not wait for one another.
 template <int HD>
 __global__ void __launch_bounds__(128)
     paged_join_kernel(const __grid_constant__ Paged p, const __grid_constant__ PagedAttn a,
-                      int64_t rows, int wpr) {
+                      int wpr) {
   grid_dep_wait();
   grid_dep_launch();
   constexpr int DL = HD >= 32 ? HD / 32 : 1;  // dims of a lane
   __shared__ float sm[4][HD];
+  const PagedSeq seq = paged_seq(p, blockIdx.y);
+  if (!paged_is_split(a, seq)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / wpr) + warp / wpr;
-  const int part = warp % wpr, heads = p.kv_heads * a.group;
-  int n = 0, tok = 0, head = 0;
-  if (row < rows) {
-    tok = static_cast<int>(row / heads);
-    head = static_cast<int>(row % heads);
-    const int b = paged_seq_of_row(p, tok);
-    if (b >= 0) {
-      const PagedSeq s = paged_seq(p, b);
-      if (paged_is_split(a, s) && tok >= s.row0 && tok < s.row0 + s.n) {
-        const int lim = a.causal ? min(s.len, max(0, s.pos0 + (tok - s.row0) + 1)) : s.len;
-        n = min(a.splits, (lim + paged_split_keys(a, s) - 1) / paged_split_keys(a, s));
-        if (n == 0) n = -1;  // a split sequence's row that sees no key
+  const int part = warp % wpr, heads = p.kv_heads * a.group, per_cta = 4 / wpr;
+  const int keys = paged_split_keys(a, seq);
+  const bool mine = HD >= 32 || lane < HD;
+  const int64_t rows = static_cast<int64_t>(seq.n) * heads;
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per_cta; r0 < rows;
+       r0 += static_cast<int64_t>(gridDim.x) * per_cta) {
+    const int64_t r = r0 + warp / wpr;
+    const bool real = r < rows;  // the same for a warp
+    const int i = real ? static_cast<int>(r / heads) : 0, head = static_cast<int>(r % heads);
+    const int lim = a.causal ? min(seq.len, max(0, seq.pos0 + i + 1)) : seq.len;
+    const int n = real ? min(paged_split_count(a, seq), (lim + keys - 1) / keys) : 0;
+    const int64_t base = (static_cast<int64_t>(seq.row0 + i) * heads + head) * a.splits;
+    float m = -INFINITY, l = 0.f, acc[DL];
+#pragma unroll
+    for (int e = 0; e < DL; ++e) acc[e] = 0.f;
+    for (int s = lane; s < n; s += 32) m = fmaxf(m, a.part_ml[base + s].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int s0 = 0; s0 < n; s0 += 32) {
+      float f = 0.f;
+      bool seen = false;  // the split saw a key of this row
+      if (s0 + lane < n) {
+        const float2 ml = a.part_ml[base + s0 + lane];
+        f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - m);
+        seen = !(f == 0.f && ml.y == 0.f);
+        if (seen) l += f * ml.y;
+      }
+      const uint32_t used = __ballot_sync(0xffffffffu, seen);
+      const int count = min(32, n - s0);
+#pragma unroll 4
+      for (int j = part; j < count; j += wpr) {
+        const float g = __shfl_sync(0xffffffffu, f, j);
+        float v[DL];
+        if (mine) load_floats<DL>(a.part_o + (base + s0 + j) * HD + lane * DL, v);
+        if ((used >> j) & 1u) {
+#pragma unroll
+          for (int e = 0; e < DL; ++e) acc[e] = mine ? acc[e] + g * v[e] : 0.f;
+        }
       }
     }
-  }
-  const int64_t base = row * a.splits;
-  float m = -INFINITY, acc[DL], l = 0.f;
 #pragma unroll
-  for (int e = 0; e < DL; ++e) acc[e] = 0.f;
-  for (int s = lane; s < n; s += 32) m = fmaxf(m, a.part_ml[base + s].x);
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    if (wpr > 1) {
+      if (mine) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  for (int s = 0; s < n; ++s) {
-    const float2 ml = a.part_ml[base + s];
-    const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2(ml.x - m);
-    if (f == 0.f && ml.y == 0.f) continue;
-    l += f * ml.y;
-    if (s % wpr != part) continue;
-    const float* src = a.part_o + (base + s) * HD + lane * DL;
-    if (HD >= 32 || lane < HD) {
+        for (int e = 0; e < DL; ++e) sm[warp][lane * DL + e] = acc[e];
+      }
+      __syncthreads();
+      if (warp == 0 && mine) {
 #pragma unroll
-      for (int e = 0; e < DL; ++e) acc[e] += f * src[e];
+        for (int w = 1; w < 4; ++w)
+#pragma unroll
+          for (int e = 0; e < DL; ++e) acc[e] += sm[w][lane * DL + e];
+      }
+      __syncthreads();
+    }
+    if (part != 0 || !real || !mine) continue;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    __half* dst = a.out + static_cast<int64_t>(seq.row0 + i) * a.ld_out + head * HD + lane * DL;
+    if constexpr (DL == 1) {
+      *dst = __float2half_rn(acc[0] * inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < DL; e += 2)
+        *reinterpret_cast<uint32_t*>(dst + e) = pack_half2(acc[e] * inv, acc[e + 1] * inv);
     }
   }
-  if (wpr > 1) {
-    if (HD >= 32 || lane < HD) {
-#pragma unroll
-      for (int e = 0; e < DL; ++e) sm[warp][lane * DL + e] = acc[e];
-    }
-    __syncthreads();
-    if (warp != 0) return;
-#pragma unroll
-    for (int w = 1; w < 4; ++w)
-#pragma unroll
-      for (int e = 0; e < DL; ++e)
-        if (HD >= 32 || lane < HD) acc[e] += sm[w][lane * DL + e];
-  }
-  if (n == 0 || (HD < 32 && lane >= HD)) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  __half* dst = a.out + static_cast<int64_t>(tok) * a.ld_out + head * HD + lane * DL;
-#pragma unroll
-  for (int e = 0; e < DL; ++e) dst[e] = __float2half_rn(acc[e] * inv);
 }
 
+// rows: (token, head) rows of a sequence that may be split, at most.
 template <int HD>
-int launch_join(const Paged& p, const PagedAttn& a, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.kv_heads * a.group;
+int launch_join(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t stream) {
+  const int64_t all = static_cast<int64_t>(p.num_tokens) * p.kv_heads * a.group;
   const int wpr = a.splits > 16 ? 4 : 1, per_cta = 4 / wpr;
-  launch_pdl(paged_join_kernel<HD>, dim3(static_cast<unsigned>((rows + per_cta - 1) / per_cta)),
-             dim3(128), 0, stream, p, a, rows, wpr);
+  // A CTA for every per_cta rows of the longest sequence, but not many more in all
+  // than there are rows.
+  int64_t most = 2 * ((all + per_cta - 1) / per_cta) / p.batch;
+  if (most < 4096 / p.batch) most = 4096 / p.batch;
+  int64_t x = (rows + per_cta - 1) / per_cta;
+  if (x > most) x = most < 1 ? 1 : most;
+  launch_pdl(paged_join_kernel<HD>, dim3(static_cast<unsigned>(x), static_cast<unsigned>(p.batch)),
+             dim3(128), 0, stream, p, a, wpr);
   return check_launch("paged_join_kernel");
 }
 
-int join_hd(const Paged& p, const PagedAttn& a, int head_dim, cudaStream_t stream) {
+int join_hd(const Paged& p, const PagedAttn& a, int head_dim, int64_t rows, cudaStream_t stream) {
   switch (head_dim) {
-    case 8: return launch_join<8>(p, a, stream);
-    case 16: return launch_join<16>(p, a, stream);
-    case 32: return launch_join<32>(p, a, stream);
-    case 64: return launch_join<64>(p, a, stream);
-    case 128: return launch_join<128>(p, a, stream);
-    default: return launch_join<256>(p, a, stream);
+    case 8: return launch_join<8>(p, a, rows, stream);
+    case 16: return launch_join<16>(p, a, rows, stream);
+    case 32: return launch_join<32>(p, a, rows, stream);
+    case 64: return launch_join<64>(p, a, rows, stream);
+    case 128: return launch_join<128>(p, a, rows, stream);
+    default: return launch_join<256>(p, a, rows, stream);
   }
 }
 
@@ -109,7 +158,7 @@ struct Plan {
   int block_rows;   // of the mma.sync kernel
   int tc_rows;      // sequences with more rows go to the tcgen05 kernel
   bool tc, small;   // which kernels run
-  int splits, kps, kps_tc, cluster;
+  int splits, splits_rows, splits_tc, kps, kps_tc, cluster;
   int64_t ml_offset, bytes;  // workspace
 };
 
@@ -213,10 +262,10 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   } else {
     pl.kps = round_keys(kv, parts);
   }
-  int64_t least = pl.tc ? pl.kps_tc : pl.kps;
-  if (pl.small && pl.kps < least) least = pl.kps;
-  pl.splits = static_cast<int>((kv + least - 1) / least);
-  if (pl.cluster > 0) pl.splits = 1;
+  pl.splits_tc = pl.tc ? static_cast<int>((kv + pl.kps_tc - 1) / pl.kps_tc) : 1;
+  pl.splits_rows =
+      pl.small && pl.cluster == 0 ? static_cast<int>((kv + pl.kps - 1) / pl.kps) : 1;
+  pl.splits = pl.splits_tc > pl.splits_rows ? pl.splits_tc : pl.splits_rows;
   if (pl.splits > 1) {
     const int64_t part_rows = static_cast<int64_t>(b->num_tokens) * q_heads * pl.splits;
     pl.ml_offset = part_rows * hd;  // floats; head_dim is even: float2 stays aligned
@@ -316,6 +365,8 @@ int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* 
   a.scale_log2 = scale_log2;
   a.causal = causal != 0;
   a.splits = pl.splits;
+  a.splits_rows = pl.splits_rows;
+  a.splits_tc = pl.splits_tc;
   a.kps = pl.kps;
   a.kps_tc = pl.kps_tc;
   a.tc_rows = pl.tc_rows;
@@ -329,7 +380,9 @@ int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* 
     default: st = launch_attention_code<kCodeE4M3>(cache, p, a, pl, stream); break;
   }
   if (st != TFX_OK || pl.splits == 1) return st;
-  return join_hd(p, a, cache->head_dim, stream);
+  // (the sequences with more rows are the tcgen05 kernel's)
+  const int64_t rows = pl.tc && pl.splits_tc == 1 ? pl.tc_rows : pl.rows;
+  return join_hd(p, a, cache->head_dim, rows * cache->kv_heads, stream);
 }
 
 }  // extern "C"

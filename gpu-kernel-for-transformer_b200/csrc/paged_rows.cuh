@@ -179,7 +179,7 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int b = blockIdx.z, hk = blockIdx.y;
-  const int parts = a.cluster > 0 ? a.cluster : a.splits;
+  const int parts = a.cluster > 0 ? a.cluster : a.splits_rows;
   const int rows = seq.n * a.group;  // below 2^31: checked on the host
   const int r0 = rb * C::kRows;
   // Keys that row r sees: [0, lim(r)).
@@ -194,7 +194,7 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
     k_begin = min(split * share, lim_last);
     k_end = min(k_begin + share, lim_last);
   } else {
-    // Splits behind the sequence (64 bits: splits is the larger kernel's number).
+    // Splits behind the sequence.
     if (is_split ? static_cast<int64_t>(split) * a.kps >= lim_last : split > 0) return;
     if (is_split) {
       k_begin = split * a.kps;
@@ -758,7 +758,7 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
                       int row_blocks) {
   if constexpr (!MIXED) grid_dep_wait();
   grid_dep_launch();
-  const int parts = a.cluster > 0 ? a.cluster : a.splits;
+  const int parts = a.cluster > 0 ? a.cluster : a.splits_rows;
   const int split = static_cast<int>(blockIdx.x) % parts;  // cluster: also the CTA's rank
   // The last rows see the most keys: they go first.
   const int rb = row_blocks - 1 - static_cast<int>(blockIdx.x) / parts;
@@ -788,7 +788,7 @@ int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t s
   int st = ensure_smem(reinterpret_cast<const void*>(kern), C::kSmem, done);
   if (st != TFX_OK) return st;
   const int64_t blocks = (rows + C::kRows - 1) / C::kRows;
-  const int parts = a.cluster > 0 ? a.cluster : a.splits;
+  const int parts = a.cluster > 0 ? a.cluster : a.splits_rows;
   if (blocks * parts > 0x7fffffffLL)
     return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: too many rows");
   cudaLaunchAttribute attr[2];
@@ -816,7 +816,7 @@ int launch_rows(const Paged& p, const PagedAttn& a, int64_t rows, cudaStream_t s
 template <int CODE, int HD>
 int launch_rows_hd(const Paged& p, const PagedAttn& a, int block_rows, bool mixed, int64_t rows,
                    cudaStream_t stream) {
-  // (beside the tcgen05 kernel: it has head_dim 64 and more, and leaves this one 64 rows at most, 16 at 256)
+  // (the tcgen05 kernel has head_dim 64 and more, and leaves 64 rows at most, 16 at 256)
   if constexpr (HD >= 64) {
     if (mixed) return launch_rows<CODE, HD, HD <= 128 ? 4 : 2, true>(p, a, rows, stream);
   }

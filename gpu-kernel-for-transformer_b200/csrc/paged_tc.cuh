@@ -147,9 +147,9 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   // ---- this CTA's work
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.x, b = blockIdx.y;
-  const int split = static_cast<int>(blockIdx.z) % a.splits;
+  const int split = static_cast<int>(blockIdx.z) % a.splits_tc;
   // The last rows of all sequences and heads see the most keys: they go first.
-  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.z) / a.splits;
+  const int rb = row_blocks - 1 - static_cast<int>(blockIdx.z) / a.splits_tc;
   const int group = a.group, tile_tokens = kPtTile / group;
   const PagedSeq seq = paged_seq(p, b);
   const int i0 = rb * L::kNT * tile_tokens;  // first token
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     return a.causal ? min(seq.len, max(0, seq.pos0 + i + 1)) : seq.len;
   };
   const bool is_split = paged_is_split(a, seq);
-  // Splits behind the sequence (64 bits: splits is the larger kernel's number).
+  // Splits behind the sequence.
   if (is_split ? static_cast<int64_t>(split) * a.kps_tc >= seq.len : split > 0) return;
   const int k_begin = is_split ? split * a.kps_tc : 0;
   const int k_stop = is_split ? paged_split_end(a, seq, split, k_begin) : seq.len;  // of the split
@@ -993,9 +993,9 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   if (st == TFX_OK) st = make_tmap(&tv, p.v, dt, 4, kd, ks, kb, sw);
   if (st != TFX_OK) return st;
   const int64_t blocks = (tokens + L::kNT * tile_tokens - 1) / (L::kNT * tile_tokens);
-  if (blocks * a.splits > 65535)
+  if (blocks * a.splits_tc > 65535)
     return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: max_query_len is too long for the grid");
-  launch_pdl(kern, dim3(p.kv_heads, p.batch, static_cast<unsigned>(blocks * a.splits)),
+  launch_pdl(kern, dim3(p.kv_heads, p.batch, static_cast<unsigned>(blocks * a.splits_tc)),
              dim3(L::kThreads), L::kSmem, stream, tq, tk, tv, p, a, static_cast<int>(blocks),
              device_error_word());
   return check_launch("paged_tc_kernel");
