@@ -280,9 +280,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: P
     token and head (max|x| / 127 or / 448): codes are those of exact
     arithmetic, ties to even; a row of zeros gets scale 0, a row with an
     infinity or NaN gets scale NaN and reads back as NaN. Tokens whose page is
-    outside the pool are dropped. Where two tokens of a batch share a slot, one
-    of them is kept. The paged form of the reference's ``_append_kv_cache``
-    (torch_transformer_benchmark.py:426-462).
+    outside the pool are dropped. Two tokens of a batch must not share a slot (it
+    would hold parts of both; other slots are not affected). The paged form of the
+    reference's ``_append_kv_cache`` (torch_transformer_benchmark.py:426-462).
     """
     index = _paged_device(cache, batch)
     n, heads, hd, dev = batch.num_tokens, cache.kv_heads, cache.head_dim, cache.device

@@ -30,7 +30,17 @@ _CODES = {
 }
 
 
-class PagedKVCache:
+class _Fixed:
+    """Attributes that the C structure (`_ref`, set last) was built from: not to be replaced."""
+
+    def __setattr__(self, name, value):
+        if "_ref" in self.__dict__:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed once the object is made: "
+                                 "write into its tensors, or make another")
+        super().__setattr__(name, value)
+
+
+class PagedKVCache(_Fixed):
     """A pool of ``num_pages`` pages of ``page_size`` tokens (16, 32, 64, 128 or 256).
 
     ``dtype``: ``torch.float16``; or ``torch.int8`` / ``torch.float8_e4m3fn``,
@@ -92,9 +102,9 @@ class PagedKVCache:
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if quant else None,
             v_scale.data_ptr() if quant else None, _CODES[k.dtype], pages, page_size, heads, hd,
             *strides[:3])
-        self._ref = ctypes.byref(self._struct)
         self._half = k.new_empty(0, dtype=torch.float16)  # outputs are allocated from it
         self._geometry = (heads, hd, page_size, k.dtype)
+        self._ref = ctypes.byref(self._struct)
 
 
 def _strides(t: torch.Tensor):
@@ -107,7 +117,7 @@ def _strides(t: torch.Tensor):
     return tuple(out)
 
 
-class PagedBatch:
+class PagedBatch(_Fixed):
     """The sequences of one step, their new tokens packed one behind the other.
 
     ``page_table`` int32 [B, max_pages]: the pages of each sequence in order of
@@ -124,7 +134,8 @@ class PagedBatch:
     split over the GPU.
 
     The device tensors are kept and read when a kernel runs, so a captured
-    graph sees what they hold at its replay.
+    graph sees what they hold at its replay. (Write into them; attributes cannot
+    be replaced.)
     """
 
     def __init__(self, page_table: torch.Tensor, query_start: torch.Tensor, kv_len: torch.Tensor,
@@ -153,8 +164,8 @@ class PagedBatch:
             page_table.data_ptr(), page_table.stride(0) if b > 1 else width, width,
             query_start.data_ptr(), kv_len.data_ptr(), b, num_tokens, self.max_query_len,
             min(self.max_kv_len, 1 << 30))
-        self._ref = ctypes.byref(self._struct)
         self._workspaces = {}
+        self._ref = ctypes.byref(self._struct)
 
     def _workspace_bytes(self, lib, cache: PagedKVCache, q_heads: int) -> int:
         """Workspace of an attention call (a function of sizes only, looked up once)."""

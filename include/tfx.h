@@ -343,7 +343,8 @@ typedef struct tfx_paged_batch {
  * 8-bit types: per token and head scale = max|x| / 127 (or / 448) in fp32 and
  * code = x / scale rounded to nearest, ties to even, as if computed exactly;
  * a row of zeros has scale 0, a row with an infinity or NaN has scale NaN (it
- * reads back as NaN) and codes 0.
+ * reads back as NaN) and codes 0. Two tokens of a batch must not share a slot
+ * (it would hold parts of both).
  * k, v: fp16, element (row, h, e) at k[row*ld_k + h*head_dim + e]; 16-byte
  * aligned, ld a multiple of 8.
  */
@@ -370,8 +371,9 @@ TFX_API int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* 
  * row that sees no key is zero.
  * q, out: fp16, element (row, h, e) at q[row*ld_q + h*head_dim + e], 16-byte
  * aligned, ld a multiple of 8, not overlapping (slices of one row are fine);
- * scale > 0 and finite. q_heads is a multiple of cache->kv_heads. The new tokens' keys and values must be in the cache
- * (tfx_paged_append before, on the same stream).
+ * scale > 0 and finite. q_heads is a multiple of cache->kv_heads. The new tokens'
+ * keys and values must be in the cache (tfx_paged_append before, on the same
+ * stream).
  * workspace: tfx_paged_attention_workspace_bytes() of the same arguments (0:
  * may be NULL), 256-byte aligned, for partial results of keys split over
  * CTAs; calls that may overlap need one each.

@@ -169,6 +169,28 @@ def test_copies_leave_everything_else(pkg, dev, dtype):
                     assert _same(row, (code.float() * scale[..., None]).half())
 
 
+@pytest.mark.parametrize("dtype", [F16, I8, E4], ids=["fp16", "int8", "e4m3"])
+def test_the_same_slot_twice(pkg, dev, dtype):
+    """Tokens that share a slot, which is not allowed, leave every other slot right."""
+    heads, hd, page = 3, 64, 16
+    gen = torch.Generator().manual_seed(77)
+    x = torch.randn(40, 2, heads, hd, generator=gen).half()
+    cache = pkg.PagedKVCache(4, page, heads, hd, dtype, dev)
+    # sequence 0 has page 2 twice (positions 0-15 and 16-31), sequence 1 page 0
+    batch = pkg.PagedBatch(torch.tensor([[2, 2], [0, 1]], dtype=torch.int32, device=dev),
+                           torch.tensor([0, 20, 40], dtype=torch.int32, device=dev),
+                           torch.tensor([20, 20], dtype=torch.int32, device=dev), 40)
+    pkg.ops.paged_append(x[:, 0].to(dev), x[:, 1].to(dev), cache, batch)
+    k, v = pkg.ops.paged_read(cache, batch)
+    for which, got in enumerate((k.cpu(), v.cpu())):
+        for row in [*range(4, 16), *range(20, 40)]:  # slots 0-3 of page 2 are written twice
+            want = x[row, which]
+            if dtype != F16:
+                code, scale = pr.quantise(want, dtype)
+                want = (code.float() * scale[..., None]).half()
+            assert _same(got[row], want)
+
+
 def _attend(pkg, dev, pool, group, causal=True, scale=None, hints=True, q=None, gain=1.5):
     cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled()))
     batch = _batch(pkg, dev, pool, **(_hints(pool) if hints else {}))

@@ -185,3 +185,18 @@ def test_the_model_of_the_cache():
     k, v = pool.values(0, 0), pool.values(0, 1)
     w = torch.softmax(q[4, 3].double() @ k[:, 1].T / 4, -1)
     assert torch.allclose(out[4].view(4, 16)[3], w @ v[:, 1], atol=1e-14)
+
+
+def test_handles_are_fixed():
+    """The C structures hold the tensors' addresses: replacing one would leave them behind."""
+    pkg = load_package()
+    cache = pkg.PagedKVCache(3, 16, 2, 32, I8, "cpu")
+    batch = pkg.PagedBatch(torch.zeros(2, 3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32),
+                           torch.zeros(2, dtype=torch.int32), 4)
+    for obj, name, value in ((cache, "k", cache.k.clone()), (cache, "k_scale", None),
+                             (cache, "head_dim", 16), (batch, "num_tokens", 2),
+                             (batch, "kv_len", torch.ones(2, dtype=torch.int32)),
+                             (batch, "max_query_len", 1)):
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(obj, name, value)
+    batch.kv_len.fill_(5)
