@@ -164,12 +164,20 @@ struct PagedAttn {
   int group;  // query heads per key/value head
   float scale_log2;
   int causal;
+  int q_len;  // tokens of a sequence that are attended: max_query_len
   int tc_rows;
   int splits, splits_rows, splits_tc, kps, kps_tc;
   int cluster;  // mma.sync kernel: CTAs of a cluster that share a row block's keys; 0: splits
   float* part_o;
   float2* part_ml;
 };
+
+// The sequence as attention takes it: its first q_len tokens (which stay where they are).
+__device__ __forceinline__ PagedSeq paged_attn_seq(const Paged& p, const PagedAttn& a, int b) {
+  PagedSeq s = paged_seq(p, b);
+  s.n = min(s.n, a.q_len);
+  return s;
+}
 
 __device__ __forceinline__ bool paged_is_tc(const PagedAttn& a, const PagedSeq& s) {
   return s.n * a.group > a.tc_rows;  // below 2^31: checked on the host

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(128)
   grid_dep_launch();
   constexpr int DL = HD >= 32 ? HD / 32 : 1;  // dims of a lane
   __shared__ float sm[4][HD];
-  const PagedSeq seq = paged_seq(p, blockIdx.y);
+  const PagedSeq seq = paged_attn_seq(p, a, blockIdx.y);
   if (!paged_is_split(a, seq)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp % wpr, heads = p.kv_heads * a.group, per_cta = 4 / wpr;
@@ -364,6 +364,7 @@ int tfx_paged_attention(const tfx_half* q, int64_t ld_q, const tfx_paged_cache* 
   a.group = q_heads / cache->kv_heads;
   a.scale_log2 = scale_log2;
   a.causal = causal != 0;
+  a.q_len = static_cast<int>(pl.q);
   a.splits = pl.splits;
   a.splits_rows = pl.splits_rows;
   a.splits_tc = pl.splits_tc;

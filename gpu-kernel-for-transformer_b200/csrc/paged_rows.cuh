@@ -762,7 +762,7 @@ __global__ void __launch_bounds__((RowsCfg<CODE, HD, NT>::kThreads))
   const int split = static_cast<int>(blockIdx.x) % parts;  // cluster: also the CTA's rank
   // The last rows see the most keys: they go first.
   const int rb = row_blocks - 1 - static_cast<int>(blockIdx.x) / parts;
-  const PagedSeq seq = paged_seq(p, blockIdx.z);
+  const PagedSeq seq = paged_attn_seq(p, a, blockIdx.z);
   const int left = seq.n * a.group - rb * 8 * NT;
   const bool mine = left > 0 && !paged_is_tc(a, seq);  // the same for a whole cluster
   if constexpr (!MIXED) {

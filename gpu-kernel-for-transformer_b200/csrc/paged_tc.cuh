@@ -151,7 +151,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   // The last rows of all sequences and heads see the most keys: they go first.
   const int rb = row_blocks - 1 - static_cast<int>(blockIdx.z) / a.splits_tc;
   const int group = a.group, tile_tokens = kPtTile / group;
-  const PagedSeq seq = paged_seq(p, b);
+  const PagedSeq seq = paged_attn_seq(p, a, b);
   const int i0 = rb * L::kNT * tile_tokens;  // first token
   if (i0 >= seq.n || !paged_is_tc(a, seq)) return;
   auto lim_of = [&](int i) {  // token i sees keys [0, lim)

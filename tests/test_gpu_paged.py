@@ -383,6 +383,30 @@ def test_sequences_longer_than_the_hint(pkg, dev, dtype, lens, hint):
     _check(pool, got, q, 2)
 
 
+@pytest.mark.parametrize("dtype", [F16, I8], ids=["fp16", "int8"])
+@pytest.mark.parametrize("hd,heads,lens,most", [
+    (64, 2, [(5, 3000), (1, 40), (2, 700)], 2),         # keys split over CTAs, and joined
+    (32, 3, [(40, 50), (9, 9), (1, 1)], 11),            # more than a block of rows
+    (128, 10, [(300, 900), (1, 500), (190, 190)], 150),  # the tcgen05 kernel, and few rows
+    (64, 1, [(400, 9000)], 130),
+])
+def test_more_new_tokens_than_the_bound(pkg, dev, dtype, hd, heads, lens, most):
+    """The first max_query_len tokens of a sequence attend as ever, further rows stay as
+    they were."""
+    pool, group = pr.Pool(lens, 64, heads, hd, dtype, 14), 2
+    cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled()))
+    batch = _batch(pkg, dev, pool, max_query_len=most, max_kv_len=int(pool.kv.max()))
+    q = torch.randn(pool.tokens, heads * group, hd, generator=pool.q_gen).half()
+    out = torch.full((pool.tokens, heads * group * hd), -3.0, dtype=F16, device=dev)
+    got = pkg.ops.paged_attention(q.to(dev), cache, batch, out=out).double().cpu()
+    ref, mag, expo = pr.attention(pool, q, group, True, None, ())
+    ok = (got - ref).abs() <= pr.tolerance(pool, ref, mag, expo)
+    for b, (n, _) in enumerate(lens):
+        rows = int(pool.start[b]) + torch.arange(n)
+        assert bool(ok[rows[:most]].all())
+        assert bool((got[rows[most:]] == -3).all())
+
+
 @pytest.mark.parametrize("dtype", [F16, E4], ids=["fp16", "e4m3"])
 def test_shared_pages_and_packed_slices(pkg, dev, dtype):
     """Two sequences share the pages of a common prefix; q, k, v are slices of one
