@@ -9,16 +9,15 @@
 //
 // Quantisation rounds x / s as if in exact arithmetic, so that a code is the
 // nearest one even when the quotient lies within an fp32 rounding of the
-// border between two codes:
+// border between two codes. x times a number just below 1/s and x times one just
+// above give the same code, which is then that of x / s, for all but a few
+// elements in 10^5; there the 8 elements of the thread are done again:
 //  int8: c = rint(x * (1/s)) is the nearest code or, next to a border, its
 //        neighbour; e = fma(-c, s, x) is x - c*s exactly (x has 11 bits, and
 //        near a border ulp(s) <= ulp(x), so e has at most 24), and |e| against
 //        s/2 tells which.
-//  e4m3: the quotient's bits behind the 3 of the code decide unless they are
-//        within 8 ulp of a half (or the code is subnormal); then the quotient
-//        is divided out and rounded to odd, which rounds on correctly.
-// Eight elements are quantised without a branch, and again with these
-// corrections where one of them needs it (a few in 10^5 for int8).
+//  e4m3: the quotient is divided out and rounded to odd, which rounds on
+//        correctly.
 #include "paged.cuh"
 
 namespace tfx {
@@ -77,55 +76,67 @@ __device__ __forceinline__ uint2 quantise(const uint4& x, uint32_t top, float* s
   const float s = scale_of<CODE>(__half2float(__ushort_as_half(static_cast<unsigned short>(top))));
   *scale = s;
   if (top == 0u) return make_uint2(0u, 0u);
-  float inv;  // within an ulp: the checks below allow for it
+  // 1/s lies between lo and hi (the approximation is within 2^-23), so the quotient
+  // rounds to the code that x * lo and x * hi have in common.
+  constexpr float kWide = CODE == kCodeI8 ? 1.f / (1 << 22) : 1.f / (1 << 21);
+  float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
-  const float half_s = 0.5f * s;
+  const float lo = inv * (1.f - kWide), hi = inv * (1.f + kWide);
+  const uint64_t lo2 = f2_pack(lo, lo), hi2 = f2_pack(hi, hi);
   float f[8];
+  uint64_t f2[4];
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 y = __half22float2(bits_h2(w[i]));
     f[2 * i] = y.x;
     f[2 * i + 1] = y.y;
+    f2[i] = f2_pack(y.x, y.y);
   }
-  uint32_t out[2];
-  bool border = false;
+  uint32_t out[2], differ = 0;
   if constexpr (CODE == kCodeI8) {
-    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the code
+    const uint64_t round2 = f2_pack(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the low byte is the code
     uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float m = fmaf(f[i], inv, kRound);
-      border |= fabsf(fmaf(kRound - m, s, f[i])) >= half_s;
-      c[i] = __float_as_uint(m);
+    for (int i = 0; i < 4; ++i) {
+      float a0, a1, b0, b1;
+      f2_unpack(f2_fma(f2[i], lo2, round2), a0, a1);
+      f2_unpack(f2_fma(f2[i], hi2, round2), b0, b1);
+      c[2 * i] = __float_as_uint(a0);
+      c[2 * i + 1] = __float_as_uint(a1);
+      differ |= c[2 * i] ^ __float_as_uint(b0);
+      differ |= c[2 * i + 1] ^ __float_as_uint(b1);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       out[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040),
                            __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
-    if (border) {
+    if (differ != 0u) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = exact_i8(f[i], inv, s, half_s) & 0xff;
+      for (int i = 0; i < 8; ++i) c[i] = exact_i8(f[i], inv, s, 0.5f * s) & 0xff;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         out[i] = c[4 * i] | (c[4 * i + 1] << 8) | (c[4 * i + 2] << 16) | (c[4 * i + 3] << 24);
     }
   } else {
-    float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y[i] = f[i] * inv;
-      // The low 20 bits within 8 of a half, tested at the top of the word; below 2^-6.
-      border |= __float_as_uint(y[i]) * 4096u - (0x7fff8u << 12) <= (16u << 12);
-      border |= fabsf(y[i]) < 0.015625f;
+    for (int i = 0; i < 2; ++i) {
+      float a[4], b[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f2_unpack(f2_mul(f2[2 * i + j], lo2), a[2 * j], a[2 * j + 1]);
+        f2_unpack(f2_mul(f2[2 * i + j], hi2), b[2 * j], b[2 * j + 1]);
+      }
+      out[i] = e4m3x2(a[0], a[1]) | (e4m3x2(a[2], a[3]) << 16);
+      differ |= out[i] ^ (e4m3x2(b[0], b[1]) | (e4m3x2(b[2], b[3]) << 16));
     }
-    if (border) {
+    if (differ != 0u) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = exact_quot(f[i], s);
+      for (int i = 0; i < 8; ++i) f[i] = exact_quot(f[i], s);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        out[i] = e4m3x2(f[4 * i], f[4 * i + 1]) | (e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      out[i] = e4m3x2(y[4 * i], y[4 * i + 1]) | (e4m3x2(y[4 * i + 2], y[4 * i + 3]) << 16);
   }
   return make_uint2(out[0], out[1]);
 }
