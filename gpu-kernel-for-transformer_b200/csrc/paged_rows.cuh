@@ -102,6 +102,11 @@ __device__ __forceinline__ void rows_mma(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float rows_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float4 rows_peer4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
@@ -554,9 +559,23 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
       }
     }
 
-    // ---- weights, as the second product's B operand
+    // ---- weights, as the second product's B operand. The sum takes them as rounded
+    // to fp16, or a row in which one key has nearly all the weight would carry that
+    // key's rounding in full. 8 bit: the weight that is rounded is w * x, x = scale / U,
+    // so the sum takes w + (rounded - w * x) / x (not for keys of tiny scales, whose
+    // rounding is coarse and matters to nobody's output).
     uint32_t pf[NT][KB][2];
     const float inv_unit = kQuant ? 1.f / unit : 1.f;
+    [[maybe_unused]] float back_x[kQuant ? KB : 1][2];
+    if constexpr (kQuant) {
+#pragma unroll
+      for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          vs[j][r] *= inv_unit;
+          back_x[j][r] = vs[j][r] >= 1.f / 64 && vs[j][r] <= 64.f ? rows_rcp(vs[j][r]) : 0.f;
+        }
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float m_use[2];  // nothing seen yet: weights 0, no NaN
@@ -566,23 +585,30 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
       for (int j = 0; j < KB; ++j)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float w[2];
+          float w[2], wx[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             w[e] = fast_exp2(s[nt][j][2 * r + e] - m_use[e]);
-            l_run[nt][e] += w[e];
+            wx[e] = w[e];
             if constexpr (kQuant) {
-              s[nt][j][2 * r + e] = w[e];
-              w[e] *= vs[j][r] * inv_unit;
+              wx[e] *= vs[j][r];
+              if (need_mask && w[e] == 0.f) wx[e] = 0.f;  // a masked key's scale may be anything
             }
           }
+          const uint32_t h = pack_half2(wx[0], wx[1]);
+          const float2 hf = __half22float2(bits_h2(h));
           if constexpr (kQuant) {
-            if (need_mask) {  // a masked key's scale may be anything
-              if (s[nt][j][2 * r] == 0.f) w[0] = 0.f;
-              if (s[nt][j][2 * r + 1] == 0.f) w[1] = 0.f;
+            l_run[nt][0] += w[0];
+            l_run[nt][1] += w[1];
+            if (back_x[j][r] != 0.f) {
+              l_run[nt][0] += (hf.x - wx[0]) * back_x[j][r];
+              l_run[nt][1] += (hf.y - wx[1]) * back_x[j][r];
             }
+          } else {
+            l_run[nt][0] += hf.x;
+            l_run[nt][1] += hf.y;
           }
-          pf[nt][j][r] = rows_movm_t(pack_half2(w[0], w[1]));
+          pf[nt][j][r] = rows_movm_t(h);
         }
     }
 
