@@ -237,12 +237,11 @@ def attention(
     return out
 
 
-def _packed_rows(t: torch.Tensor, what: str, tokens: int, heads: int, hd: int,
-                 device: torch.device) -> int:
+def _packed_rows(t: torch.Tensor, what: str, tokens: int, heads: int, hd: int, index: int) -> int:
     """Checks a packed [T, heads, head_dim] fp16 tensor; its row stride in elements."""
     if t.dtype != torch.float16 or t.shape != (tokens, heads, hd):
         raise ValueError(f"{what} must be float16 [{tokens}, {heads}, {hd}]")
-    if t.device != device:
+    if t.get_device() != index:
         raise ValueError(f"{what} must be on the cache's device")
     st = t.stride()
     if st[2] != 1 or (heads > 1 and st[1] != hd):
@@ -252,11 +251,12 @@ def _packed_rows(t: torch.Tensor, what: str, tokens: int, heads: int, hd: int,
 
 def _paged_device(cache: PagedKVCache, batch: PagedBatch) -> int:
     """Index of the device that both live on."""
-    if not cache.device.type == "cuda":
+    index = cache._index
+    if index is None:
         raise ValueError("the paged cache requires CUDA tensors")
-    if batch.device != cache.device:
+    if batch._index != index:
         raise ValueError("batch and cache must be on one device")
-    return cache.device.index
+    return index
 
 
 def _call_on(index: int, what: str, fn, *args) -> None:
@@ -285,9 +285,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: P
     reference's ``_append_kv_cache`` (torch_transformer_benchmark.py:426-462).
     """
     index = _paged_device(cache, batch)
-    n, heads, hd, dev = batch.num_tokens, cache.kv_heads, cache.head_dim, cache.device
-    ld_k = _packed_rows(k, "k", n, heads, hd, dev)
-    ld_v = _packed_rows(v, "v", n, heads, hd, dev)
+    n, heads, hd = batch.num_tokens, cache.kv_heads, cache.head_dim
+    ld_k = _packed_rows(k, "k", n, heads, hd, index)
+    ld_v = _packed_rows(v, "v", n, heads, hd, index)
     if n:
         _call_on(index, "tfx_paged_append", _lib.load().tfx_paged_append, k.data_ptr(), ld_k,
                  v.data_ptr(), ld_v, cache._ref, batch._ref)
@@ -306,14 +306,14 @@ def paged_read(
     that belong to no sequence are not written. ``out``: write into these two.
     """
     index = _paged_device(cache, batch)
-    n, heads, hd, dev = batch.num_tokens, cache.kv_heads, cache.head_dim, cache.device
+    n, heads, hd = batch.num_tokens, cache.kv_heads, cache.head_dim
     if out is None:
         k, v = cache._half.new_empty(n, heads, hd), cache._half.new_empty(n, heads, hd)
         ld_k = ld_v = heads * hd
     else:
         k, v = out
-        ld_k = _packed_rows(k, "out[0]", n, heads, hd, dev)
-        ld_v = _packed_rows(v, "out[1]", n, heads, hd, dev)
+        ld_k = _packed_rows(k, "out[0]", n, heads, hd, index)
+        ld_v = _packed_rows(v, "out[1]", n, heads, hd, index)
     if n:
         _call_on(index, "tfx_paged_read", _lib.load().tfx_paged_read, cache._ref, batch._ref,
                  k.data_ptr(), ld_k, v.data_ptr(), ld_v)
@@ -342,17 +342,17 @@ def paged_attention(
     torch_transformer_benchmark.py:747-765.
     """
     index = _paged_device(cache, batch)
-    n, hd, dev = batch.num_tokens, cache.head_dim, cache.device
+    n, hd = batch.num_tokens, cache.head_dim
     if q.ndim != 3:
         raise ValueError("q must be [num_tokens, q_heads, head_dim]")
     heads = q.shape[1]
-    ld_q = _packed_rows(q, "q", n, heads, hd, dev)
+    ld_q = _packed_rows(q, "q", n, heads, hd, index)
     if heads == 0 or heads % cache.kv_heads:
         raise ValueError(f"q_heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
     ld_out = heads * hd
     if out is None:
         out = q.new_empty(n, ld_out)
-    elif out.shape != (n, ld_out) or out.dtype != torch.float16 or out.device != dev or \
+    elif out.shape != (n, ld_out) or out.dtype != torch.float16 or out.get_device() != index or \
             (n > 0 and out.stride(1) != 1):
         raise ValueError("out must be float16 [num_tokens, q_heads * head_dim] with contiguous rows")
     elif n > 1:
@@ -367,7 +367,7 @@ def paged_attention(
         # on different streams, and graphs captured apart, never share one.
         ws = cache._half.new_empty(need // 2)
     _call_on(index, "tfx_paged_attention", lib.tfx_paged_attention, q.data_ptr(), ld_q, cache._ref,
-             batch._ref, out.data_ptr(), ld_out, heads, hd ** -0.5 if scale is None else float(scale),
+             batch._ref, out.data_ptr(), ld_out, heads, cache._scale if scale is None else float(scale),
              int(is_causal), None if ws is None else ws.data_ptr(), max(need, 0))
     return out
 

@@ -30,6 +30,9 @@ _CODES = {
 }
 
 
+_GEOMETRIES: dict = {}  # sizes that decide an attention call's workspace -> a small number
+
+
 class _Fixed:
     """Attributes that the C structure (`_ref`, set last) was built from: not to be replaced."""
 
@@ -103,7 +106,9 @@ class PagedKVCache(_Fixed):
             v_scale.data_ptr() if quant else None, _CODES[k.dtype], pages, page_size, heads, hd,
             *strides[:3])
         self._half = k.new_empty(0, dtype=torch.float16)  # outputs are allocated from it
-        self._geometry = (heads, hd, page_size, k.dtype)
+        self._index = k.device.index if k.device.type == "cuda" else None
+        self._scale = hd ** -0.5
+        self._geometry = _GEOMETRIES.setdefault((heads, hd, page_size, k.dtype), len(_GEOMETRIES))
         self._ref = ctypes.byref(self._struct)
 
 
@@ -158,6 +163,7 @@ class PagedBatch(_Fixed):
             raise ValueError("num_tokens, max_query_len and max_kv_len must not be negative")
         self.page_table, self.query_start, self.kv_len = page_table, query_start, kv_len
         self.device, self.num_tokens = page_table.device, num_tokens
+        self._index = page_table.device.index if page_table.device.type == "cuda" else None
         self.max_query_len = num_tokens if max_query_len is None else max_query_len
         self.max_kv_len = (1 << 30) if max_kv_len is None else max_kv_len
         self._struct = _lib.TfxPagedBatch(
@@ -169,7 +175,7 @@ class PagedBatch(_Fixed):
 
     def _workspace_bytes(self, lib, cache: PagedKVCache, q_heads: int) -> int:
         """Workspace of an attention call (a function of sizes only, looked up once)."""
-        key = (q_heads, cache._geometry)
+        key = q_heads << 32 | cache._geometry
         need = self._workspaces.get(key)
         if need is None:
             need = lib.tfx_paged_attention_workspace_bytes(cache._ref, self._ref, q_heads)
