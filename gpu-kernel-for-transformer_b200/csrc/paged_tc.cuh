@@ -180,7 +180,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* k_full = q_full + 1;
   uint64_t* v_full = k_full + S;        // fp16: V loaded
-  uint64_t* v_ready = v_full + S;       // V may be multiplied
+  uint64_t* v_seen = v_full + S;        // fp16: and warp 3 knows
+  uint64_t* v_ready = v_seen + S;       // V may be multiplied
   uint64_t* k_empty = v_ready + S;      // [2][S]
   uint64_t* v_empty = k_empty + 2 * S;  // [2][S]
   constexpr int N = L::kParts, SB = L::kBufs;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + SC);
   volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
   float* scales = reinterpret_cast<float*>(smem + L::kSc);  // [SC][K 64, V 64]
-  static_assert((1 + 7 * S + 2 + 8 * SB + 2 * R + 4 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
+  static_assert((1 + 8 * S + 2 + 8 * SB + 2 * R + 4 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q);
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     for (int s = 0; s < S; ++s) {
       mbar_init(&k_full[s], kQuant ? kPtConvert : 1);
       mbar_init(&v_full[s], 1);
+      mbar_init(&v_seen[s], 1);
       mbar_init(&v_ready[s], kQuant ? kPtConvert : 1);
       for (int x = 0; x < 2; ++x) {
         mbar_init(&k_empty[x * S + s], 1);
@@ -306,6 +308,11 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
                        slot_coord(j, part), hk, page);
           k_issued = j + 1;
           if (!stage_free(v_empty, j)) break;
+          // (a barrier's parity tells only neighbouring phases apart: no load may start
+          // before everyone who watches v_full knows of the one before)
+          if (j >= S && !__all_sync(0xffffffffu, mbar_wait_sleep(&v_seen[st], ((j / S) - 1) & 1, err,
+                                                                 kDevTimeoutEmpty)))
+            break;
           if (lane == 0) mbar_arrive_expect_tx(&v_full[st], L::kTileBytes);
           __syncwarp();
           if (mine)
@@ -324,10 +331,10 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         // ---------------------------------------------- V tiles not all see
         for (int j = 0; j < n_iter; ++j) {
           const int st = j % S, key0 = k_begin + j * L::kKT;
-          // (every phase is waited for: a parity tells only neighbours apart)
           if (!__all_sync(0xffffffffu,
                           mbar_wait_sleep(&v_full[st], (j / S) & 1, err, kDevTimeoutFull)))
             break;
+          if (lane == 0) mbar_arrive(&v_seen[st]);
           if (j < j_partly) continue;
           uint8_t* tile = smem + L::kV + st * L::kTileBytes;
           bool found = false;

@@ -188,3 +188,63 @@ def tolerance(pool, ref, mag, expo):
     # an error d of the exponents moves weights by at most exp(2d) - 1 of themselves
     return 2.0 ** -11 * ref.abs() + 2.0 ** -25 + (per + torch.expm1(2 * on_exp)) * mag + \
         n * 2.0 ** -25 * most
+
+
+def attention_own(pool, q, group, causal=True, scale=None, absent=()):
+    """(out, tol): fp64 result [T, heads * group * hd], and how far fp16 results may be off
+    it, element by element, from the keys that the element's own row sees and nothing else.
+
+    With weights w_j (sum 1), values v_j = s_j c_j (s a value's scale in 8 bits, else 1) and
+    A = sum w_j |v_j| >= |out|:
+      the result is rounded: 2^-11 |out|, 2^-25 where it is subnormal;
+      w_j s_j is rounded to fp16, relative to its largest, R = max w_j s_j, which the kernels'
+      reference does not exceed: 2^-11 of itself, and below 2^-14 R by 2^-25 R, but never by
+      more than itself: 2^-11 A + sum min(w_j s_j, 2^-25 R) |c_j|;
+      the weights' sum may take them as rounded: (2^-11 + n 2^-25 max w) |out|;
+      exponentials are within 2^-13 (the polynomial's 7.5e-5), in both sums;
+      an exponent is off by d_j: hd products summed in fp32 in steps that may truncate (2^-23
+      of the largest sum each) and 8 more steps; 8 bits add log2(s_j), within 2^-22 of itself,
+      40 at most, and a step of exponents up to 40 larger: w_j is off by expm1(d_j) of itself,
+      in both sums;
+      both sums are in fp32, one step of 2^-23 for each 16 keys and 8 more."""
+    hd, quant = pool.hd, pool.dtype != torch.float16
+    scale = hd ** -0.5 if scale is None else scale
+    out = torch.zeros(pool.tokens, pool.heads * group, hd, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    for b, (n, kv) in enumerate(pool.lens):
+        if n == 0 or kv == 0:
+            continue
+        k, v = pool.values(b, 0), pool.values(b, 1)
+        s = torch.ones(kv, pool.heads, dtype=torch.float64)
+        if quant:
+            s = quantise(pool.data[b][1], pool.dtype)[1].double()
+        pos = torch.arange(kv)
+        held = torch.ones(kv, dtype=torch.bool)
+        for ab, page in absent:
+            if ab == b:
+                held &= pos // pool.page != page
+        last = torch.arange(kv - n, kv) if causal else torch.full((n,), kv - 1)
+        seen = (pos[None] <= last[:, None]) & held[None]
+        lo = int(pool.start[b])
+        for h in range(pool.heads * group):
+            x = q[lo:lo + n, h].double()
+            kk, vv, ss = k[:, h // group], v[:, h // group], s[:, h // group]
+            cc = torch.where(ss[:, None] > 0, vv.abs() / ss[:, None], 0.0)
+            e = torch.where(seen, x @ kk.T * scale, -torch.inf)
+            m = e.amax(-1, keepdim=True)
+            w = torch.where(seen, torch.exp(e - torch.where(m == -torch.inf, 0.0, m)), 0.0)
+            total = w.sum(-1, keepdim=True)
+            w = torch.where(total > 0, w / total, 0.0)
+            o, mag = w @ vv, w @ vv.abs()
+            reach = (x.abs() @ kk.abs().T) * scale
+            d = torch.expm1((hd + 8) * 2.0 ** -23 * reach + 2.0 ** -21 +
+                            (40 * (2.0 ** -22 + 2.0 ** -23) if quant else 0.0)) * w
+            y = w * ss[None]
+            lost = torch.minimum(y, 2.0 ** -25 * y.amax(-1, keepdim=True)) @ cc
+            count = seen.sum(-1, keepdim=True)
+            both = 2.0 ** -11 + 2.0 ** -13 + (count / 16 + 8) * 2.0 ** -23
+            out[lo:lo + n, h] = o
+            tol[lo:lo + n, h] = (2.0 ** -11 * o.abs() + 2.0 ** -25 + both * (mag + o.abs()) + lost +
+                                 d @ vv.abs() + d.sum(-1, keepdim=True) * o.abs() +
+                                 count * 2.0 ** -25 * w.amax(-1, keepdim=True) * o.abs())
+    return out.flatten(1), tol.flatten(1)
