@@ -118,6 +118,37 @@ __device__ __forceinline__ uint32_t codes_to_h2(uint32_t x) {
   }
 }
 
+// ------------------------------------------------- scales of cached values
+// 8 bit: the second product takes a key's weight times its value's scale, in fp16,
+// and one scale may be any power of two away from another. So the scale is an
+// exponent, added to the key's score in the log2 domain, and a row's running maximum
+// is that of these sums: what is rounded is relative to the largest weight * scale that
+// the row itself sees, whatever other keys and rows hold. The sum of weights takes each
+// over its scale. (Weights over one unit for all scales of a CTA lost values of 0.01
+// beside a token of 65504, seen or not.) In the tcgen05 kernel this takes as long as
+// the unit did; finding out from the weighted results that a maximum has grown, and
+// doing the keys again, took longer (prompt_parts_grouped_int8: 702, 702 and 758 us).
+//
+// log2 of a scale, at least -40: values of smaller scales (448 * 2^-40 = 4e-10 at most)
+// are nothing in fp16, and a key whose values are zeros (scale 0) needs a weight in
+// the sum still. NaN for a scale that is negative or NaN, and +inf for +inf, so that
+// a row which sees one is NaN.
+__device__ __forceinline__ float value_scale_log2(float scale) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;\n\tmax.NaN.f32 %0, %0, %2;" : "=&f"(y) : "f"(scale), "f"(-40.0f));
+  return y;
+}
+// One over a scale: finite and above 0 whatever it is (a masked key's may be anything).
+__device__ __forceinline__ float value_scale_inverse(float scale) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fminf(fmaxf(scale, 0x1p-40f), 0x1p100f)));
+  return y;
+}
+// A scale that makes its token NaN for the rows that see it.
+__device__ __forceinline__ bool value_scale_bad(float scale) {
+  return !(scale >= 0.f && scale < INFINITY);
+}
+
 // True where either fp16 of the pair is an infinity or NaN.
 __device__ __forceinline__ bool h2_not_finite(uint32_t w) {
   return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;

@@ -23,11 +23,9 @@
 //
 // 8-bit caches are expanded to fp16 in registers, between ldmatrix and the
 // product, without the scales: a key's scale multiplies its row of scores, a
-// value's scale its row of weights, both in fp32. Weights are rounded to fp16
-// for the second product; so that w * scale neither overflows nor loses bits
-// for scales far from 1, it is divided by a unit U, the largest scale of an
-// earlier tile or at least 1/16 of the largest so far, which is put back at
-// the end.
+// value's is an exponent added to them (see value_scale_log2), both in fp32.
+// The weights, with the values' scales in them, are rounded to fp16 for the second
+// product.
 //
 // Fragment orders. An 8x8 ldmatrix block of 16-bit words holds 8 keys x 16
 // codes. Scores: thread (g, t) gets codes 4t..4t+3 of key g and uses (4t, 4t+1)
@@ -40,8 +38,8 @@
 // (0 * inf), so values beyond the sequence are loaded as zeros, and in tiles
 // that some rows of the block see and others do not, non-finite fp16 values
 // (NaN codes) are cleared before the product and added at the end to the rows
-// that see them. (A scale that is not finite stays in its row: it multiplies
-// weights, which are 0 where masked.)
+// that see them. (A scale that is not finite stays in its row: it makes the score
+// NaN, which is replaced where masked.)
 //
 // Keys over CTAs: either ranges of kps keys whose unnormalised results a second
 // kernel joins, or, where 8 ranges are enough, a cluster of CTAs with equal
@@ -102,11 +100,6 @@ __device__ __forceinline__ void rows_mma(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float rows_rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float4 rows_peer4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
@@ -121,7 +114,6 @@ __device__ __forceinline__ float2 rows_peer2(uint32_t addr) {
 }
 
 constexpr float kRowsRescale = 8.0f;  // log2 units, see the file's comment
-constexpr float kRowsUnit = 16.0f;
 
 template <int CODE, int HD, int NT>
 struct RowsCfg {
@@ -343,7 +335,6 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
   float o[NT][DB][4];
   float m_ref[NT][2], l_run[NT][2];
   int lim[NT][2];
-  float unit = 1e-37f;  // U (its reciprocal stays finite)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -473,30 +464,23 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
       }
     }
 
-    // ---- scores in the log2 domain, masked; does a maximum or the unit grow?
-    float vs[kQuant ? KB : 1][2];
-    uint32_t top = 0;
-    if constexpr (kQuant) {
-#pragma unroll
-      for (int j = 0; j < KB; ++j)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          vs[j][r] = sc[KT + j * 16 + g + 8 * r];
-          const uint32_t x = __float_as_uint(vs[j][r]) & 0x7fffffffu;
-          top = max(top, x < 0x7f800000u ? x : 0u);  // non-negative floats order as integers
-        }
-    }
-    bool grow = kQuant && __uint_as_float(top) > unit * kRowsUnit;
+    // ---- scores in the log2 domain, masked; does a maximum grow?
+    [[maybe_unused]] float back_x[kQuant ? KB : 1][2];  // 1 / the values' scales
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float f = a.scale_log2;
-        if constexpr (kQuant) f *= sc[j * 16 + g + 8 * r];
+        float f = a.scale_log2, e = 0.f;
+        if constexpr (kQuant) {
+          f *= sc[j * 16 + g + 8 * r];
+          const float vs = sc[KT + j * 16 + g + 8 * r];
+          e = value_scale_log2(vs);
+          back_x[j][r] = value_scale_inverse(vs);
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          s[nt][j][2 * r] *= f;
-          s[nt][j][2 * r + 1] *= f;
+          s[nt][j][2 * r] = kQuant ? fmaf(s[nt][j][2 * r], f, e) : s[nt][j][2 * r] * f;
+          s[nt][j][2 * r + 1] = kQuant ? fmaf(s[nt][j][2 * r + 1], f, e) : s[nt][j][2 * r + 1] * f;
         }
       }
     }
@@ -515,6 +499,7 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
         }
     }
     float mx[NT][2];
+    bool grow = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -527,14 +512,6 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
     for (int nt = 0; nt < NT; ++nt)
       grow = grow || mx[nt][0] > m_ref[nt][0] + kRowsRescale || mx[nt][1] > m_ref[nt][1] + kRowsRescale;
     if (__any_sync(0xffffffffu, grow)) {
-      float unit_corr = 1.f;
-      if constexpr (kQuant) {
-        const float now = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
-        if (now > unit) {
-          unit_corr = unit / now;
-          unit = now;
-        }
-      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float corr[2];
@@ -547,7 +524,6 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
           corr[e] = m == m_ref[nt][e] ? 1.f : fast_exp2(m_ref[nt][e] - m);  // from -inf: 0
           m_ref[nt][e] = m;
           l_run[nt][e] *= corr[e];
-          corr[e] *= unit_corr;
         }
 #pragma unroll
         for (int n = 0; n < DB; ++n) {
@@ -561,21 +537,10 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
 
     // ---- weights, as the second product's B operand. The sum takes them as rounded
     // to fp16, or a row in which one key has nearly all the weight would carry that
-    // key's rounding in full. 8 bit: the weight that is rounded is w * x, x = scale / U,
-    // so the sum takes w + (rounded - w * x) / x (not for keys of tiny scales, whose
-    // rounding is coarse and matters to nobody's output).
+    // key's rounding in full. 8 bit: what is rounded has the value's scale in it, and a
+    // key of small values may have all the weight: rounded only where that is a normal
+    // fp16 number.
     uint32_t pf[NT][KB][2];
-    const float inv_unit = kQuant ? 1.f / unit : 1.f;
-    [[maybe_unused]] float back_x[kQuant ? KB : 1][2];
-    if constexpr (kQuant) {
-#pragma unroll
-      for (int j = 0; j < KB; ++j)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          vs[j][r] *= inv_unit;
-          back_x[j][r] = vs[j][r] >= 1.f / 64 && vs[j][r] <= 64.f ? rows_rcp(vs[j][r]) : 0.f;
-        }
-    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float m_use[2];  // nothing seen yet: weights 0, no NaN
@@ -585,25 +550,14 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
       for (int j = 0; j < KB; ++j)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float w[2], wx[2];
+          float w[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            w[e] = fast_exp2(s[nt][j][2 * r + e] - m_use[e]);
-            wx[e] = w[e];
-            if constexpr (kQuant) {
-              wx[e] *= vs[j][r];
-              if (need_mask && w[e] == 0.f) wx[e] = 0.f;  // a masked key's scale may be anything
-            }
-          }
-          const uint32_t h = pack_half2(wx[0], wx[1]);
+          for (int e = 0; e < 2; ++e) w[e] = fast_exp2(s[nt][j][2 * r + e] - m_use[e]);
+          const uint32_t h = pack_half2(w[0], w[1]);
           const float2 hf = __half22float2(bits_h2(h));
           if constexpr (kQuant) {
-            l_run[nt][0] += w[0];
-            l_run[nt][1] += w[1];
-            if (back_x[j][r] != 0.f) {
-              l_run[nt][0] += (hf.x - wx[0]) * back_x[j][r];
-              l_run[nt][1] += (hf.y - wx[1]) * back_x[j][r];
-            }
+            l_run[nt][0] += (w[0] < 0x1p-14f ? w[0] : hf.x) * back_x[j][r];
+            l_run[nt][1] += (w[1] < 0x1p-14f ? w[1] : hf.y) * back_x[j][r];
           } else {
             l_run[nt][0] += hf.x;
             l_run[nt][1] += hf.y;
@@ -667,7 +621,6 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
   float2* ml = reinterpret_cast<float2*>(area + C::kMergeRows);    // [warp][8] (max, sum)
   float* cta_o = reinterpret_cast<float*>(area + C::kMergeMl);     // cluster: [kRows][HD]
   float2* cta_ml = reinterpret_cast<float2*>(area + C::kPart);     // cluster: [kRows]
-  const float back = kQuant ? unit : 1.f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     if (r0 + nt * 8 >= rows) break;  // uniform
@@ -681,7 +634,7 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
       for (int n = 0; n < DB; ++n) {
         if constexpr (kQuant) {
           *reinterpret_cast<float2*>(dst + n * 16 + 2 * g) =
-              make_float2(o[nt][n][e] * back, o[nt][n][2 + e] * back);
+              make_float2(o[nt][n][e], o[nt][n][2 + e]);
         } else {
           dst[n * 16 + g] = o[nt][n][e];
           if constexpr (HD >= 16) dst[n * 16 + 8 + g] = o[nt][n][2 + e];

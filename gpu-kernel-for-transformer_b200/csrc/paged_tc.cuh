@@ -32,11 +32,10 @@
 // keys (O alone is 256 columns, Q 64 KB), two of them in S.
 //
 // 8-bit codes are expanded to fp16 exactly, without the scales: a key's scale
-// multiplies its column of scores, a value's its column of weights, in fp32 (as
-// fp16 factors of the tiles they cost as much, in the warps that expand, and
-// five times the error: a key's rounded scale multiplies its whole score).
-// Weights are divided by a unit U, the largest scale so far or at least 1/16 of
-// it, before they are rounded to fp16; U is put back at the end.
+// multiplies its column of scores, a value's is an exponent added to it (see
+// value_scale_log2), in fp32 (as fp16 factors of the tiles they cost as much, in the
+// warps that expand, and five times the error: a key's rounded scale multiplies its
+// whole score).
 //
 // What a row does not see must not reach it, and 0 * inf does: V rows behind
 // the sequence are cleared; in tiles that some rows of the CTA see and others
@@ -78,12 +77,15 @@ struct PtCfg {
   static constexpr int kK = kNT * kQBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
   static constexpr int kR = kV + kStages * kTileBytes;
-  // 8 bit: scales of kSlots parts of tiles, K's times the softmax scale, V's over U
+  // 8 bit: scales of kSlots parts of tiles: K's times the softmax scale, log2 of V's and
+  // one over V's (with two, and slack to align shared memory in, the two query tiles of
+  // head_dim 128 wait for one another: 750 against 702 us, prompt_parts_grouped_int8)
   static constexpr int kSlots = 3;
+  static constexpr int kSlotFloats = 3 * 64;
   static constexpr int kSc = kR + kRaws * kRawBytes;
-  static constexpr int kBar = kSc + (kQuant ? kSlots * 2 * 64 * 4 : 0);
+  static constexpr int kBar = kSc + (kQuant ? kSlots * kSlotFloats * 4 : 0);
   static constexpr int kBarBytes = HD == 64 ? 1024 : 512;
-  static constexpr int kSmem = kBar + kBarBytes + 1024;  // barriers + alignment slack
+  static constexpr int kSmem = kBar + kBarBytes;
   static constexpr bool kSepP = HD == 64 && !kQuant;  // P has its own TMEM columns
   static constexpr int kParts = kSepP || kKT == 64 ? 1 : 2;  // a tile's S in so many parts
   static constexpr int kKeys = kKT / kParts;                 // keys of one
@@ -111,8 +113,6 @@ __device__ __forceinline__ void pt_expand(uint32_t x, uint32_t& lo, uint32_t& hi
   hi = codes_to_h2<CODE, 2, 3>(x);
 }
 
-constexpr float kPtUnit = 16.0f;  // U grows when a scale is more than so many times it
-
 // Adds the non-finite values of keys [lo, hi) to a finished row (rare; out of
 // the kernel's registers): exactly what its weights, all above 0, make of them.
 template <int CODE, int HD>
@@ -122,7 +122,8 @@ __device__ __noinline__ void pt_add_cleared(const Paged& p, int b, int hk, int l
     const int page = paged_page(p, b, key);
     if (page < 0) continue;
     const int64_t at = paged_offset(p, page, key) + hk * p.head_stride;
-    const float vs = CODE != kCodeF16 ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
+    float vs = CODE != kCodeF16 ? p.v_scale[paged_scale_offset(p, page, hk, key)] : 1.f;
+    if (value_scale_bad(vs)) vs = __uint_as_float(0x7fc00000u);
     for (int d = 0; d < HD; ++d) {
       const float y = paged_value<CODE>(p.v, at + d, vs);
       if (isfinite(y)) continue;
@@ -174,9 +175,13 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   const int lim_first = lim_of(i0);
   const int j_partly = max(0, lim_first - k_begin) / L::kKT;
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
+  // (aligned as declared: there is no room for slack, and addresses are constants.
+  // With slack, prompt_part_fp16 549 us and so 494.)
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if ((smem_u32(smem) & 1023u) != 0u) {
+    record_error(err, kDevTimeoutOther);
+    return;
+  }
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
   uint64_t* k_full = q_full + 1;
   uint64_t* v_full = k_full + S;        // fp16: V loaded
@@ -195,11 +200,10 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
   constexpr int SC = L::kSlots;
   uint64_t* c_full = r_empty + R;       // [SC] scales of a part
   uint64_t* c_empty = c_full + SC;      // [2][SC]
-  float2* units = reinterpret_cast<float2*>(c_empty + 2 * SC);  // [SC] (old U / U, U)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(units + SC);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(c_empty + 2 * SC);
   volatile int* cleared = reinterpret_cast<int*>(tmem_slot + 1);
-  float* scales = reinterpret_cast<float*>(smem + L::kSc);  // [SC][K 64, V 64]
-  static_assert((1 + 8 * S + 2 + 8 * SB + 2 * R + 4 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
+  float* scales = reinterpret_cast<float*>(smem + L::kSc);
+  static_assert((1 + 8 * S + 2 + 8 * SB + 2 * R + 3 * SC) * 8 + 8 <= L::kBarBytes, "barrier space");
 
   if (threadIdx.x == 0) {
     prefetch_tmap(&tm_q);
@@ -453,7 +457,6 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         }
       } else {
         // ------------------------------------------------------ the scales
-        float unit = 1e-37f;  // U (its reciprocal stays finite)
         // Lane = two consecutive keys of the part, one part ahead.
         float2 ks, vs;
         auto load_scales = [&](int u) {
@@ -479,25 +482,17 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           }
           if (!__all_sync(0xffffffffu, ok)) break;
           if (k_begin + (u + 1) * L::kKeys > lim_first) {
-            // A scale that is not finite must not leak to rows that do not see it.
-            const bool x = !isfinite(vs.x), y = !isfinite(vs.y);
+            // A scale that is none must not leak to rows that do not see it.
+            const bool x = value_scale_bad(vs.x), y = value_scale_bad(vs.y);
             if (x) vs.x = 0.f;
             if (y) vs.y = 0.f;
             if (x || y) *cleared = 1;
           }
-          const uint32_t vx = __float_as_uint(vs.x) & 0x7fffffffu, vy = __float_as_uint(vs.y) & 0x7fffffffu;
-          const float top = __uint_as_float(__reduce_max_sync(
-              0xffffffffu, max(vx < 0x7f800000u ? vx : 0u, vy < 0x7f800000u ? vy : 0u)));
-          float ratio = 1.f;
-          if (top > unit * kPtUnit) {
-            ratio = unit / top;
-            unit = top;
-          }
-          const float inv = 1.f / unit;
-          float2* dst = reinterpret_cast<float2*>(scales + slot * 128) + lane;
-          dst[0] = make_float2(ks.x * a.scale_log2, ks.y * a.scale_log2);
-          dst[32] = make_float2(vs.x * inv, vs.y * inv);
-          if (lane == 0) units[slot] = make_float2(ratio, unit);
+          float* dst = scales + slot * L::kSlotFloats;
+          reinterpret_cast<float2*>(dst)[lane] = make_float2(ks.x * a.scale_log2, ks.y * a.scale_log2);
+          reinterpret_cast<float2*>(dst + 64)[lane] = make_float2(value_scale_log2(vs.x), value_scale_log2(vs.y));
+          reinterpret_cast<float2*>(dst + 128)[lane] =
+              make_float2(value_scale_inverse(vs.x), value_scale_inverse(vs.y));
           load_scales(u + 1);
           __syncwarp();
           if (lane == 0) mbar_arrive(&c_full[slot]);
@@ -609,7 +604,6 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     const int lim_tile = lim_of(min(first, seq.n - 1));  // smallest of the tile
     float m_ref = -INFINITY;  // -inf: no key seen yet
     float l = 0.f;
-    float unit = 1.f;  // 8 bit: U
     bool ok = true;
     auto wait_o = [&](int u) {  // the product of part u is through
       return mbar_wait(&o_done[x * SB + u % SB], (u / SB) & 1, err, kDevTimeoutAccum);
@@ -748,8 +742,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     };
     // 8 bit: every score and weight meets a scale from shared memory. A lane holds
     // 16 keys of 4 rows (lane / 4 + 8 k: the layout of matrix fragments) and so reads
-    // 16 + 16 scales a part; with 64 keys of one row it read 64 + 64, and that was
-    // what bounded the kernel (128 bytes a clock: 1024 of a part's 3100 clocks).
+    // the scales of 16 keys a part; with 64 keys of one row it read those of 64, and that
+    // was what bounded the kernel (128 bytes a clock: 1024 of a part's 3100 clocks).
     auto softmax_quant = [&](auto with_holes) {
     static_assert(!kQuant || KC == 64, "one fragment load per 16 rows");
     const int quad = lane & 3, sub = lane >> 2;
@@ -778,19 +772,17 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       tmem_ld_16x64(t_s + h * KC, s[0]);
       tmem_ld_16x64(t_s + (16u << 16) + h * KC, s[1]);
       tmem_ld_wait();
-      const float2 un = units[slot];
-      const float ratio = un.x;
-      unit = un.y;
-      const float2* sk = reinterpret_cast<const float2*>(scales + slot * 128) + quad;
+      const float2* sk = reinterpret_cast<const float2*>(scales + slot * L::kSlotFloats) + quad;
+      const float2* sv = reinterpret_cast<const float2*>(scales + slot * L::kSlotFloats + 128) + quad;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {  // scores in the log2 domain from here on
-        const float2 f = sk[4 * c];
-        const uint64_t f2 = f2_pack(f.x, f.y);
+        const float2 f = sk[4 * c], g = sk[32 + 4 * c];
+        const uint64_t f2 = f2_pack(f.x, f.y), e2 = f2_pack(g.x, g.y);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t* at = &s[k >> 1][4 * c + 2 * (k & 1)];
           float y0, y1;
-          f2_unpack(f2_mul(f2_pack(__uint_as_float(at[0]), __uint_as_float(at[1])), f2), y0, y1);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(at[0]), __uint_as_float(at[1])), f2, e2), y0, y1);
           at[0] = __float_as_uint(y0);
           at[1] = __float_as_uint(y1);
         }
@@ -832,8 +824,8 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
         for (int k = 0; k < 4; ++k) mn[k] = fmaxf(mn[k], __shfl_xor_sync(0xffffffffu, mn[k], m));
 #pragma unroll
       for (int k = 0; k < 4; ++k) more |= mn[k] > mr[k] + kPtRescale;
-      bool rescale = u > 0 && ratio != 1.f;  // the same for every row
-      float f = 1.f;                         // of this lane's row of O
+      bool rescale = false;
+      float f = 1.f;  // of this lane's row of O
       if (u == 0) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) mr[k] = mn[k];
@@ -858,18 +850,17 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
       uint32_t pr[2][16];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const float2 w = sk[32 + 4 * c];  // the values' scales over U
+        const float2 w = sv[4 * c];  // one over the values' scales
         const uint64_t w2 = f2_pack(w.x, w.y);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t* at = &s[k >> 1][4 * c + 2 * (k & 1)];
           const uint64_t arg =
               f2_add(f2_pack(__uint_as_float(at[0]), __uint_as_float(at[1])), neg[k]);
-          float a0, a1, e0, e1;
+          float a0, a1;
           f2_unpack(arg, a0, a1);
-          const uint64_t e = f2_pack(fast_exp2(a0), fast_exp2(a1));
-          ls[k] = f2_add(ls[k], e);
-          f2_unpack(f2_mul(e, w2), e0, e1);
+          const float e0 = fast_exp2(a0), e1 = fast_exp2(a1);
+          ls[k] = f2_fma(f2_pack(e0, e1), w2, ls[k]);
           pr[k >> 1][2 * c + (k & 1)] = pack_half2(e0, e1);
         }
       }
@@ -881,7 +872,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
           break;
         }
         tc_fence_after();
-        rescale_o(f * ratio);
+        rescale_o(f);
       }
       tmem_st_16x32(t_p + h * KC, pr[0]);
       tmem_st_16x32(t_p + (16u << 16) + h * KC, pr[1]);
@@ -915,7 +906,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
     if (ok) {
       const bool fix = *cleared != 0;  // the writer arrived before the last product
       const int head = hk * group + row % group;
-      const float inv = l == 0.f ? 0.f : unit / l;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
       const int64_t at = (static_cast<int64_t>(seq.row0 + tok) * (p.kv_heads * group) + head) *
                              a.splits + split;
       __half* dst = a.out + static_cast<int64_t>(seq.row0 + tok) * a.ld_out + head * HD;
@@ -936,8 +927,7 @@ __global__ void __launch_bounds__((PtCfg<CODE, HD>::kThreads), 1)
             float4* d4 = reinterpret_cast<float4*>(a.part_o + at * HD + c);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              d4[i] = make_float4(of[4 * i] * unit, of[4 * i + 1] * unit, of[4 * i + 2] * unit,
-                                  of[4 * i + 3] * unit);
+              d4[i] = make_float4(of[4 * i], of[4 * i + 1], of[4 * i + 2], of[4 * i + 3]);
             if (c == 0) a.part_ml[at] = make_float2(m_ref, l);
           } else {
             uint4* d4 = reinterpret_cast<uint4*>(dst + c);

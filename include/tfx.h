@@ -281,7 +281,8 @@ TFX_API int tfx_forward_kv(const tfx_model* model, const float* x, float* y, int
  */
 
 /* What a cache holds. The 8-bit types have one fp32 scale for each token and
- * head, of K and of V: value = code * scale. */
+ * head, of K and of V: value = code * scale, with scale >= 0. (Attention takes
+ * a scale of V that is negative, infinite or NaN for NaN.) */
 typedef enum tfx_cache_dtype {
   TFX_CACHE_F16 = 0,
   TFX_CACHE_INT8 = 1, /* codes -127..127, scale = max|x| / 127          */
@@ -368,7 +369,9 @@ TFX_API int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* 
  * h / (q_heads / kv_heads). causal: the token at position p sees positions
  * 0..p; otherwise all kv_len of its sequence. A key that a query does not see
  * has no part in its row, whatever its cached values are (NaN included); a
- * row that sees no key is zero.
+ * row that sees no key is zero. What is rounded to fp16 on the way is the
+ * weight of a key (8-bit types: times its value's scale), relative to the
+ * largest that the row itself sees.
  * q, out: fp16, element (row, h, e) at q[row*ld_q + h*head_dim + e], 16-byte
  * aligned, ld a multiple of 8, not overlapping (slices of one row are fine);
  * scale > 0 and finite. q_heads is a multiple of cache->kv_heads. The new tokens'

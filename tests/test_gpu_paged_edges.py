@@ -38,3 +38,79 @@ def test_prompt_parts_behind_long_prefixes(pkg, dev, hd, heads, lens):  # noqa: 
     ref, tol = pr.attention_own(last, q[few], 1)
     err = (outs[0].double().cpu()[few] - ref).abs()
     assert bool((err <= tol).all()), float((err / tol).max())
+
+
+def _attend_own(pkg, dev, pool, group, q, tensors=None):  # noqa: F811
+    cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled() if tensors is None else tensors))
+    return pkg.ops.paged_attention(q.to(dev), cache, _batch(pkg, dev, pool, **_hints(pool))).double().cpu()
+
+
+def _check_own(pool, got, q, group, rows=slice(None)):
+    ref, tol = pr.attention_own(pool, q, group)
+    err = (got - ref).abs()[rows]
+    assert bool((err <= tol[rows]).all()), float((err / tol[rows]).max())
+
+
+SHAPES = {"draft": ([(6, 300), (1, 64), (7, 7), (3, 1025), (2, 31)], 2, 2), "prompt": (CHUNK, 10, 2),
+          "long": ([(2, 9000), (1, 5000)], 1, 4)}
+
+
+@pytest.mark.parametrize("dtype", [F16, I8, E4], ids=_ids)
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("kind", ["later", "earlier", "mixed", "zeros"])
+def test_values_of_very_different_sizes(pkg, dev, dtype, hd, shape, kind):  # noqa: F811
+    """The largest value there is, in a token that a row does not see or gives no weight,
+    beside small ones; tokens of every size; values of zero with nearly all the weight."""
+    lens, heads, group = SHAPES[shape]
+    for small in (1.0, 1e-2, 1e-3) if kind in ("later", "earlier") else (1.0,):
+        pool = pr.Pool(lens, 16, heads, hd, dtype, 51)
+        q = (1.5 * torch.randn(pool.tokens, heads * group, hd, generator=pool.q_gen)).half()
+        q[:, :, 0] = 4.0
+        for (k, v), (n, kv) in zip(pool.data, lens):
+            v *= small
+            if kind == "later" and n > 1:
+                v[-1] = 65504.0
+            if kind == "earlier" and kv > n:
+                v[kv // 3 if kv // 3 < kv - n else 0] = 65504.0
+            if kind == "mixed":
+                size = 10.0 ** (8 * torch.rand(kv, heads, 1, generator=pool.q_gen) - 4)
+                v.copy_((v.float() * size).clamp(-65504, 65504))
+            at = kv // 3 if kv // 3 < kv - n else 0
+            if kind in ("earlier", "zeros") and kv > n:
+                k[at] = 0
+                k[at, :, 0] = (-15.0 if kind == "earlier" else 5.0) * hd ** 0.5  # 60 less, 20 more
+            if kind == "zeros":
+                v[::3] = 0
+                v[at] = 0
+        tensors = pool.filled()
+        if kind == "zeros" and dtype != F16:  # a scale of zero makes any code zero
+            codes, scale = tensors[1].view(torch.uint8), tensors[3].transpose(1, 2)
+            codes[scale == 0] = 0x55
+        got = _attend_own(pkg, dev, pool, group, q, tensors)
+        _check_own(pool, got, q, group)
+
+
+@pytest.mark.parametrize("dtype", [I8, E4], ids=_ids)
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("scale", [-0.01, float("inf"), float("nan")])
+def test_scales_that_are_none(pkg, dev, dtype, hd, shape, scale):  # noqa: F811
+    """A value's scale that is negative, infinite or NaN makes the rows that see it NaN, in its
+    head, and no other."""
+    lens, heads, group = SHAPES[shape]
+    pool = pr.Pool(lens, 16, heads, hd, dtype, 52)
+    q = torch.randn(pool.tokens, heads * group, hd, generator=pool.q_gen).half()
+    tensors, hit = pool.filled(), torch.zeros(pool.tokens, heads * group, dtype=torch.bool)
+    for b, pos in ((0, lens[0][1] - 2), (2 % len(lens), 0)):  # not seen by all; seen by all
+        page, slot = pool.place(b, pos)
+        tensors[3][page, 0, slot] = scale
+        n, kv = lens[b]
+        first = int(pool.start[b]) + max(0, pos - (kv - n))
+        hit[first:int(pool.start[b]) + n, :group] = True
+    got = _attend_own(pkg, dev, pool, group, q, tensors).view(pool.tokens, heads * group, hd)
+    ref, tol = pr.attention_own(pool, q, group)
+    ref, tol = ref.view_as(got), tol.view_as(got)
+    assert bool(torch.isnan(got[hit]).all())
+    err = (got - ref).abs()[~hit]
+    assert bool((err <= tol[~hit]).all()), float((err / tol[~hit]).max())
