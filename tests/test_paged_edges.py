@@ -1,0 +1,33 @@
+"""The paged KV cache on the host, where it is most likely to go wrong: no GPU is needed."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import paged_reference as pr
+
+F16, I8, E4 = torch.float16, torch.int8, torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("dtype", [F16, I8, E4], ids=["fp16", "int8", "e4m3"])
+@pytest.mark.parametrize("lens", [[(4, 300), (1, 64), (7, 7), (3, 1025), (0, 0), (2, 31)],
+                                  [(130, 400), (1, 77), (64, 64), (257, 300), (31, 1000)]],
+                         ids=["draft", "chunk"])
+def test_the_tolerance_can_fail(dtype, lens):
+    """A value of 60000 in one token: results of zero, and results that a token leaks into which
+    the row does not see, are far outside the tolerance of the rows that do not see it."""
+    pool, group = pr.Pool(lens, 16, 2, 64, dtype, 11), 2
+    pool.data[2][1][5, 1, :] = 60000.0
+    q = (1.5 * torch.randn(pool.tokens, 4, 64, generator=pool.q_gen)).half()
+    ref, tol = (x.view(pool.tokens, 4, 64) for x in pr.attention_own(pool, q, group))
+    plain = pr.attention(pool, q, group)[0].view_as(ref)
+    assert bool(((ref - plain).abs() <= 1e-13 * (1 + ref.abs())).all())
+    blind = torch.ones(pool.tokens, 4, dtype=torch.bool)  # (row, head) that do not see it
+    first, n = int(pool.start[2]), lens[2][0]
+    blind[first + 5:first + n, 2:] = False
+    zero = (ref.abs() > tol)[blind]
+    assert float(zero.double().mean()) > 0.97 and bool(zero.any(-1).all())
+    leaky = pr.attention_own(pool, q, group, causal=False)[0].view_as(ref)
+    leaked = ((leaky - ref).abs() > tol)[first:first + 5, 2:]
+    assert bool(leaked.all())
