@@ -208,10 +208,14 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   // (written and read once, in units of a key's time): cutting pays where there
   // are few row blocks.
   const int tokens = group <= 128 ? (hd == 256 ? 1 : 2) * (128 / group) : 1;
-  const int64_t tc_blocks = pairs * ((pl.q + tokens - 1) / tokens);
+  // Row blocks x ranges are the launch's gridDim.z. More row blocks than that (from 65536
+  // new tokens in groups of 65 at head_dim 256) are the mma.sync kernel's.
+  constexpr int64_t kGridZ = 65535;
+  const int64_t tc_row_blocks = (pl.q + tokens - 1) / tokens, tc_blocks = pairs * tc_row_blocks;
   int64_t tc_parts = 1;
   double tc_cost = 0., tc_keys = 0.;
-  for (int64_t n = 1; n <= 16 && (n == 1 || (kv + n - 1) / n >= 1024); ++n) {
+  for (int64_t n = 1; n <= 16 && (n == 1 || ((kv + n - 1) / n >= 1024 && tc_row_blocks * n <= kGridZ));
+       ++n) {
     const double waves = static_cast<double>((tc_blocks * n + num_sms() - 1) / num_sms());
     const double join = n > 1 ? 500. + 1e-5 * 8. * b->num_tokens * q_heads * n * hd : 0.;
     const double cost = waves * ((kv + n - 1) / n + 768) + join;
@@ -227,7 +231,7 @@ Plan make_plan(const tfx_paged_cache* c, const tfx_paged_batch* b, int q_heads) 
   // both kernels at 1 to 64 sequences of 2 000 to 30 000 tokens, 8 heads, 16 to 128
   // rows; e.g. 128 rows, head_dim 64, fp16: 1 x 2 000 26 us tcgen05, 13 mma.sync;
   // 1 x 30 000 40 and 56; 16 x 3 000 47 and 108; 64 x 4 000 210 and 382.
-  pl.tc = hd >= 64 && group <= 128 && pl.rows > tc_rows(hd);
+  pl.tc = hd >= 64 && group <= 128 && pl.rows > tc_rows(hd) && tc_row_blocks <= kGridZ;
   if (pl.tc) {
     const int i = hd == 64 ? 0 : hd == 128 ? 1 : 2;
     constexpr double kTcKey[2][3] = {{11., 13., 16.}, {12.5, 13., 16.}};

@@ -990,8 +990,6 @@ int launch_tc_hd(const tfx_paged_cache* c, const Paged& p, const PagedAttn& a, i
   if (st == TFX_OK) st = make_tmap(&tv, p.v, dt, 4, kd, ks, kb, sw);
   if (st != TFX_OK) return st;
   const int64_t blocks = (tokens + L::kNT * tile_tokens - 1) / (L::kNT * tile_tokens);
-  if (blocks * a.splits_tc > 65535)
-    return fail(TFX_ERR_UNSUPPORTED, "tfx_paged_attention: max_query_len is too long for the grid");
   launch_pdl(kern, dim3(p.kv_heads, p.batch, static_cast<unsigned>(blocks * a.splits_tc)),
              dim3(L::kThreads), L::kSmem, stream, tq, tk, tv, p, a, static_cast<int>(blocks),
              device_error_word());

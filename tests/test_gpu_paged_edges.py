@@ -114,3 +114,20 @@ def test_scales_that_are_none(pkg, dev, dtype, hd, shape, scale):  # noqa: F811
     assert bool(torch.isnan(got[hit]).all())
     err = (got - ref).abs()[~hit]
     assert bool((err <= tol[~hit]).all()), float((err / tol[~hit]).max())
+
+
+def test_more_row_blocks_than_a_grid_has(pkg, dev):  # noqa: F811
+    """65600 new tokens in groups of 65 at head_dim 256, one to a CTA of the tcgen05 kernel.
+    (All but the last 40 have no position, and so see nothing.)"""
+    pool, group, many = pr.Pool([(40, 40), (3, 500)], 16, 1, 256, F16, 61), 65, 65600
+    cache = pkg.PagedKVCache.from_tensors(*pool.on(dev, pool.filled()))
+    table = torch.full((2, 64), -1, dtype=torch.int32)
+    table[:, :pool.table.shape[1]] = pool.table
+    q = torch.randn(pool.tokens, group, 256, generator=pool.q_gen).half()
+    rows = torch.zeros(many + 3, group, 256, dtype=F16, device=dev)
+    rows[many - 40:] = q.to(dev)
+    start = torch.tensor([0, many, many + 3], dtype=torch.int32, device=dev)
+    got = pkg.ops.paged_attention(rows, cache, pkg.PagedBatch(table.to(dev), start, pool.kv.to(dev),
+                                                              many + 3))
+    assert bool((got[:many - 40] == 0).all())
+    _check_own(pool, got[many - 40:].double().cpu(), q, group)
