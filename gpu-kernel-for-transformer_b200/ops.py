@@ -347,8 +347,9 @@ def paged_attention(
         raise ValueError("q must be [num_tokens, q_heads, head_dim]")
     heads = q.shape[1]
     ld_q = _packed_rows(q, "q", n, heads, hd, index)
-    if heads == 0 or heads % cache.kv_heads:
-        raise ValueError(f"q_heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads})")
+    if heads == 0 or heads % cache.kv_heads or heads >= 2 ** 31:
+        raise ValueError(f"q_heads ({heads}) must be a multiple of kv_heads ({cache.kv_heads}), "
+                         "below 2^31")
     ld_out = heads * hd
     if out is None:
         out = q.new_empty(n, ld_out)

@@ -30,6 +30,9 @@ _CODES = {
 }
 
 
+_INT_MAX = 2 ** 31 - 1  # sizes are ints in the C structures, and ctypes cuts what is longer
+
+
 _GEOMETRIES: dict = {}  # sizes that decide an attention call's workspace -> a small number
 
 
@@ -91,6 +94,8 @@ class PagedKVCache(_Fixed):
         strides = _strides(k)
         if strides != _strides(v) or strides[3] != 1:
             raise ValueError("k and v must have the same strides, the last dimension contiguous")
+        if max(pages, page_size, heads) > _INT_MAX:
+            raise ValueError("num_pages, page_size and kv_heads must be below 2^31")
         quant = k.dtype != torch.float16
         for s in (k_scale, v_scale):
             if (s is not None) != quant:
@@ -161,6 +166,8 @@ class PagedBatch(_Fixed):
             raise ValueError("rows of page_table, query_start and kv_len must be contiguous")
         if num_tokens < 0 or (max_query_len or 0) < 0 or (max_kv_len or 0) < 0:
             raise ValueError("num_tokens, max_query_len and max_kv_len must not be negative")
+        if max(b, width, num_tokens) > _INT_MAX:
+            raise ValueError("B, max_pages and num_tokens must be below 2^31")
         self.page_table, self.query_start, self.kv_len = page_table, query_start, kv_len
         self.device, self.num_tokens = page_table.device, num_tokens
         self._index = page_table.device.index if page_table.device.type == "cuda" else None
@@ -168,7 +175,7 @@ class PagedBatch(_Fixed):
         self.max_kv_len = (1 << 30) if max_kv_len is None else max_kv_len
         self._struct = _lib.TfxPagedBatch(
             page_table.data_ptr(), page_table.stride(0) if b > 1 else width, width,
-            query_start.data_ptr(), kv_len.data_ptr(), b, num_tokens, self.max_query_len,
+            query_start.data_ptr(), kv_len.data_ptr(), b, num_tokens, min(self.max_query_len, num_tokens),
             min(self.max_kv_len, 1 << 30))
         self._workspaces = {}
         self._ref = ctypes.byref(self._struct)

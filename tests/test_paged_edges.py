@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import paged_reference as pr
+from conftest import load_package
 
 F16, I8, E4 = torch.float16, torch.int8, torch.float8_e4m3fn
 
@@ -31,3 +32,28 @@ def test_the_tolerance_can_fail(dtype, lens):
     leaky = pr.attention_own(pool, q, group, causal=False)[0].view_as(ref)
     leaked = ((leaky - ref).abs() > tol)[first:first + 5, 2:]
     assert bool(leaked.all())
+
+
+def test_sizes_past_32_bits():
+    """Sizes are ints in the C structures: a longer one is refused, never cut to what is left of
+    it; a bound above num_tokens says as much as num_tokens does."""
+    pkg = load_package()
+    i = lambda *s: torch.empty(s, dtype=torch.int32, device="meta")  # noqa: E731
+    batch = pkg.PagedBatch(i(1, 4), i(2), i(1), 7, max_query_len=2 ** 32)
+    assert batch.max_query_len == 2 ** 32 and batch._struct.max_query_len == 7
+    assert pkg.PagedBatch(i(1, 4), i(2), i(1), 7, max_query_len=3)._struct.max_query_len == 3
+    assert pkg.PagedBatch(i(1, 4), i(2), i(1), 7, max_kv_len=2 ** 33)._struct.max_kv_len == 2 ** 30
+    for args in ((i(1, 4), i(2), i(1), 2 ** 32 + 7), (i(1, 2 ** 32 + 4), i(2), i(1), 7),
+                 (i(2 ** 31, 1), i(2 ** 31 + 1), i(2 ** 31), 7)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            pkg.PagedBatch(*args)
+    pool = torch.empty(2 ** 31, 16, 1, 8, dtype=F16, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        pkg.PagedKVCache.from_tensors(pool, pool)
+    cache = pkg.PagedKVCache(3, 16, 1, 8, F16, "meta")
+    one = pkg.PagedBatch(i(1, 4), i(2), i(1), 1)
+    q = torch.empty(1, 2 ** 32 + 1, 8, dtype=F16, device="meta")
+    for handle in (cache, one):
+        handle.__dict__["_index"] = q.get_device()  # as if they were on a GPU
+    with pytest.raises(ValueError, match="2\\^31"):
+        pkg.ops.paged_attention(q, cache, one)
