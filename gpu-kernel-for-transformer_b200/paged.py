@@ -17,6 +17,7 @@ no allocator here.
 from __future__ import annotations
 
 import ctypes
+import itertools
 from typing import Optional
 
 import torch
@@ -34,6 +35,7 @@ _INT_MAX = 2 ** 31 - 1  # sizes are ints in the C structures, and ctypes cuts wh
 
 
 _GEOMETRIES: dict = {}  # sizes that decide an attention call's workspace -> a small number
+_NUMBERS = itertools.count()  # (their count would give two threads the same one)
 
 
 class _Fixed:
@@ -113,7 +115,7 @@ class PagedKVCache(_Fixed):
         self._half = k.new_empty(0, dtype=torch.float16)  # outputs are allocated from it
         self._index = k.device.index if k.device.type == "cuda" else None
         self._scale = hd ** -0.5
-        self._geometry = _GEOMETRIES.setdefault((heads, hd, page_size, k.dtype), len(_GEOMETRIES))
+        self._geometry = _GEOMETRIES.setdefault((heads, hd, page_size, k.dtype), next(_NUMBERS))
         self._ref = ctypes.byref(self._struct)
 
 

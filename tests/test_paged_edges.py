@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import importlib
+import threading
+
 import pytest
 import torch
 
@@ -57,3 +60,32 @@ def test_sizes_past_32_bits():
         handle.__dict__["_index"] = q.get_device()  # as if they were on a GPU
     with pytest.raises(ValueError, match="2\\^31"):
         pkg.ops.paged_attention(q, cache, one)
+
+
+def test_geometries_made_at_once(monkeypatch):
+    """Two threads that make caches of different sizes at the same moment get different numbers
+    (a batch keeps the workspace sizes of its calls under them)."""
+    pkg = load_package()
+    paged = importlib.import_module(pkg.__name__ + ".paged")
+
+    class Late(dict):  # both have looked before either has written
+        def __init__(self):
+            super().__init__()
+            self.looked = threading.Barrier(2)
+
+        def setdefault(self, key, value):
+            self.looked.wait(20)
+            return super().setdefault(key, value)
+
+    monkeypatch.setattr(paged, "_GEOMETRIES", Late())
+    caches = {}
+
+    def make(hd):
+        caches[hd] = pkg.PagedKVCache(2, 16, 1, hd, F16, "cpu")
+
+    threads = [threading.Thread(target=make, args=(hd,)) for hd in (8, 256)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert caches[8]._geometry != caches[256]._geometry
