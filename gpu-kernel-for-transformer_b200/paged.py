@@ -187,6 +187,7 @@ class PagedBatch(_Fixed):
         key = q_heads << 32 | cache._geometry
         need = self._workspaces.get(key)
         if need is None:
-            need = lib.tfx_paged_attention_workspace_bytes(cache._ref, self._ref, q_heads)
+            with torch.cuda.device(self._index):  # the plan follows the device's SM count
+                need = lib.tfx_paged_attention_workspace_bytes(cache._ref, self._ref, q_heads)
             self._workspaces[key] = need
         return need

@@ -89,3 +89,33 @@ def test_geometries_made_at_once(monkeypatch):
     for t in threads:
         t.join()
     assert caches[8]._geometry != caches[256]._geometry
+
+
+def test_workspace_is_planned_on_the_cache_s_device(monkeypatch):
+    """The plan depends on the device's SM count: it is made where the call will run, whichever
+    device is current."""
+    pkg = load_package()
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    current, planned = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Lib:
+        @staticmethod
+        def tfx_paged_attention_workspace_bytes(cache, batch, heads):
+            planned.append((current[-1], heads))
+            return 512
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    cache, batch = pkg.PagedKVCache(2, 16, 1, 8, F16, "cpu"), pkg.PagedBatch(i(1, 2), i(2), i(1), 1)
+    batch.__dict__["_index"] = 3
+    assert [batch._workspace_bytes(Lib, cache, h) for h in (4, 4, 8)] == [512] * 3
+    assert planned == [(3, 4), (3, 8)]
