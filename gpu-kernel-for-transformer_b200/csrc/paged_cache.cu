@@ -458,7 +458,10 @@ int tfx_paged_append(const tfx_half* k, int64_t ld_k, const tfx_half* v, int64_t
   fail(TFX_OK, "%s", "");
   Paged p;
   const int st = check_copy("tfx_paged_append", k, ld_k, v, ld_v, cache, batch, &p);
-  if (st != TFX_OK || p.num_tokens == 0) return st;
+  if (st != TFX_OK) return st;
+  if (p.k == p.v || (p.k_scale != nullptr && p.k_scale == p.v_scale))
+    return fail(TFX_ERR_INVALID_ARGUMENT, "tfx_paged_append: the cache's k and v are one memory");
+  if (p.num_tokens == 0) return TFX_OK;
   return launch_copy_code(true, cache, reinterpret_cast<__half*>(const_cast<tfx_half*>(k)), ld_k,
                           reinterpret_cast<__half*>(const_cast<tfx_half*>(v)), ld_v, p,
                           reinterpret_cast<cudaStream_t>(stream));

@@ -281,7 +281,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache, batch: P
     arithmetic, ties to even; a row of zeros gets scale 0, a row with an
     infinity or NaN gets scale NaN and reads back as NaN. Tokens whose page is
     outside the pool are dropped. Two tokens of a batch must not share a slot (it
-    would hold parts of both; other slots are not affected). The paged form of the
+    would hold parts of both; other slots are not affected); a cache whose k and v
+    are one tensor is refused, and k and v must not lie in it. The paged form of the
     reference's ``_append_kv_cache`` (torch_transformer_benchmark.py:426-462).
     """
     index = _paged_device(cache, batch)

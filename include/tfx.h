@@ -345,7 +345,8 @@ typedef struct tfx_paged_batch {
  * code = x / scale rounded to nearest, ties to even, as if computed exactly;
  * a row of zeros has scale 0, a row with an infinity or NaN has scale NaN (it
  * reads back as NaN) and codes 0. Two tokens of a batch must not share a slot
- * (it would hold parts of both).
+ * (it would hold parts of both), nor the cache's k and v (or their scales) their
+ * memory, and the rows must not lie in the cache.
  * k, v: fp16, element (row, h, e) at k[row*ld_k + h*head_dim + e]; 16-byte
  * aligned, ld a multiple of 8.
  */

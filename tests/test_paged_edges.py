@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import ctypes
 import importlib
 import threading
 
@@ -119,3 +120,17 @@ def test_workspace_is_planned_on_the_cache_s_device(monkeypatch):
     batch.__dict__["_index"] = 3
     assert [batch._workspace_bytes(Lib, cache, h) for h in (4, 4, 8)] == [512] * 3
     assert planned == [(3, 4), (3, 8)]
+
+
+def test_append_refuses_one_memory_for_keys_and_values():
+    """Every slot would hold parts of both."""
+    pkg = load_package()
+    importlib.import_module(pkg.__name__ + ".build").build()
+    L = pkg._lib
+    lib = L.load()
+    batch = ctypes.byref(L.TfxPagedBatch(256, 6, 6, 320, 384, 3, 0, 4, 80))  # no token: no launch
+    for k, v, ks, vs, want in ((4096, 8192, 512, 1024, 0), (4096, 4096, 512, 1024, L.TFX_ERR_INVALID_ARGUMENT),
+                               (4096, 8192, 512, 512, L.TFX_ERR_INVALID_ARGUMENT)):
+        cache = ctypes.byref(L.TfxPagedCache(k, v, ks, vs, L.TFX_CACHE_INT8, 10, 16, 2, 64, 2048, 64, 1024))
+        assert lib.tfx_paged_append(4096, 128, 8192, 128, cache, batch, None) == want
+        assert lib.tfx_paged_read(cache, batch, 4096, 128, 8192, 128, None) == 0  # reading is fine
