@@ -131,3 +131,61 @@ def test_more_row_blocks_than_a_grid_has(pkg, dev):  # noqa: F811
                                                               many + 3))
     assert bool((got[:many - 40] == 0).all())
     _check_own(pool, got[many - 40:].double().cpu(), q, group)
+
+
+@pytest.mark.parametrize("dtype,hd,heads", [(F16, 32, 3), (F16, 64, 16), (F16, 128, 10), (I8, 64, 16),
+                                            (I8, 128, 10), (E4, 256, 8)], ids=_ids)
+def test_one_capture_for_every_batch(pkg, dev, dtype, hd, heads):  # noqa: F811
+    """Write, attend and read back, captured once: replays on another stream take the lengths,
+    starts, pages and rows that the tensors hold then, whether prompts, running sequences or
+    both; rows of no sequence stay as they were."""
+    group, page, rows, width, pages = 2, 16, 310, 80, 160
+    index = lambda *s: torch.zeros(s, dtype=torch.int32, device=dev)  # noqa: E731
+    table, start, kv = index(3, width), index(4), index(3)
+    cache = pkg.PagedKVCache(pages, page, heads, hd, dtype, dev)
+    batch = pkg.PagedBatch(table, start, kv, rows, max_query_len=300)
+    new = torch.zeros(rows, 2, heads, hd, dtype=F16, device=dev)
+    q = torch.zeros(rows, heads * group, hd, dtype=F16, device=dev)
+    out = torch.zeros(rows, heads * group * hd, dtype=F16, device=dev)
+    back = tuple(torch.zeros(rows, heads, hd, dtype=F16, device=dev) for _ in range(2))
+
+    def step():
+        pkg.ops.paged_append(new[:, 0], new[:, 1], cache, batch)
+        pkg.ops.paged_attention(q, cache, batch, out=out)
+        pkg.ops.paged_read(cache, batch, out=back)
+
+    step()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        step()
+    batches = [[(250, 900), (1, 500), (49, 49)], [(1, 700), (1, 1), (200, 1100)],
+               [(0, 64), (300, 300), (0, 0)], [(1, 33), (1, 1279), (1, 800)], [(8, 40), (0, 7), (3, 1200)]]
+    for seed, lens in enumerate(batches):
+        pool = pr.Pool(lens, page, heads, hd, dtype, 70 + seed)
+        assert pool.pages <= pages
+        torch.cuda.synchronize()
+        for mine, there in zip((cache.k, cache.v, cache.k_scale, cache.v_scale),
+                               pool.on(dev, pool.filled(upto=[m - n for n, m in lens]))):
+            if mine is not None:
+                bits = (lambda t: t.view(torch.uint8)) if mine.dtype in (I8, E4) else (lambda t: t)
+                bits(mine)[:pool.pages].copy_(bits(there))
+        table.fill_(-1)
+        table[:, :min(width, pool.table.shape[1])] = pool.table[:, :width].to(dev)
+        start.copy_(pool.start)
+        kv.copy_(pool.kv)
+        new.zero_()
+        new[:pool.tokens] = torch.stack((pool.rows(0), pool.rows(1)), 1).to(dev)
+        qs = torch.randn(pool.tokens, heads * group, hd, generator=pool.q_gen).half()
+        q[:pool.tokens] = qs.to(dev)
+        for t in (out, *back):
+            t.fill_(-3)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        for t in (out, *back):
+            assert bool((t[pool.tokens:] == -3).all())
+        _check_own(pool, out[:pool.tokens].double().cpu(), qs, group)
+        for which in (0, 1):
+            want = torch.cat([pool.values(b, which)[m - n:] for b, (n, m) in enumerate(lens)])
+            assert torch.equal(back[which][:pool.tokens].cpu(), want.float().half())
