@@ -303,7 +303,7 @@ def paged_read(
 
     The same tokens that ``paged_append`` writes: the last ones of each
     sequence, all of it where query_start counts kv_len tokens. 8-bit caches
-    give code * scale, rounded once. Tokens without a page read as zeros; rows
+    give code * scale in fp32, rounded to fp16. Tokens without a page read as zeros; rows
     that belong to no sequence are not written. ``out``: write into these two.
     """
     index = _paged_device(cache, batch)

@@ -356,7 +356,8 @@ TFX_API int tfx_paged_append(const tfx_half* k, int64_t ld_k, const tfx_half* v,
 
 /*
  * Reads k and v of the same tokens (the last n of each sequence: the whole
- * sequence where n = kv_len) into fp16 rows laid out as tfx_paged_append's.
+ * sequence where n = kv_len) into fp16 rows laid out as tfx_paged_append's; in
+ * the 8-bit types code * scale in fp32, rounded to fp16.
  * Tokens without a page, and positions before 0, read as zeros. k_out and
  * v_out must not overlap (slices of one row are fine).
  */
