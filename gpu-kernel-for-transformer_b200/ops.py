@@ -337,8 +337,8 @@ def paged_attention(
     cache already (``paged_append``). ``is_causal``: a token sees the positions up
     to its own; otherwise all of its sequence. ``scale`` (default
     head_dim ** -0.5) is positive. Returns ctx [num_tokens, q_heads * head_dim]
-    fp16 (``out`` if given); a row that sees no key is zero, rows that belong to
-    no sequence are not written. Single tokens, drafts of a few and chunks of a
+    fp16 (``out`` if given); a row that sees no key, or only keys whose scores
+    are -inf, is zero, rows that belong to no sequence are not written. Single tokens, drafts of a few and chunks of a
     prompt may share a batch. The paged form of the cached attention of
     torch_transformer_benchmark.py:747-765.
     """

@@ -371,7 +371,7 @@ TFX_API int tfx_paged_read(const tfx_paged_cache* cache, const tfx_paged_batch* 
  * h / (q_heads / kv_heads). causal: the token at position p sees positions
  * 0..p; otherwise all kv_len of its sequence. A key that a query does not see
  * has no part in its row, whatever its cached values are (NaN included); a
- * row that sees no key is zero. What is rounded to fp16 on the way is the
+ * row that sees no key, or only keys whose scores are -infinity, is zero. What is rounded to fp16 on the way is the
  * weight of a key (8-bit types: times its value's scale), relative to the
  * largest that the row itself sees.
  * q, out: fp16, element (row, h, e) at q[row*ld_q + h*head_dim + e], 16-byte

@@ -189,3 +189,37 @@ def test_one_capture_for_every_batch(pkg, dev, dtype, hd, heads):  # noqa: F811
         for which in (0, 1):
             want = torch.cat([pool.values(b, which)[m - n:] for b, (n, m) in enumerate(lens)])
             assert torch.equal(back[which][:pool.tokens].cpu(), want.float().half())
+
+
+@pytest.mark.parametrize("hd", [8, 32, 64, 128, 256])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_infinite_scores(pkg, dev, hd, shape):  # noqa: F811
+    """A key whose score is -inf has no weight; a row that sees no other key is zero, as one that
+    sees none. A score of +inf makes its row NaN."""
+    lens, heads, group = SHAPES[shape]
+    pool = pr.Pool(lens, 16, heads, hd, F16, 81)
+    q = torch.randn(pool.tokens, heads * group, hd, generator=pool.q_gen).half()
+    q[:, :, 0] = 2.0
+    tensors = pool.filled()
+    hidden = {0: [0, lens[0][1] // 2, lens[0][1] - 1], len(lens) - 1: range(lens[-1][1])}
+    for b, positions in hidden.items():
+        for pos in positions:
+            page, slot = pool.place(b, pos)
+            tensors[0][page, slot, :, 0] = -float("inf")
+            pool.data[b][0][pos] = 0
+            pool.data[b][0][pos, :, 0] = -60000.0  # no weight left either
+    if len(lens) > 2:  # the first key of a sequence in between
+        page, slot = pool.place(1, 0)
+        tensors[0][page, slot, 0, 0] = float("inf")
+    got = _attend_own(pkg, dev, pool, group, q, tensors).view(pool.tokens, heads * group, hd)
+    ref, tol = (x.view_as(got) for x in pr.attention_own(pool, q, group))
+    fine = torch.ones(pool.tokens, heads * group, dtype=torch.bool)
+    if len(lens) > 2:
+        row = slice(int(pool.start[1]), int(pool.start[2]))
+        assert bool(torch.isnan(got[row, :group]).all())
+        fine[row, :group] = False
+    last = slice(int(pool.start[-2]), pool.tokens)
+    assert bool((got[last] == 0).all())
+    fine[last] = False
+    err = (got - ref).abs()[fine]
+    assert bool((err <= tol[fine]).all()), float((err / tol[fine]).max())
