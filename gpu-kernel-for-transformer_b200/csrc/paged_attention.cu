@@ -5,7 +5,8 @@
 namespace tfx {
 namespace {
 
-// Keys of a split: a multiple of every kernel's round of tiles over its warps.
+// Keys of a split: a multiple of every kernel's tile and of the mma.sync kernel's round of
+// tiles over its warps (but for its six warps at 512-byte rows, 96 keys a round).
 constexpr int kSplitKeys = 256;
 // Sequences with more rows (new tokens x query heads per key/value head) may go
 // to the tcgen05 kernel, whose tiles have 128: the wider the head, the more the

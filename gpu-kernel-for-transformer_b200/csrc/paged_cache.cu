@@ -58,7 +58,8 @@ __device__ __forceinline__ uint32_t row_absmax(const uint4& x) {
 }
 
 // x / 127 or x / 448, correctly rounded: a product with the rounded reciprocal and
-// one correction by the exact remainder (equal to the division for every fp16).
+// one correction by the exact remainder (Markstein's method; equal to the division for
+// every fp16).
 template <int CODE>
 __device__ __forceinline__ float scale_of(float top) {
   constexpr float kTop = CODE == kCodeI8 ? 127.0f : 448.0f, kInv = 1.0f / kTop;

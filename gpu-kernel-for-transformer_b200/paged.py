@@ -35,7 +35,7 @@ _INT_MAX = 2 ** 31 - 1  # sizes are ints in the C structures, and ctypes cuts wh
 
 
 _GEOMETRIES: dict = {}  # sizes that decide an attention call's workspace -> a small number
-_NUMBERS = itertools.count()  # (their count would give two threads the same one)
+_NUMBERS = itertools.count()  # (len() of the table could give two threads the same one)
 
 
 class _Fixed:
