@@ -125,9 +125,8 @@ __device__ __forceinline__ uint32_t codes_to_h2(uint32_t x) {
 // is that of these sums: what is rounded is relative to the largest weight * scale that
 // the row itself sees, whatever other keys and rows hold. The sum of weights takes each
 // over its scale. (Weights over one unit for all scales of a CTA lost values of 0.01
-// beside a token of 65504, seen or not.) In the tcgen05 kernel this takes as long as
-// the unit did; finding out from the weighted results that a maximum has grown, and
-// doing the keys again, took longer (prompt_parts_grouped_int8: 702, 702 and 758 us).
+// beside a token of 65504, seen or not. prompt_parts_grouped_int8: 722 us with the unit,
+// 702 so; 758 with the weights first, done again where one has outgrown the reference.)
 //
 // log2 of a scale, at least -40: values of smaller scales (448 * 2^-40 = 4e-10 at most)
 // are nothing in fp16, and a key whose values are zeros (scale 0) needs a weight in

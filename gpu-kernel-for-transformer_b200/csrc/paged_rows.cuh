@@ -728,7 +728,7 @@ __device__ __forceinline__ void rows_cta(const Paged& p, const PagedAttn& a, con
 // of its sequences are running ones, with few rows in a batch that has many: they
 // take only the blocks of 8 that hold rows. (36 sequences with 1 new token and 4 with
 // 200, 8 heads in groups of 4, head_dim 128, 800 to 8000 keys: one behind the other
-// and with all blocks 282 us, so 193; int8 309 and 216. In kernels that run alone the
+// and with all blocks 282 us, so 184; int8 309 and 190. In kernels that run alone the
 // three bodies cost more, in instructions fetched, than they save: drafts of 2 to 8
 // tokens, 55 against 43 us.)
 template <int CODE, int HD, int NT, bool MIXED>
